@@ -1,0 +1,375 @@
+"""What is measured of the operators of `diffusion-motion-inbetweening_amd/ops.py`: cases, inputs, plain forms and exact values.
+
+Three operators that meet in one transformer block of a denoiser or a text tower:
+
+* ``gated_norm``  the norms around a block with its gate and residual scale, forward and backward
+      r = a x + g * N_post(y),   h = (N_pre(r) w + b) (1 + s) + t
+* ``linear_i8``   a linear layer in 8-bit integers: rows of x get a scale each, C = (q_x q_w^T) s_x s_w + bias, then GELU or a residual
+* ``shared_prefix_attention``  attention of a batch whose sequences share one long prefix of keys and values and have some of their own
+
+``own`` says which side ``run`` takes: the framework's calls, or the plain forms below.
+"""
+import importlib
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+_DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+_BYTES = {"f32": 4, "bf16": 2, "f16": 2}
+
+
+def _ops():
+    return importlib.import_module("diffusion-motion-inbetweening_amd.ops")
+
+
+# ---- cases ------------------------------------------------------------------------------------------------------------
+
+def listed():
+    return [
+        # one token of two sequences between two blocks (a prompt's newest token, or the conditioning token): all latency
+        {"name": "norm_token", "op": "norm", "batch": 2, "seq": 1, "dim": 512, "dtype": "f32", "params": "f32", "post": "none", "pre": "layer",
+         "gate": "sample", "modulate": True, "affine": False, "train": False},
+        # the sampler's own rows: 32 motions under guidance = 64 sequences of 197 tokens of width 512, adaptive norm and gate of each sequence
+        {"name": "norm_denoiser", "op": "norm", "batch": 64, "seq": 197, "dim": 512, "dtype": "f32", "params": "f32", "post": "none", "pre": "layer",
+         "gate": "sample", "modulate": True, "affine": False, "train": False},
+        # a training step's norms of a wide block: both sides normalised, gates of each sample, gradients of everything
+        {"name": "norm_train", "op": "norm", "batch": 16, "seq": 2048, "dim": 2048, "dtype": "bf16", "params": "bf16", "post": "rms", "pre": "rms",
+         "gate": "sample", "modulate": True, "affine": True, "train": True},
+        # odd width and length (rows that no vector load divides), weights held in 32 bits, one gate for all samples
+        {"name": "norm_odd_train", "op": "norm", "batch": 5, "seq": 77, "dim": 515, "dtype": "f16", "params": "f32", "post": "layer", "pre": "layer",
+         "gate": "shared", "modulate": False, "affine": True, "train": True},
+        # a projection of 8 tokens, one of each sequence that is served: the weights' bytes are the time
+        {"name": "i8_decode", "op": "i8", "m": 8, "n": 8192, "k": 4096, "dtype": "bf16", "epi": "bias"},
+        # the denoiser's in_proj: 64 sequences of 197 tokens, 512 -> 1536, in the framework's 32-bit activations
+        {"name": "i8_denoiser", "op": "i8", "m": 12608, "n": 1536, "k": 512, "dtype": "f32", "epi": "bias"},
+        # sizes that no tile divides: 263 motion features into 515 channels with the activation
+        {"name": "i8_odd", "op": "i8", "m": 1001, "n": 515, "k": 263, "dtype": "f16", "epi": "gelu"},
+        # a long prompt through a wide layer: the matrix units are the time
+        {"name": "i8_prompt", "op": "i8", "m": 8192, "n": 8192, "k": 4096, "dtype": "bf16", "epi": "resid"},
+        # the newest token of two sequences behind one 77-token prompt: all latency
+        {"name": "prefix_token", "op": "prefix", "batch": 2, "queries": 1, "heads": 4, "kv_heads": 4, "dim": 128, "prefix": 77, "own": 32, "causal": True,
+         "dtype": "bf16", "lse": False},
+        # a served batch: 64 sequences, a long common prompt, some hundred tokens of their own each, heads in groups of four
+        {"name": "prefix_decode", "op": "prefix", "batch": 64, "queries": 1, "heads": 32, "kv_heads": 8, "dim": 128, "prefix": 8192, "own": 512,
+         "causal": True, "dtype": "bf16", "lse": False},
+        # repetitions of one motion: 197 tokens each look at a common context of 196 frames and at each other, no causal order
+        {"name": "prefix_repeats", "op": "prefix", "batch": 32, "queries": 197, "heads": 4, "kv_heads": 4, "dim": 128, "prefix": 196, "own": 197,
+         "causal": False, "dtype": "f16", "lse": True},
+        # four prompts of 1024 tokens each behind one long common document
+        {"name": "prefix_prompt", "op": "prefix", "batch": 4, "queries": 1024, "heads": 32, "kv_heads": 8, "dim": 128, "prefix": 16384, "own": 1024,
+         "causal": True, "dtype": "bf16", "lse": False},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["norm", "i8", "prefix"])
+    if op == "norm":
+        while True:
+            c = {"op": op, "batch": _log(rng, 1, 256), "seq": _log(rng, 1, 8192), "dim": _log(rng, 16, 8192)}
+            if rng.random() < 0.6:
+                c["dim"] = max(8, c["dim"] // 8 * 8)
+            if 1 << 10 <= c["batch"] * c["seq"] * c["dim"] <= 16 * 2048 * 2048:
+                break
+        c["dtype"] = rng.choice(["f32", "bf16", "bf16", "f16"])
+        c["params"] = rng.choice([c["dtype"], "f32"])
+        c["post"] = rng.choice(["none", "rms", "layer"])
+        c["pre"] = rng.choice(["rms", "layer"])
+        c["gate"] = rng.choice(["none", "shared", "sample"])
+        c["modulate"] = rng.random() < 0.5
+        c["affine"] = rng.random() < 0.7
+        c["train"] = rng.random() < 0.5
+        if c["dtype"] == "f32" and c["batch"] * c["seq"] * c["dim"] > 16 * 2048 * 1024:
+            c["seq"] = (c["seq"] + 1) // 2
+        return c
+    if op == "i8":
+        while True:
+            c = {"op": op, "m": _log(rng, 1, 16384), "n": _log(rng, 32, 16384), "k": _log(rng, 32, 16384)}
+            if rng.random() < 0.6:
+                c["n"], c["k"] = max(32, c["n"] // 32 * 32), max(32, c["k"] // 32 * 32)
+            if c["m"] * c["n"] * c["k"] <= 8192 * 8192 * 4096 and c["m"] * c["n"] <= 8192 * 8192:
+                break
+        c["dtype"] = rng.choice(["f32", "bf16", "bf16", "f16"])
+        c["epi"] = rng.choice(["bias", "gelu", "resid"])
+        return c
+    while True:
+        kind = rng.choice(["token", "token", "few", "many"])
+        c = {"op": op, "batch": _log(rng, 1, 256 if kind == "token" else 64), "queries": {"token": 1, "few": rng.randint(2, 16), "many": _log(rng, 17, 2048)}[kind]}
+        c["kv_heads"] = rng.choice([1, 2, 3, 4, 8, 16])
+        c["heads"] = c["kv_heads"] * rng.choice([1, 1, 2, 4, 5, 8])
+        c["dim"] = rng.choice([64, 128, 128])
+        c["prefix"] = rng.choice([0, _log(rng, 1, 128), _log(rng, 64, 32768), _log(rng, 64, 32768)])
+        c["own"] = max(c["queries"], _log(rng, 1, 4096))
+        if c["heads"] <= 32 and c["batch"] * c["own"] * c["kv_heads"] * c["dim"] <= 1 << 28 \
+                and c["batch"] * c["heads"] * c["queries"] * (c["prefix"] + c["own"]) * c["dim"] <= 4 * 32 * 1024 * 17408 * 128:
+            break
+    c["causal"] = rng.random() < 0.7
+    c["dtype"] = rng.choice(["bf16", "bf16", "f16"])
+    c["lse"] = rng.random() < 0.5
+    return c
+
+
+# ---- inputs -----------------------------------------------------------------------------------------------------------
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(int(seed) * 7919 + 17)
+
+
+def _randn(g, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float32).to(dtype)
+
+
+def _rows_i8(w, pad):
+    """Rows of w in 8 bits with a scale each (largest magnitude = 127), columns padded with zeros to a multiple of `pad`."""
+    amax = w.abs().amax(1)
+    inv = torch.where(amax > 0, torch.full_like(amax, 127.0) / amax, torch.zeros_like(amax))  # one division, rounded once
+    q = torch.zeros(w.shape[0], (w.shape[1] + pad - 1) // pad * pad, dtype=torch.int8, device=w.device)
+    q[:, :w.shape[1]] = torch.round(w * inv[:, None]).to(torch.int8)
+    return q, amax / 127.0
+
+
+def prepare(case, seed):
+    g = _gen(seed)
+    dt = _DT[case["dtype"]]
+    s = {"case": case}
+    if case["op"] == "norm":
+        b, n, d, pt = case["batch"], case["seq"], case["dim"], _DT[case["params"]]
+        s["x"] = _randn(g, b, n, d, dtype=dt) * 2
+        s["y"] = _randn(g, b, n, d, dtype=dt)
+        # one linear layer of the conditioning makes gate, scale and shift side by side: the operators get views with its row stride
+        mod = _randn(g, b, 3 * d, dtype=pt) * 0.3
+        gate, scale, shift = mod[:, :d], mod[:, d:2 * d], mod[:, 2 * d:]
+        s["gate"] = {"none": None, "shared": _randn(g, d, dtype=pt) * 0.5, "sample": gate}[case["gate"]]
+        s["scale"], s["shift"] = (scale, shift) if case["modulate"] else (None, None)
+        one = lambda: (1 + 0.1 * _randn(g, d)).to(pt)  # noqa: E731
+        small = lambda: (0.1 * _randn(g, d)).to(pt)  # noqa: E731
+        s["weight"] = one() if case["affine"] else None
+        s["bias"] = small() if case["affine"] and case["pre"] == "layer" else None
+        s["post_weight"] = one() if case["affine"] and case["post"] != "none" else None
+        s["post_bias"] = small() if case["affine"] and case["post"] == "layer" else None
+        if case["train"]:
+            s["grad_r"] = _randn(g, b, n, d, dtype=dt)
+            s["grad_h"] = _randn(g, b, n, d, dtype=dt)
+        return s
+    if case["op"] == "i8":
+        m, n, k = case["m"], case["n"], case["k"]
+        x = _randn(g, m, k)
+        x *= torch.exp(0.5 * _randn(g, m, 1))          # tokens of different size
+        x[:, :: max(1, k // 3)] *= 6                   # and a few channels that stand out
+        s["x"] = x.to(dt)
+        s["w"], s["w_scale"] = _rows_i8(_randn(g, n, k) / math.sqrt(k), 128)
+        s["bias"] = _randn(g, n)
+        s["resid"] = _randn(g, m, n, dtype=dt) if case["epi"] == "resid" else None
+        return s
+    b, q, h, hk, d, p, o = (case[x] for x in ("batch", "queries", "heads", "kv_heads", "dim", "prefix", "own"))
+    s["q"] = _randn(g, b, q, h, d, dtype=dt)
+    s["prefix_k"], s["prefix_v"] = _randn(g, p, hk, d, dtype=dt), _randn(g, p, hk, d, dtype=dt)
+    s["own_k"], s["own_v"] = _randn(g, b, o, hk, d, dtype=dt), _randn(g, b, o, hk, d, dtype=dt)
+    # sequences are at different places: between a third of the room and all of it (never less than their queries)
+    low = max(q, o // 3)
+    s["own_len"] = (low + torch.floor(torch.rand(b, generator=g, device="cuda") * (o - low + 1))).clamp(max=o).to(torch.int32)
+    return s
+
+
+_GRADS = ("x", "y", "gate", "weight", "bias", "scale", "shift", "post_weight", "post_bias")
+
+
+# ---- one pass ---------------------------------------------------------------------------------------------------------
+
+def run(state):
+    case = state["case"]
+    return {"norm": _run_norm, "i8": _run_i8, "prefix": _run_prefix}[case["op"]](case, state)
+
+
+def _run_norm(case, s):
+    leaves = {k: s[k] for k in _GRADS if s[k] is not None}
+    if case["train"]:
+        leaves = {k: (v.detach() if own else v.detach().float()).requires_grad_() for k, v in leaves.items()}
+    if own:
+        r, h = _ops().gated_norm(leaves["x"], leaves["y"], gate=leaves.get("gate"), residual_scale=1.0, post=case["post"], pre=case["pre"],
+                                 post_weight=leaves.get("post_weight"), post_bias=leaves.get("post_bias"), weight=leaves.get("weight"),
+                                 bias=leaves.get("bias"), scale=leaves.get("scale"), shift=leaves.get("shift"), eps=1e-5)
+    else:
+        r, h = _plain_norm(case, leaves)
+    out = {"r": r.detach().to(s["x"].dtype), "h": h.detach().to(s["x"].dtype)}
+    if case["train"]:
+        grads = torch.autograd.grad((r, h), list(leaves.values()), (s["grad_r"].to(r.dtype), s["grad_h"].to(h.dtype)))
+        out.update({"grad_" + k: g.to(s[k].dtype) for k, g in zip(leaves, grads)})
+    return out
+
+
+def _plain_one_norm(kind, v, weight, bias):
+    if kind == "layer":
+        v = v - v.mean(-1, keepdim=True)
+    if kind != "none":
+        v = v * torch.rsqrt((v * v).mean(-1, keepdim=True) + 1e-5)
+    if weight is not None:
+        v = v * weight
+    return v if bias is None else v + bias
+
+
+def _plain_norm(case, t):
+    row = lambda k: None if t.get(k) is None else (t[k].float() if t[k].dim() == 1 else t[k].float()[:, None, :])  # noqa: E731
+    m = _plain_one_norm(case["post"], t["y"].float(), row("post_weight"), row("post_bias"))
+    if t.get("gate") is not None:
+        m = m * row("gate")
+    r = t["x"].float() + m
+    h = _plain_one_norm(case["pre"], r, row("weight"), row("bias"))
+    if t.get("scale") is not None:
+        h = h * (1 + row("scale")) + row("shift")
+    return r, h
+
+
+def _run_i8(case, s):
+    if own:
+        return _ops().linear_i8(s["x"], s["w"], s["w_scale"], s["bias"], epi=case["epi"], resid=s["resid"])
+    qx, sx = _rows_i8(s["x"].float(), 128)
+    acc = torch.zeros(case["m"], case["n"], dtype=torch.int32, device="cuda")
+    for k in range(0, qx.shape[1], 1024):  # 1024 products of 8-bit integers stay whole numbers in 32-bit floats
+        acc += (qx[:, k:k + 1024].float() @ s["w"][:, k:k + 1024].float().t()).to(torch.int32)
+    c = acc.float() * sx[:, None] * s["w_scale"][None, :] + s["bias"]
+    if case["epi"] == "gelu":
+        c = 0.5 * c * (1 + torch.erf(c * math.sqrt(0.5)))
+    if case["epi"] == "resid":
+        c = c + s["resid"].float()
+    return c.to(s["x"].dtype)
+
+
+def _run_prefix(case, s):
+    if own:
+        out = _ops().shared_prefix_attention(s["q"], s["prefix_k"], s["prefix_v"], s["own_k"], s["own_v"], s["own_len"], causal=case["causal"],
+                                             return_lse=case["lse"])
+        return out if case["lse"] else (out,)
+    b, n, h, d = s["q"].shape
+    p, hk = s["prefix_k"].shape[:2]
+    o, grp = s["own_k"].shape[1], h // hk
+    # rows of one key head: its group's queries, sequence after sequence
+    q = s["q"].float().view(b, n, hk, grp, d).permute(2, 0, 1, 3, 4)                              # [hk, b, n, grp, d]
+    pk, pv = (s[x].float().transpose(0, 1).contiguous() for x in ("prefix_k", "prefix_v"))         # [hk, p, d]
+    ok, ov = (s[x].float().permute(2, 0, 1, 3).contiguous() for x in ("own_k", "own_v"))           # [hk, b, o, d]
+    sp = (q.reshape(hk, b * n * grp, d) @ pk.transpose(1, 2).contiguous()).view(hk, b, n * grp, p)
+    so = q.reshape(hk, b, n * grp, d) @ ok.transpose(2, 3).contiguous()                            # [hk, b, n grp, o]
+    key = torch.arange(o, device="cuda")
+    last = s["own_len"].long()[:, None] - n + torch.arange(n, device="cuda") if case["causal"] else (s["own_len"].long()[:, None] - 1).expand(b, n)
+    seen = (key <= last[:, :, None]).repeat_interleave(grp, 1)                                     # [b, n grp, o]
+    so = torch.where(seen, so, torch.full_like(so, -math.inf))
+    sc = torch.cat([sp, so], -1) / math.sqrt(d)
+    top = sc.amax(-1, keepdim=True)
+    e = torch.exp(sc - torch.where(top == -math.inf, torch.zeros_like(top), top))
+    den = e.sum(-1, keepdim=True)
+    av = (e[..., :p].reshape(hk, b * n * grp, p) @ pv).view(hk, b, n * grp, d) + e[..., p:] @ ov
+    av = torch.where(den > 0, av / den, torch.zeros_like(av))
+    out = av.view(hk, b, n, grp, d).permute(1, 2, 0, 3, 4).reshape(b, n, h, d).to(s["q"].dtype)
+    if not case["lse"]:
+        return (out,)
+    return out, (top + torch.log(den)).view(hk, b, n, grp).permute(1, 0, 3, 2).reshape(b, h, n)
+
+
+# ---- what a pass cannot do without ------------------------------------------------------------------------------------
+
+def work(case):
+    e = _BYTES[case["dtype"]]
+    if case["op"] == "norm":
+        n = case["batch"] * case["seq"] * case["dim"]
+        # x, y -> r, h; in training also their two gradients -> the gradients of x and y
+        return {"bytes": n * e * (8 if case["train"] else 4), "flops": n * (45 if case["train"] else 15)}
+    if case["op"] == "i8":
+        m, n, k = case["m"], case["n"], case["k"]
+        return {"bytes": m * k * e + n * k + m * n * e * (2 if case["epi"] == "resid" else 1) + 8 * n, "flops": 2 * m * n * k}
+    b, q, h, hk, d, p, o = (case[x] for x in ("batch", "queries", "heads", "kv_heads", "dim", "prefix", "own"))
+    mean = (max(q, o // 3) + o) / 2                       # keys of its own that a sequence holds on average
+    seen = mean - (q - 1) / 2 if case["causal"] else mean  # and that one of its queries sees
+    return {"bytes": int(e * d * (2 * b * q * h + 2 * hk * p + 2 * b * mean * hk)), "flops": int(4 * b * q * h * d * (p + seen))}
+
+
+# ---- the operators by their definition, in 64 bits --------------------------------------------------------------------
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"norm": _exact_norm, "i8": _exact_i8, "prefix": _exact_prefix}[case["op"]](case, s)
+
+
+def _exact_norm(case, s):
+    f = lambda k: None if s.get(k) is None else s[k].double()  # noqa: E731
+    b, n, d = s["x"].shape
+    per = lambda v, default: torch.full((1, 1, d), default, dtype=torch.float64, device="cuda") if v is None else v.reshape(-1, 1, d)  # noqa: E731
+    x, y = f("x"), f("y")
+    gate, scale, shift = per(f("gate"), 1.0), per(f("scale"), 0.0), per(f("shift"), 0.0)
+    w, c, wp, cp = per(f("weight"), 1.0), per(f("bias"), 0.0), per(f("post_weight"), 1.0), per(f("post_bias"), 0.0)
+
+    def hat(kind, v):
+        if kind == "none":
+            return v, torch.ones_like(v[..., :1])
+        if kind == "layer":
+            v = v - v.sum(-1, keepdim=True) / d
+        inv = 1 / torch.sqrt((v ** 2).sum(-1, keepdim=True) / d + 1e-5)
+        return v * inv, inv
+
+    def back(kind, dn, nn, inv):
+        if kind == "none":
+            return dn
+        dv = dn - nn * (dn * nn).sum(-1, keepdim=True) / d
+        if kind == "layer":
+            dv = dv - dn.sum(-1, keepdim=True) / d
+        return dv * inv
+
+    ny, iy = hat(case["post"], y)
+    m = ny * wp + cp
+    r = x + gate * m
+    nr, ir = hat(case["pre"], r)
+    u = nr * w + c
+    out = {"r": r, "h": u * (1 + scale) + shift}
+    if not case["train"]:
+        return out
+    gr, gh = f("grad_r"), f("grad_h")
+    du = gh * (1 + scale)
+    dr = gr + back(case["pre"], du * w, nr, ir)
+    dm = dr * gate
+    full = {"x": dr, "y": back(case["post"], dm * wp, ny, iy), "gate": dr * m, "weight": du * nr, "bias": du, "scale": gh * u, "shift": gh,
+            "post_weight": dm * ny, "post_bias": dm}
+    for k in _GRADS:
+        if s[k] is not None:
+            v = full[k]
+            out["grad_" + k] = v if v.shape == s[k].shape else v.sum((0, 1)) if s[k].dim() == 1 else v.sum(1)
+    return out
+
+
+def _exact_i8(case, s):
+    # the definition rounds x / (largest magnitude / 127) as 32-bit floats do: 127 / amax first, then the product, halves to even
+    x = s["x"].float().cpu().numpy()
+    amax = np.abs(x).max(1)
+    with np.errstate(divide="ignore"):
+        inv = np.where(amax > 0, np.float32(127.0) / amax, np.float32(0)).astype(np.float32)
+    q = np.rint(x * inv[:, None])
+    qx = torch.from_numpy(q).cuda().double()
+    c = qx @ s["w"][:, :case["k"]].double().t().contiguous()
+    c = c * (torch.from_numpy(amax).cuda().double() / 127)[:, None] * s["w_scale"].double() + s["bias"].double()
+    if case["epi"] == "gelu":
+        c = c * 0.5 * torch.erfc(-c / math.sqrt(2.0))
+    return c if case["epi"] != "resid" else c + s["resid"].double()
+
+
+def _exact_prefix(case, s):
+    b, n, h, d = s["q"].shape
+    hk, p = s["prefix_k"].shape[1], case["prefix"]
+    lens = s["own_len"].tolist()
+    out = torch.empty(b, n, h, d, dtype=torch.float64, device="cuda")
+    lse = torch.empty(b, h, n, dtype=torch.float64, device="cuda")
+    for i in range(b):
+        at = torch.arange(n, device="cuda") + (lens[i] - n)
+        hide = torch.arange(lens[i], device="cuda")[None, :] > at[:, None] if case["causal"] else torch.zeros(n, lens[i], dtype=torch.bool, device="cuda")
+        hide = torch.cat([torch.zeros(n, p, dtype=torch.bool, device="cuda"), hide], 1)
+        for j in range(h):
+            kh = j // (h // hk)
+            k = torch.cat([s["prefix_k"][:, kh], s["own_k"][i, :lens[i], kh]]).double()
+            v = torch.cat([s["prefix_v"][:, kh], s["own_v"][i, :lens[i], kh]]).double()
+            a = (s["q"][i, :, j].double() @ k.t().contiguous() / math.sqrt(d)).masked_fill(hide, -math.inf)
+            lse[i, j] = torch.logsumexp(a, -1)
+            out[i, :, j] = torch.exp(a - lse[i, j][:, None]).nan_to_num(0.0) @ v
+    return (out, lse) if case["lse"] else (out,)
