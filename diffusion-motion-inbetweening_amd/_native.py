@@ -74,6 +74,32 @@ class Condition(C.Structure):
     ]
 
 
+CMDI_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+CMDI_NORMS = {"none": 0, "rms": 1, "layer": 2}
+
+
+class GatedNormDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "seq", "dim", "dtype", "param_dtype", "post", "pre")] + [
+        ("residual_scale", C.c_float), ("eps", C.c_float), ("d_x", C.c_void_p), ("d_y", C.c_void_p),
+        ("x_stride", C.c_int64 * 2), ("y_stride", C.c_int64 * 2)] + [
+        (n, C.c_void_p) for n in ("d_gate", "d_scale", "d_shift")] + [
+        (n, C.c_int64) for n in ("gate_stride", "scale_stride", "shift_stride")] + [
+        (n, C.c_void_p) for n in ("d_weight", "d_bias", "d_post_weight", "d_post_bias")]
+
+
+class GatedNormGrads(C.Structure):
+    _fields_ = [("d_gr", C.c_void_p), ("d_gh", C.c_void_p), ("gr_stride", C.c_int64 * 2), ("gh_stride", C.c_int64 * 2)] + [
+        (n, C.c_void_p) for n in ("d_gx", "d_gy", "d_ggate", "d_gscale", "d_gshift", "d_gweight", "d_gbias", "d_gpost_weight",
+                                  "d_gpost_bias", "d_work")] + [("work_bytes", C.c_int64)]
+
+
+class PrefixAttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "queries", "heads", "kv_heads", "dim", "prefix", "own_max", "causal", "dtype")] + [
+        ("scale", C.c_float)] + [(n, C.c_void_p) for n in ("d_q", "d_prefix_k", "d_prefix_v", "d_own_k", "d_own_v")] + [
+        ("q_stride", C.c_int64 * 3), ("prefix_k_stride", C.c_int64 * 2), ("prefix_v_stride", C.c_int64 * 2),
+        ("own_k_stride", C.c_int64 * 3), ("own_v_stride", C.c_int64 * 3), ("d_own_len", C.c_void_p)]
+
+
 # name -> (restype, argtypes); mirrors include/condmdi.h one-to-one
 _VP, _I32, _I64, _U64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
 SIGNATURES = {
@@ -112,6 +138,13 @@ SIGNATURES = {
     "cmdi_clip_encode_text": (C.c_int, [_VP, _VP, _I32, _VP, _VP]),
     "cmdi_pack_x6": (C.c_int, [_VP, _VP, _I64, _I32, _VP]),
     "cmdi_gemm_x6": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _I32, _VP]),
+    "cmdi_gated_norm_fwd": (C.c_int, [C.POINTER(GatedNormDesc), _VP, _VP, _VP]),
+    "cmdi_gated_norm_vjp": (C.c_int, [C.POINTER(GatedNormDesc), C.POINTER(GatedNormGrads), _VP]),
+    "cmdi_gated_norm_vjp_workspace": (_I64, [C.POINTER(GatedNormDesc), C.POINTER(GatedNormGrads)]),
+    "cmdi_quant_rows_i8": (C.c_int, [_VP, _I32, _I64, _I32, _I64, _VP, _I32, _VP, _VP]),
+    "cmdi_gemm_i8": (C.c_int, [_VP] * 7 + [_I32] * 3 + [_I64] * 4 + [_I32] * 2 + [_VP]),
+    "cmdi_prefix_attention": (C.c_int, [C.POINTER(PrefixAttentionDesc), _VP, _VP, _VP, _I64, _VP]),
+    "cmdi_prefix_attention_workspace": (_I64, [C.POINTER(PrefixAttentionDesc)]),
     "cmdi_philox4x32_10": (None, [C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
     "cmdi_workspace_bytes": (_I64, [_VP]),
     "cmdi_pipeline_parts": (C.c_int, [_VP]),

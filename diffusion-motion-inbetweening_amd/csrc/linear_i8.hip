@@ -1,0 +1,307 @@
+// The linear layer in 8-bit integers: rows of activations and weights carry a scale each.
+//
+//   s[r] = max_k |x[r, k]| / 127,  q[r, k] = round(x[r, k] * (127 / max)), halves to even        (quantise)
+//   C[m, n] = (sum_k q_x[m, k] q_w[n, k]) s_x[m] s_w[n] + bias[n],  then GELU or + residual        (product)
+//
+// The sum is exact: 8-bit products in 32-bit integers (K <= kI8MaxK keeps them below 2^31), whatever order the tiles and waves
+// add in, so every schedule below gives the same bits; it is rounded to fp32 once, before the scales.
+#include "linear_i8.hpp"
+
+#include <type_traits>
+
+#include "../../include/condmdi.h"
+#include "ops_common.hpp"
+
+namespace cmdi {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// ---- quantise ------------------------------------------------------------------------------------------------------------
+// A team of TEAM lanes takes a row; its first NV vectors of a lane stay in registers between the two passes, the rest of a
+// longer row is read again (from the L2).  Bound by memory: 2 or 4 bytes read, 1 written.
+template <class T, int W, int TEAM>
+__global__ __launch_bounds__(256) void quant_rows_i8_kernel(const QuantRowsArgs a) {
+    constexpr int NV = W == 1 ? 8 : 4, TPB = 256 / TEAM;
+    __shared__ float lds[2][4];
+    const int lane = threadIdx.x % TEAM;
+    const int team = TPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
+    const int64_t row = (int64_t)blockIdx.x * TPB + team;
+    if (row >= a.rows) return;                 // whole waves; never where the team is the block
+    const T* x = static_cast<const T*>(a.x) + row * a.ld;
+    float v[NV][W];
+    float top = 0.f, odd = 0.f;                // odd: NaN once a value is not finite (0 * inf, 0 * nan)
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int e = (c * TEAM + lane) * W;
+        if (e < a.cols) {
+            load_vec<T, W>(x + e, v[c]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[c][i] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < W; ++i) { top = fmaxf(top, fabsf(v[c][i])); odd += 0.f * v[c][i]; }
+    for (int e = (NV * TEAM + lane) * W; e < a.cols; e += TEAM * W) {
+        float u[W];
+        load_vec<T, W>(x + e, u);
+#pragma unroll
+        for (int i = 0; i < W; ++i) { top = fmaxf(top, fabsf(u[i])); odd += 0.f * u[i]; }
+    }
+    top = wave_highest(top);
+    odd = wave_total(odd);
+    if constexpr (TEAM > 64) {
+        if ((threadIdx.x & 63) == 0) { lds[0][threadIdx.x >> 6] = top; lds[1][threadIdx.x >> 6] = odd; }
+        __syncthreads();
+        top = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
+        odd = (lds[1][0] + lds[1][1]) + (lds[1][2] + lds[1][3]);
+    }
+    // below 1e-35 the factor 127 / top would leave the range: such a row is all zeros.  A row with an infinity or a NaN has the
+    // scale NaN, so that its products say so
+    const bool fine = odd == 0.f, some = fine && top >= 1e-35f;
+    const float inv = some ? 127.f / top : 0.f;
+    if (lane == 0) a.scale[row] = fine ? (some ? top / 127.f : 0.f) : __builtin_nanf("");
+    int8_t* q = a.q + row * a.kp;
+    struct alignas(W) Out { int8_t e[W]; };
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int e = (c * TEAM + lane) * W;
+        if (e < a.kp) {                        // columns behind `cols` hold 0: the padding
+            Out o;
+#pragma unroll
+            for (int i = 0; i < W; ++i) o.e[i] = (int8_t)(fine ? (int)rintf(v[c][i] * inv) : 0);
+            *reinterpret_cast<Out*>(q + e) = o;
+        }
+    }
+    for (int e = (NV * TEAM + lane) * W; e < a.kp; e += TEAM * W) {
+        float u[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) u[i] = 0.f;
+        if (e < a.cols) load_vec<T, W>(x + e, u);
+        Out o;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o.e[i] = (int8_t)(fine ? (int)rintf(u[i] * inv) : 0);
+        *reinterpret_cast<Out*>(q + e) = o;
+    }
+}
+
+// ---- product -------------------------------------------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ void finish(const GemmI8Args& p, int row, int col, int acc, float sa, float sw, float bias) {
+    float v = (float)acc * sa * sw + bias;
+    if (p.epi == 1) v = gelu_erf(v);
+    if (p.epi == 3) v += Elem<T>::up(static_cast<const T*>(p.resid)[(int64_t)row * p.ldr + col]);
+    static_cast<T*>(p.c)[(int64_t)row * p.ldc + col] = Elem<T>::down(v);
+}
+
+// Tiles: WM x WN waves, a wave owns TM x TN fragments of 32 x 32 (v_mfma_i32_32x32x32_i8).  K runs in steps of 128 columns
+// through two LDS stages filled by LDS-DMA: the next step's requests are out while this one is multiplied, one barrier a step.
+// A row of a stage is 128 bytes = eight 16-byte slots; slot t of row r holds columns 16 (t ^ (r & 7)): the 8 rows of a wave's
+// read phase hit 8 different slots.  Rows behind the matrix repeat its last one and are not stored.
+template <class T, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmI8Args p, int tiles_m, int tiles_n) {
+    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
+    constexpr int PIECES = (BM + BN) / 8 / NW;       // 1-KiB pieces (8 rows) a wave brings per step
+    static_assert((BM / 8) % NW == 0 && (BN / 8) % NW == 0, "a piece lies in one operand for every wave");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN, l31 = lane & 31, hi = lane >> 5;
+    // neighbouring tiles of an XCD share operand panels in its L2: 8 rows of tiles, then the next column
+    const int id = xcd_remap(blockIdx.x, tiles_m * tiles_n);
+    const int band = id / (8 * tiles_n), in = id % (8 * tiles_n);
+    const int bh = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+    const int m0 = (band * 8 + in % bh) * BM, n0 = (in / bh) * BN;
+
+    unsigned off[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int pc = i * NW + wave;                // pieces 0 .. BM/8 - 1: A, then W
+        const bool is_a = pc < BM / 8;
+        const int r = (is_a ? pc : pc - BM / 8) * 8 + (lane >> 3);
+        const int last = (is_a ? p.m - m0 : p.n - n0) - 1;
+        const int rr = r < last ? r : last;
+        off[i] = (unsigned)(rr * (is_a ? p.lda : p.ldw)) + (((lane & 7) ^ (r & 7)) << 4);
+    }
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.a + (int64_t)m0 * p.lda), 0, 0x7fffffff, 0x00020000);
+    const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.w + (int64_t)n0 * p.ldw), 0, 0x7fffffff, 0x00020000);
+    auto bring = [&](int step, int stage) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int pc = i * NW + wave;
+            char* dst = lds + stage * STAGE + pc * 1024;
+            if (i * NW < BM / 8)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)dst, 16, (int)off[i], step * 128, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)dst, 16, (int)off[i], step * 128, 0, 0);
+        }
+    };
+
+    i32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+
+    const int steps = p.k / 128;
+    bring(0, 0);
+    const int arow = (wm * TM * 32 + l31) * 128, brow = (BM + wn * TN * 32 + l31) * 128, sw = l31 & 7;
+    for (int s = 0; s < steps; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                             // step s is in LDS, and every wave has left step s - 1
+        if (s + 1 < steps) bring(s + 1, (s + 1) & 1);
+        const char* st = lds + (s & 1) * STAGE;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const int slot = ((ks * 2 + hi) ^ sw) << 4;
+            i32x4 fa[TM], fb[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const i32x4*>(st + arow + i * 32 * 128 + slot);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const i32x4*>(st + brow + j * 32 * 128 + slot);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int col = n0 + (wn * TN + j) * 32 + l31;
+        if (col >= p.n) continue;
+        const float ws = p.w_scale[col], bias = p.bias ? p.bias[col] : 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = m0 + (wm * TM + i) * 32 + mfma32_row(r, lane);
+                if (row < p.m) finish<T>(p, row, col, acc[i][j][r], p.a_scale[row], ws, bias);
+            }
+    }
+}
+
+// Few rows (M <= 16 MT): the weights' bytes are the time.  A block takes 16 weight rows, its 4 waves split K and read their
+// weights straight into the registers of v_mfma_i32_16x16x64_i8 (weights as its rows, activations as its columns), 8 steps of 64
+// columns in flight; the waves' sums join through LDS.
+template <class T, int MT>
+__global__ __launch_bounds__(256) void gemm_i8_rows_kernel(const GemmI8Args p) {
+    __shared__ i32x4 part[4][MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l15 = lane & 15, kg = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int wr = n0 + l15 < p.n ? n0 + l15 : p.n - 1;
+    const int8_t* w = p.w + (int64_t)wr * p.ldw + kg * 16;
+    const int8_t* a[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int r = t * 16 + l15 < p.m ? t * 16 + l15 : p.m - 1;
+        a[t] = p.a + (int64_t)r * p.lda + kg * 16;
+    }
+    i32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+    const int steps = p.k / 64;
+    constexpr int U = 8;
+    for (int s0 = wave * U; s0 < steps; s0 += 4 * U) {
+        i32x4 fw[U];
+        const int n = steps - s0 < U ? steps - s0 : U;
+        if (n == U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) fw[u] = *reinterpret_cast<const i32x4*>(w + (int64_t)(s0 + u) * 64);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const i32x4 fa = *reinterpret_cast<const i32x4*>(a[t] + (int64_t)(s0 + u) * 64);
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fa, acc[t], 0, 0, 0);
+                }
+        } else {
+            for (int u = 0; u < n; ++u) {
+                const i32x4 f = *reinterpret_cast<const i32x4*>(w + (int64_t)(s0 + u) * 64);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const i32x4 fa = *reinterpret_cast<const i32x4*>(a[t] + (int64_t)(s0 + u) * 64);
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, fa, acc[t], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    // lane of fragment t: activation row 16 t + l15, weight rows 4 kg + r
+    for (int t = wave; t < MT; t += 4) {
+        const i32x4 s = part[0][t][lane] + part[1][t][lane] + part[2][t][lane] + part[3][t][lane];
+        const int row = t * 16 + l15;
+        if (row >= p.m) continue;
+        const float sa = p.a_scale[row];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int col = n0 + 4 * kg + r;
+            if (col < p.n) finish<T>(p, row, col, s[r], sa, p.w_scale[col], p.bias ? p.bias[col] : 0.f);
+        }
+    }
+}
+
+template <class T, int TM, int TN, int WM, int WN>
+hipError_t launch_tile(const GemmI8Args& p, hipStream_t stream) {
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, LDS = 2 * (BM + BN) * 128;
+    auto* kernel = gemm_i8_tile_kernel<T, TM, TN, WM, WN>;
+    if (LDS > 64 * 1024) {
+        static PerDevice<int> set;
+        int& done = set.get();
+        if (!done) {
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+            if (e != hipSuccess) return e;
+            done = 1;
+        }
+    }
+    const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
+    kernel<<<dim3((unsigned)tm * tn), dim3(64 * WM * WN), LDS, stream>>>(p, tm, tn);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_typed(const GemmI8Args& p, hipStream_t stream) {
+    const dim3 g16((unsigned)((p.n + 15) / 16));
+    if (p.m <= 16) { gemm_i8_rows_kernel<T, 1><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
+    if (p.m <= 32) { gemm_i8_rows_kernel<T, 2><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
+    if (p.m <= 64) { gemm_i8_rows_kernel<T, 4><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
+    const int cus = device_cu_count();
+    auto tiles = [&](int bm, int bn) { return (int64_t)((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn); };
+    if (tiles(256, 256) >= cus) return launch_tile<T, 4, 2, 2, 4>(p, stream);
+    if (tiles(128, 128) >= cus) return launch_tile<T, 2, 2, 2, 2>(p, stream);
+    return launch_tile<T, 1, 1, 2, 2>(p, stream);
+}
+
+}  // namespace
+
+hipError_t launch_quant_rows_i8(const QuantRowsArgs& a, hipStream_t stream) {
+    auto go = [&](auto t, auto w) {
+        using T = decltype(t);
+        constexpr int W = decltype(w)::value;
+        if (a.cols <= 2048) quant_rows_i8_kernel<T, W, 64><<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, stream>>>(a);
+        else quant_rows_i8_kernel<T, W, 256><<<dim3((unsigned)a.rows), 256, 0, stream>>>(a);
+        return hipGetLastError();
+    };
+    switch (a.dtype) {
+        case CMDI_DT_F32: return a.vec ? go(float(), std::integral_constant<int, 4>()) : go(float(), std::integral_constant<int, 1>());
+        case CMDI_DT_BF16: return a.vec ? go(Bf16(), std::integral_constant<int, 8>()) : go(Bf16(), std::integral_constant<int, 1>());
+        default: return a.vec ? go(_Float16(), std::integral_constant<int, 8>()) : go(_Float16(), std::integral_constant<int, 1>());
+    }
+}
+
+hipError_t launch_gemm_i8(const GemmI8Args& p, hipStream_t stream) {
+    switch (p.dtype) {
+        case CMDI_DT_F32: return launch_typed<float>(p, stream);
+        case CMDI_DT_BF16: return launch_typed<Bf16>(p, stream);
+        default: return launch_typed<_Float16>(p, stream);
+    }
+}
+
+}  // namespace cmdi

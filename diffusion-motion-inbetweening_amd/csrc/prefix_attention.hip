@@ -1,0 +1,451 @@
+// Attention of a batch whose sequences share one long prefix of keys and values and have some of their own:
+//
+//   out[b, i, h] = softmax_j (scale q . k_j) v_j   over the prefix's keys and the own keys j < visible(b, i)
+//   visible = own_len[b], or with causal order own_len[b] - queries + i + 1 (the queries are the sequence's newest tokens)
+//
+// A pass over the keys keeps a running maximum and sum per row (fp32, base-2 exponentials):
+//   m' = max(m, max s),  l' = l 2^(m - m') + sum 2^(s - m'),  o' = o 2^(m - m') + sum 2^(s - m') v
+// and partial results over different keys join the same way, so the prefix can be read ONCE for all sequences: their rows
+// (sequence, query, head of the key head's group) are packed into tiles that run over a chunk of the prefix; each sequence's own
+// keys are a second set of items; a last kernel joins a row's partial results through their log-sums.  Few queries: bound by the
+// keys' bytes, prefix read once instead of once a sequence.  Many queries: a tile of one sequence's rows runs over prefix and own
+// keys in one loop, bound by the matrix units.
+//
+// Matrix instructions: v_mfma_f32_16x16x32 (bf16 / f16 operands, fp32 sums).  S^T = K Q^T puts a row of Q into a lane column,
+// so maximum and sum stay in the lane but for two exchanges, and S^T's accumulators ARE the operand of O^T += V^T P^T: lane group
+// g holds keys 4 g + r and 16 + 4 g + r of a 32-key block, and the transposed LDS reads (ds_read_b64_tr_b16) fetch V in that same
+// order.  P is rounded to the operands' 16 bits (half a step relative, as the matrix unit asks), its sum l is taken before that.
+#include "prefix_attention.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+#include "../../include/condmdi.h"
+#include "ops_common.hpp"
+
+namespace cmdi {
+namespace {
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+template <class T> struct Mma;
+template <> struct Mma<Bf16> {
+    static __device__ __forceinline__ f32x4 mul(s8 a, s8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ unsigned pack(float x, float y) { return __builtin_bit_cast(unsigned, b2{(__bf16)x, (__bf16)y}); }
+};
+template <> struct Mma<_Float16> {
+    static __device__ __forceinline__ f32x4 mul(s8 a, s8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ unsigned pack(float x, float y) { return __builtin_bit_cast(unsigned, h2{(_Float16)x, (_Float16)y}); }
+};
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+
+// A key row of a stage is DIM elements in 16-byte slots; slot t of key k is stored at t ^ swz(k).  K's reads (16 keys, one slot)
+// and V's transposed reads (8 keys, two neighbouring slots) both spread over all 64 banks.
+template <int DIM>
+__device__ __forceinline__ int swz(int k) {
+    return DIM == 128 ? ((k & 7) << 1) | ((k >> 3) & 1) : (((k >> 1) & 3) << 1) | ((k >> 3) & 1);
+}
+
+// One item: a tile of rows over a chunk of keys.  BYWAVE: at most 16 rows, every wave takes every fourth 32-key tile through its
+// own LDS ring, and the waves join at the end; otherwise wave w owns rows [16 RT w, +16 RT) and all share 64-key stages.
+template <class T, int DIM, int RT, bool BYWAVE>
+__global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(const PrefixAttnArgs a, const PrefixAttnLaunch L, int slots) {
+    constexpr int KT = BYWAVE ? 32 : 64, ROWB = DIM * 2, TILE = KT * ROWB, STAGE = 2 * TILE, KB = KT / 16, DB = DIM / 16, DS = DIM / 32;
+    constexpr int SLOTS = DIM / 8, RPP = 64 / SLOTS;              // 16-byte slots of a key row; key rows of a 1-KiB piece
+    constexpr int PIECES = KT / RPP / (BYWAVE ? 1 : 4);           // pieces of K (and as many of V) a wave brings per stage
+    static_assert(!BYWAVE || RT == 1, "");
+    extern __shared__ __attribute__((aligned(16))) char lds_all[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l15 = lane & 15, g = lane >> 4;
+    char* lds = lds_all + (BYWAVE ? wave * 2 * STAGE : 0);
+
+    // ---- which item ----
+    const int grp = a.heads / a.kv_heads;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int tile = id % L.tiles, rest = id / L.tiles;
+    const int chunk = rest % L.chunks, bh = rest / L.chunks;
+    const int hk = bh % a.kv_heads, b0 = bh / a.kv_heads;         // packed: b0 = 0, the sample comes from the row
+    const int n_rows = (L.packed ? a.batch : 1) * a.queries * grp;
+    constexpr int BM = BYWAVE ? 16 : 64 * RT;
+
+    // ---- rows of this lane: column l15 of each of the wave's RT row tiles ----
+    int row_b[RT], row_i[RT], row_h[RT], vis[RT];
+    bool row_ok[RT];
+    int vis_top = 0, vis_low = 0x7fffffff;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        int r = tile * BM + (BYWAVE ? 0 : wave * RT * 16) + t * 16 + l15;
+        row_ok[t] = r < n_rows;
+        if (!row_ok[t]) r = n_rows - 1;
+        row_h[t] = hk * grp + r % grp;
+        const int q = r / grp;
+        row_i[t] = q % a.queries;
+        row_b[t] = L.packed ? q / a.queries : b0;
+        vis[t] = 0;
+    }
+    int own_tiles_end = 0;                                        // own keys this block has to look at
+    if (L.k_end > a.prefix) {                                     // (never for packed rows)
+        int len = a.own_len ? a.own_len[b0] : a.own_max;
+        len = len < 0 ? 0 : len > a.own_max ? a.own_max : len;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            int v = a.causal ? len - a.queries + row_i[t] + 1 : len;
+            vis[t] = v < 0 ? 0 : v > len ? len : v;
+        }
+        const int last = (tile + 1) * BM < n_rows ? (tile + 1) * BM - 1 : n_rows - 1;
+        int v = a.causal ? len - a.queries + last / grp + 1 : len;
+        vis_top = v < 0 ? 0 : v > len ? len : v;
+        v = a.causal ? len - a.queries + (tile * BM) / grp + 1 : len;
+        vis_low = v < 0 ? 0 : v > len ? len : v;
+        own_tiles_end = vis_top;
+    }
+    const int c0 = L.k_begin + chunk * L.chunk;
+    const int c1 = c0 + L.chunk < L.k_end ? c0 + L.chunk : L.k_end;
+    const int p0 = c0, p1 = c1 < a.prefix ? c1 : a.prefix;        // prefix keys [p0, p1)
+    const int o0 = c0 > a.prefix ? c0 - a.prefix : 0;             // own keys [o0, o1)
+    const int o1 = c1 - a.prefix < own_tiles_end ? c1 - a.prefix : own_tiles_end;
+    const int np = p1 > p0 ? (p1 - p0 + KT - 1) / KT : 0;
+    const int no = o1 > o0 ? (o1 - o0 + KT - 1) / KT : 0;
+    const int stages = np + no;
+
+    // ---- bringing a stage: LDS-DMA through a descriptor that ends with the stage's last valid key, so that keys behind it read
+    // as zeros whatever lies there ----
+    const char* pk = static_cast<const char*>(a.pk) + (int64_t)hk * a.pk_hs * 2;
+    const char* pv = static_cast<const char*>(a.pv) + (int64_t)hk * a.pv_hs * 2;
+    const char* ok = static_cast<const char*>(a.ok) + ((int64_t)b0 * a.ok_bs + (int64_t)hk * a.ok_hs) * 2;
+    const char* ov = static_cast<const char*>(a.ov) + ((int64_t)b0 * a.ov_bs + (int64_t)hk * a.ov_hs) * 2;
+    const int w4 = BYWAVE ? 0 : wave;
+    auto bring = [&](int s, int slot) {
+        const bool own = s >= np;
+        const int k0 = own ? o0 + (s - np) * KT : p0 + s * KT;
+        const int left = (own ? o1 : p1) - k0;
+        const int valid = left < KT ? left : KT;
+        const int64_t ks = own ? a.ok_ss : a.pk_ss, vs = own ? a.ov_ss : a.pv_ss;
+        const char* kb = (own ? ok : pk) + (int64_t)k0 * ks * 2;
+        const char* vb = (own ? ov : pv) + (int64_t)k0 * vs * 2;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kb), 0, (int)((valid - 1) * ks * 2 + ROWB), 0x00020000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vb), 0, (int)((valid - 1) * vs * 2 + ROWB), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int pc = i + w4 * PIECES;
+            const int key = pc * RPP + lane / SLOTS;
+            const int t = (lane % SLOTS) ^ swz<DIM>(key);
+            char* dst = lds + slot * STAGE + pc * 1024;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)dst, 16, (int)(key * (int)ks * 2 + t * 16), 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(dst + TILE), 16, (int)(key * (int)vs * 2 + t * 16), 0, 0, 0);
+        }
+    };
+    const int first = BYWAVE ? wave : 0, step = BYWAVE ? 4 : 1;
+    if (first < stages) bring(first, 0);
+
+    // ---- Q as the B operand: lane (row l15, dims 32 s + 8 g ..) ----
+    s8 q[RT][DS];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const short* p = static_cast<const short*>(a.q) + row_b[t] * a.q_bs + row_i[t] * a.q_ss + row_h[t] * a.q_hs + 8 * g;
+#pragma unroll
+        for (int s = 0; s < DS; ++s) q[t][s] = *reinterpret_cast<const s8*>(p + 32 * s);
+    }
+
+    f32x4 o[RT][DB];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float scale2 = a.scale * kLog2e;
+    const int kswz = swz<DIM>(l15), krow = l15 * ROWB;            // K: key l15 of a 16-key block
+    const int vkey = 4 * g + (l15 >> 2);                          // V: this lane's source key of a 16-key block
+    const int vrow = TILE + vkey * ROWB + (l15 & 1) * 8, vsl = ((l15 & 3) >> 1) ^ swz<DIM>(vkey);
+
+    int slot = 0;
+    for (int s = first; s < stages; s += step) {
+        if constexpr (BYWAVE) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the other slot's reads are done
+            if (s + step < stages) {
+                bring(s + step, slot ^ 1);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PIECES) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();                                      // stage s is in LDS, and every wave has left stage s - 1
+            if (s + 1 < stages) bring(s + 1, slot ^ 1);
+        }
+        const char* st = lds + slot * STAGE;
+        slot ^= 1;
+        // ---- scores ----
+        f32x4 sc[KB][RT];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) sc[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+                const s8 kf = *reinterpret_cast<const s8*>(st + kb * 16 * ROWB + krow + (((4 * d + g) ^ kswz) << 4));
+#pragma unroll
+                for (int t = 0; t < RT; ++t) sc[kb][t] = Mma<T>::mul(kf, q[t][d], sc[kb][t]);
+            }
+        }
+        // ---- masks: keys behind the chunk's end, own keys a row does not see ----
+        const bool own = s >= np;
+        const int k0 = own ? o0 + (s - np) * KT : p0 + s * KT;
+        const int end = own ? o1 : p1;
+        if (k0 + KT > end || (own && k0 + KT > vis_low)) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const int lim = own && vis[t] < end ? vis[t] : end;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (k0 + kb * 16 + 4 * g + r >= lim) sc[kb][t][r] = -INFINITY;
+            }
+        }
+        // ---- running maximum and sum; P^T as the B operand of each 32-key block ----
+        s8 p[KB / 2][RT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float top = sc[0][t][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[kb][t][r]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(m[t], top * scale2);
+            const float base = mn == -INFINITY ? 0.f : mn;        // nothing seen yet: every p is 2^-inf = 0
+            if (__any(mn > m[t])) {
+                const float k = exp2f(m[t] - base);
+                l[t] *= k;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[t][d] *= k;
+            }
+            m[t] = mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb += 2) {
+                float e[8];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][t][r], scale2, -base));
+                    e[4 + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb + 1][t][r], scale2, -base));
+                }
+                sum += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                struct { unsigned u[4]; } pk4;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) pk4.u[r] = Mma<T>::pack(e[2 * r], e[2 * r + 1]);
+                p[kb / 2][t] = __builtin_bit_cast(s8, pk4);
+            }
+            l[t] += sum;
+        }
+        // ---- O^T += V^T P^T ----
+#pragma unroll
+        for (int kk = 0; kk < KB / 2; ++kk)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const char* at = st + kk * 32 * ROWB + vrow + ((vsl ^ (2 * d)) << 4);
+                const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
+                const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + 16 * ROWB));
+                const s8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) o[t][d] = Mma<T>::mul(v, p[kk][t], o[t][d]);
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        l[t] += __shfl_xor(l[t], 16, 64);
+        l[t] += __shfl_xor(l[t], 32, 64);
+    }
+
+    if constexpr (BYWAVE) {                                       // the four waves' results join in order
+        __syncthreads();                                          // the ring is free
+        float* jo = reinterpret_cast<float*>(lds_all);            // [4][16 rows][DIM + 4]
+        float* jm = jo + 4 * 16 * (DIM + 4);                      // [4][16], then the sums
+#pragma unroll
+        for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(jo + (wave * 16 + l15) * (DIM + 4) + 16 * d + 4 * g) = o[0][d];
+        if (g == 0) {
+            jm[wave * 16 + l15] = m[0];
+            jm[64 + wave * 16 + l15] = l[0];
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        float mt = fmaxf(fmaxf(jm[l15], jm[16 + l15]), fmaxf(jm[32 + l15], jm[48 + l15]));
+        const float base = mt == -INFINITY ? 0.f : mt;
+        float lt = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float k = exp2f(jm[w * 16 + l15] - base);
+            lt += k * jm[64 + w * 16 + l15];
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[0][d] += k * *reinterpret_cast<const f32x4*>(jo + (w * 16 + l15) * (DIM + 4) + 16 * d + 4 * g);
+        }
+        m[0] = mt;
+        l[0] = lt;
+    }
+    // ---- results: lane (row l15) holds dims 16 d + 4 g + r ----
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        if (!row_ok[t]) continue;
+        const bool some = l[t] > 0.f || l[t] != l[t];             // a NaN sum is a result, an empty row is not
+        const float inv = some ? 1.f / l[t] : 0.f;
+        const float lse2 = some ? m[t] + log2f(l[t]) : -INFINITY;
+        const int64_t row = ((int64_t)row_b[t] * a.queries + row_i[t]) * a.heads + row_h[t];
+        if (slots == 1) {
+            T* out = static_cast<T*>(a.out) + row * DIM + 4 * g;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = some ? o[t][d][r] * inv : 0.f;
+                store_vec<T, 4>(out + 16 * d, v);
+            }
+            if (a.lse && g == 0) a.lse[((int64_t)row_b[t] * a.heads + row_h[t]) * a.queries + row_i[t]] = lse2 * kLn2;
+        } else {
+            const int64_t rows = (int64_t)a.batch * a.queries * a.heads, at = (int64_t)(L.slot0 + chunk) * rows + row;
+            if (some) {
+                float* out = a.work + at * DIM + 4 * g;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(out + 16 * d) = o[t][d] * inv;
+            }
+            if (g == 0) (a.work + (int64_t)slots * rows * DIM)[at] = lse2;
+        }
+    }
+}
+
+// Joins a row's partial results: out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  One wave a row; a partial result
+// without keys has no o (never written) and is passed over.
+template <class T, int DIM>
+__global__ __launch_bounds__(256) void prefix_attention_join_kernel(const PrefixAttnArgs a, int slots, int rows) {
+    constexpr int W = DIM / 64;
+    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (row >= rows) return;
+    const float* lse = a.work + (int64_t)slots * rows * DIM + row;
+    float top = -INFINITY;
+    bool odd = false;
+    for (int s = 0; s < slots; ++s) {
+        const float v = lse[(int64_t)s * rows];
+        top = fmaxf(top, v);
+        odd |= v != v;
+    }
+    float sum = 0.f, acc[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[i] = 0.f;
+    for (int s = 0; s < slots; ++s) {
+        const float v = lse[(int64_t)s * rows];
+        if (v == -INFINITY) continue;
+        const float k = exp2f(v - top);
+        float o[W];
+        load_vec<float, W>(a.work + ((int64_t)s * rows + row) * DIM + lane * W, o);
+        sum += k;
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[i] += k * o[i];
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[i] = odd ? __builtin_nanf("") : acc[i] * inv;
+    store_vec<T, W>(static_cast<T*>(a.out) + (int64_t)row * DIM + lane * W, acc);
+    if (a.lse && lane == 0) {
+        const int h = row % a.heads, bq = row / a.heads, b = bq / a.queries, i = bq % a.queries;
+        a.lse[((int64_t)b * a.heads + h) * a.queries + i] = odd ? __builtin_nanf("") : sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    }
+}
+
+template <class T, int DIM, int RT, bool BYWAVE>
+hipError_t launch_one(const PrefixAttnArgs& a, const PrefixAttnLaunch& l, int slots, hipStream_t stream) {
+    constexpr int LDS = BYWAVE ? 4 * 2 * 2 * 32 * DIM * 2 : 2 * 2 * 64 * DIM * 2;
+    static_assert(!BYWAVE || LDS >= (4 * 16 * (DIM + 4) + 128) * 4, "the join fits the ring");
+    auto* kernel = prefix_attention_kernel<T, DIM, RT, BYWAVE>;
+    static PerDevice<int> set;
+    int& done = set.get();
+    if (LDS > 64 * 1024 && !done) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) return e;
+        done = 1;
+    }
+    const int64_t blocks = (int64_t)(l.packed ? 1 : a.batch) * a.kv_heads * l.tiles * l.chunks;
+    kernel<<<dim3((unsigned)blocks), 256, LDS, stream>>>(a, l, slots);
+    return hipGetLastError();
+}
+
+template <class T, int DIM>
+hipError_t launch_dim(const PrefixAttnArgs& a, const PrefixAttnPlan& p, hipStream_t stream) {
+    for (int i = 0; i < p.n; ++i) {
+        hipError_t e;
+        switch (p.l[i].kind) {
+            case 0: e = launch_one<T, DIM, 1, true>(a, p.l[i], p.slots, stream); break;
+            case 1: e = launch_one<T, DIM, 1, false>(a, p.l[i], p.slots, stream); break;
+            default: e = launch_one<T, DIM, 2, false>(a, p.l[i], p.slots, stream); break;
+        }
+        if (e != hipSuccess) return e;
+    }
+    if (p.slots > 1) {
+        const int rows = a.batch * a.queries * a.heads;
+        prefix_attention_join_kernel<T, DIM><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, stream>>>(a, p.slots, rows);
+        return hipGetLastError();
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+PrefixAttnPlan prefix_attention_plan(const PrefixAttnArgs& a, int cus) {
+    PrefixAttnPlan plan;
+    const int grp = a.heads / a.kv_heads;
+    const int64_t rows_own = (int64_t)a.queries * grp;
+    auto add = [&](bool packed, int k_begin, int k_end) {
+        PrefixAttnLaunch l{};
+        l.packed = packed;
+        l.k_begin = k_begin;
+        l.k_end = k_end;
+        const int64_t rows = rows_own * (packed ? a.batch : 1);
+        l.kind = rows <= 16 ? 0 : rows <= 64 ? 1 : 2;
+        const int bm = l.kind == 0 ? 16 : 64 * l.kind;
+        l.tiles = (int)((rows + bm - 1) / bm);
+        const int64_t items = (int64_t)(packed ? 1 : a.batch) * a.kv_heads * l.tiles;
+        const int keys = k_end - k_begin, unit = 128;
+        // fill the chip (two blocks a CU) with chunks of at least 256 keys
+        int64_t n = (2 * cus + items - 1) / items;
+        n = std::min<int64_t>(n, std::max(1, keys / 256));
+        n = std::min<int64_t>(n, 32);
+        l.chunk = (int)std::max<int64_t>(unit, ((keys + n - 1) / n + unit - 1) / unit * unit);   // no keys at all: one empty chunk
+        l.chunks = std::max(1, (keys + l.chunk - 1) / l.chunk);
+        l.slot0 = plan.slots;
+        plan.slots += l.chunks;
+        plan.l[plan.n++] = l;
+    };
+    if (a.batch > 1 && a.prefix >= 256 && rows_own < 64) {
+        add(true, 0, a.prefix);
+        if (a.own_max > 0) add(false, a.prefix, a.prefix + a.own_max);
+    } else {
+        add(false, 0, a.prefix + a.own_max);
+    }
+    return plan;
+}
+
+int64_t prefix_attention_work_floats(const PrefixAttnArgs& a, const PrefixAttnPlan& p) {
+    return p.slots > 1 ? (int64_t)p.slots * a.batch * a.queries * a.heads * (a.dim + 1) : 0;
+}
+
+hipError_t launch_prefix_attention(const PrefixAttnArgs& a, const PrefixAttnPlan& p, hipStream_t stream) {
+    if (a.dtype == CMDI_DT_BF16) return a.dim == 128 ? launch_dim<Bf16, 128>(a, p, stream) : launch_dim<Bf16, 64>(a, p, stream);
+    return a.dim == 128 ? launch_dim<_Float16, 128>(a, p, stream) : launch_dim<_Float16, 64>(a, p, stream);
+}
+
+}  // namespace cmdi

@@ -8,7 +8,7 @@
  *
  * Conventions
  *   - every pointer named d_* is a DEVICE pointer (HIP), everything else is a host pointer;
- *   - all floating point is IEEE fp32, timesteps are int64, masks are uint8 (0/1);
+ *   - all floating point is IEEE fp32 (the block operators also take bf16 / f16), timesteps are int64, masks are uint8 (0/1);
  *   - motion tensors use the reference layout [B, J, 1, T] with T contiguous (J*1 = n_feats);
  *   - every call returns 0 on success or a negative CMDI_E_* code; cmdi_last_error() gives text;
  *   - calls only ENQUEUE work on `stream` (a hipStream_t); they never synchronise and never throw;
@@ -244,6 +244,83 @@ int cmdi_clip_create(const cmdi_clip_desc* desc, cmdi_clip_handle* out);
 int cmdi_clip_destroy(cmdi_clip_handle h);
 int cmdi_clip_load_weight(cmdi_clip_handle h, const char* name, const float* d_src, int64_t numel, cmdi_stream stream);
 int cmdi_clip_encode_text(cmdi_clip_handle h, const int32_t* d_tokens, int32_t batch, float* d_out, cmdi_stream stream);
+
+/* ---- block operators (csrc/api_ops.hip) --------------------------------------------------------
+ * The pieces of a transformer block in reduced precision, for denoisers and text towers beyond the two the engine builds:
+ * norms with a gate, a linear layer in 8-bit integers, attention behind a prefix that a batch shares.  No handle: every
+ * buffer is the caller's, scratch included, and has to live on `stream`'s device until the work on `stream` is done.
+ * Two calls may run at once on two streams if their scratch and outputs differ. */
+enum { CMDI_DT_F32 = 0, CMDI_DT_BF16 = 1, CMDI_DT_F16 = 2 };
+enum { CMDI_NORM_NONE = 0, CMDI_NORM_RMS = 1, CMDI_NORM_LAYER = 2 };
+
+/* r = residual_scale x + gate * N_post(y),  h = (N_pre(r) weight + bias) (1 + scale) + shift.
+ * N(v) = v / sqrt(mean(v^2) + eps) (RMS), the same of v - mean(v) (LAYER), or v (NONE, post only); statistics in fp32 from
+ * the unrounded r, one rounding at each output.  Rows: x, y [batch, seq, dim], dim contiguous (1 .. 16384), strides in
+ * elements (0 allowed: a broadcast input).  gate, scale, shift: `dim` elements for every sample (stride 0) or one such row for
+ * each, `stride` elements apart; null: 1, 0, 0.  weight, bias, post_weight, post_bias: `dim` elements or null (1, 0).
+ * d_y null: r = residual_scale x (then no gate and no post).  `dtype` is x's, y's and the outputs' type, `param_dtype` that of
+ * the parameters: CMDI_DT_F32 or `dtype`.  batch * seq < 2^31; batch or seq 0: nothing to do. */
+typedef struct {
+    int32_t batch, seq, dim;
+    int32_t dtype, param_dtype;
+    int32_t post, pre;                       /* CMDI_NORM_* */
+    float residual_scale, eps;
+    const void *d_x, *d_y;
+    int64_t x_stride[2], y_stride[2];        /* samples, rows */
+    const void *d_gate, *d_scale, *d_shift;
+    int64_t gate_stride, scale_stride, shift_stride;
+    const void *d_weight, *d_bias, *d_post_weight, *d_post_bias;
+} cmdi_gated_norm_desc;
+/* d_r, d_h: contiguous [batch, seq, dim], apart from the inputs; d_r may be null. */
+int cmdi_gated_norm_fwd(const cmdi_gated_norm_desc* d, void* d_r, void* d_h, cmdi_stream stream);
+/* Gradients for d_gr, d_gh, those of r and h (either may be null = 0; strides in elements).  Every output may be null (not
+ * wanted): g_x, g_y contiguous [batch, seq, dim] of `dtype`; the others of `param_dtype`, shaped as their parameter: [dim], or
+ * contiguous [batch, dim] where its stride is not 0.  Sums over rows in fp32 in a fixed order (the same bits every run), rounded
+ * once.  d_work: cmdi_gated_norm_vjp_workspace bytes (may be null where that is 0). */
+typedef struct {
+    const void *d_gr, *d_gh;
+    int64_t gr_stride[2], gh_stride[2];
+    void *d_gx, *d_gy;
+    void *d_ggate, *d_gscale, *d_gshift, *d_gweight, *d_gbias, *d_gpost_weight, *d_gpost_bias;
+    void* d_work;
+    int64_t work_bytes;
+} cmdi_gated_norm_grads;
+int cmdi_gated_norm_vjp(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_grads* g, cmdi_stream stream);
+/* Bytes of d_work for these outputs (their pointers only say which are wanted), or a negative CMDI_E_*. */
+int64_t cmdi_gated_norm_vjp_workspace(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_grads* g);
+
+/* Rows in 8 bits: scale[r] = max|x[r]| / 127 (fp32), q[r, k] = round(x[r, k] * (127 / max)), halves to even, both fp32
+ * operations rounded; columns behind `cols` up to kp are 0.  A row whose largest magnitude is below 1e-35 is all zeros with
+ * scale 0; one with an infinity or a NaN has scale NaN.  x [rows, cols] of `dtype` with `ld` elements between rows; q
+ * [rows, kp] contiguous, 16-byte aligned, kp a multiple of 128, cols <= kp <= 130048. */
+int cmdi_quant_rows_i8(const void* d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld, void* d_q, int32_t kp,
+                       float* d_scale, cmdi_stream stream);
+/* C[m, n] = epi((sum_k a[m, k] w[n, k]) a_scale[m] w_scale[n] + bias[n]); the sum exact in 32-bit integers.  a, w: int8 rows,
+ * lda / ldw bytes apart (multiples of 16, at most 2^22), 16-byte aligned; k a multiple of 128, at most 130048.  c (and d_resid
+ * for epi 3) of `dtype`, ldc / ldr elements apart; bias fp32 or null.  epi as in cmdi_gemm_nt: 0 bias, 1 bias + GELU(erf),
+ * 3 bias + residual (d_resid may be d_c).  m 0: nothing to do. */
+int cmdi_gemm_i8(const void* d_a, const float* d_a_scale, const void* d_w, const float* d_w_scale, const float* d_bias,
+                 const void* d_resid, void* d_c, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldw, int64_t ldc,
+                 int64_t ldr, int32_t dtype, int32_t epi, cmdi_stream stream);
+
+/* out[b, i, h] = softmax_j(scale q[b, i, h] . k_j) v_j over the prefix's keys [prefix] and sample b's own keys
+ * j < visible(b, i): own_len[b], or with `causal` own_len[b] - queries + i + 1 (the queries are the newest of the own tokens).
+ * A row that sees no key is 0 with lse -inf; keys behind a length are never read.  bf16 or f16, dim 64 or 128, heads a multiple
+ * of kv_heads (head h reads key head h / (heads / kv_heads)); strides in elements, `dim` contiguous, 16-byte aligned, token
+ * strides at most 2^23.  own_len: int32 [batch] on the device (taken as 0 .. own_max), or null: own_max.  scale > 0.
+ * d_lse fp32 [batch, heads, queries] or null: log of the softmax's sum.  d_work: cmdi_prefix_attention_workspace bytes. */
+typedef struct {
+    int32_t batch, queries, heads, kv_heads, dim, prefix, own_max, causal, dtype;
+    float scale;
+    const void *d_q, *d_prefix_k, *d_prefix_v, *d_own_k, *d_own_v;
+    int64_t q_stride[3];                             /* samples, tokens, heads */
+    int64_t prefix_k_stride[2], prefix_v_stride[2];  /* tokens, heads */
+    int64_t own_k_stride[3], own_v_stride[3];
+    const int32_t* d_own_len;
+} cmdi_prefix_attention_desc;
+int cmdi_prefix_attention(const cmdi_prefix_attention_desc* d, void* d_out, float* d_lse, void* d_work, int64_t work_bytes,
+                          cmdi_stream stream);
+int64_t cmdi_prefix_attention_workspace(const cmdi_prefix_attention_desc* d);
 
 /* ---- introspection for tests / bench --------------------------------------------------------- */
 /* Raw NT GEMM used by every projection: C[M,N] = epi(A[M,K] · W[N,K]^T + bias[N]); fp32 MFMA.

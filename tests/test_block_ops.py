@@ -1,0 +1,730 @@
+"""Block operators (ops.py): gated norms, the 8-bit linear layer, shared-prefix attention, against their formulas in 64 bits.
+
+Tolerances come from arithmetic.  u = finfo(type).eps / 2 is half a step of the output's type, e = 2^-24 half a step of fp32.
+A fp32 value computed through at most n roundings from terms whose magnitudes add up to S is off by at most n e S (first order);
+the kernels' chains are a lane's elements (<= 16 of a row), 6 steps across a wave, up to 16 waves, and a dozen operations around
+them, so n = 64 covers a row's statistics and n = 128 a gradient that uses two of them.  Sums over rows add one rounding a row."""
+import ctypes as C
+import importlib
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import PKG
+
+E = 2.0 ** -24
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def ops():
+    return importlib.import_module(f"{PKG}.ops")
+
+
+def native():
+    return importlib.import_module(f"{PKG}._native")
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rounding(dtype, want):
+    """Of one rounding to dtype: half a step relative, and below the smallest normal number half the subnormals' fixed step
+    (fp16: 2^-25, which is more than 2^-11 of any value below 2^-14)."""
+    return half_step(dtype) * want.abs() + torch.finfo(dtype).smallest_normal * half_step(dtype)
+
+
+def within(got, want, tol, what):
+    got, want, tol = got.detach().double().cpu(), want.double().cpu(), tol.double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert torch.isfinite(want).all() and torch.isfinite(got).all(), what
+    worst = ((got - want).abs() / tol.expand_as(want).clamp_min(1e-300)).max().item() if want.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3g} times its tolerance"
+
+
+# ---- gated norm: the formulas in 64 bits, each beside the magnitude that its fp32 evaluation adds up ---------------------------
+
+def norm64(x, y=None, *, gate=None, residual_scale=1.0, post="none", post_weight=None, post_bias=None, pre="layer", weight=None, bias=None,
+           scale=None, shift=None, eps=1e-5, grad_r=None, grad_h=None):
+    """({name: value}, {name: tolerance without the output's own rounding}) of r, h and, with gradients given, of every input's."""
+    b, s, d = x.shape
+    D = lambda t: None if t is None else t.detach().double().cpu()  # noqa: E731
+    per = lambda t, fill: torch.full((1, 1, d), fill, dtype=torch.float64) if t is None else D(t).reshape(-1, 1, d)  # noqa: E731
+    x64, y64 = D(x), D(y)
+    g, sc, sh = per(gate, 1.0), per(scale, 0.0), per(shift, 0.0)
+    w, c, wp, cp = per(weight, 1.0), per(bias, 0.0), per(post_weight, 1.0), per(post_bias, 0.0)
+
+    def stats(kind, v, vabs):
+        """(n, k, magnitude behind n): n = (v - mean) k."""
+        if kind == "none":
+            return v, torch.ones_like(v[..., :1]), vabs
+        mean = v.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(v[..., :1])
+        k = 1 / torch.sqrt(((v - mean) ** 2).mean(-1, keepdim=True) + eps)
+        n = (v - mean) * k
+        # an error of v or of the mean reaches n through k; k's own relative error is that of the mean square, which an error dv
+        # changes by 2 mean|c dv| / mean c^2 <= 2 k max|dv|: the row's largest magnitude stands for both
+        top = vabs.amax(-1, keepdim=True)
+        return n, k, n.abs() + k * (vabs + vabs.mean(-1, keepdim=True)) + 2 * n.abs() * k * top
+
+    def back(kind, dn, dn_abs, n, n_abs, k, k_rel):
+        if kind == "none":
+            return dn, dn_abs
+        layer = kind == "layer"
+        dv = dn - n * (dn * n).mean(-1, keepdim=True) - (dn.mean(-1, keepdim=True) if layer else 0)
+        mag = dn_abs + n_abs * (dn_abs * n_abs).mean(-1, keepdim=True) + (dn_abs.mean(-1, keepdim=True) if layer else 0)
+        return dv * k, mag * k * (1 + k_rel)
+
+    val, tol = {}, {}
+    if y is not None:
+        ny, ky, ny_abs = stats(post, y64, y64.abs())
+        ky_rel = (2 * ky * y64.abs().amax(-1, keepdim=True)) if post != "none" else torch.zeros_like(ky)
+        m, m_abs = ny * wp + cp, ny_abs * wp.abs() + cp.abs()
+        r, r_abs = residual_scale * x64 + g * m, (residual_scale * x64).abs() + g.abs() * m_abs
+    else:
+        r, r_abs = residual_scale * x64, (residual_scale * x64).abs()
+    val["r"], tol["r"] = r, 64 * E * r_abs
+    n, k, n_abs = stats(pre, r, r_abs)
+    k_rel = 2 * k * r_abs.amax(-1, keepdim=True)
+    u, u_abs = n * w + c, n_abs * w.abs() + c.abs()
+    val["h"] = u * (1 + sc) + sh
+    tol["h"] = 64 * E * (u_abs * (1 + sc.abs()) + sh.abs())
+    if grad_r is None and grad_h is None:
+        return val, tol
+    gr = torch.zeros_like(r) if grad_r is None else D(grad_r)
+    gh = torch.zeros_like(r) if grad_h is None else D(grad_h)
+    du = gh * (1 + sc)
+    du_abs = gh.abs() * (1 + sc.abs())
+    dn, dn_abs = du * w, du_abs * w.abs()
+    dv, dv_abs = back(pre, dn, dn_abs, n, n_abs, k, k_rel)
+    dr, dr_abs = gr + dv, gr.abs() + dv_abs
+    full = {"x": (residual_scale * dr, abs(residual_scale) * dr_abs), "scale": (gh * u, gh.abs() * u_abs), "shift": (gh, gh.abs()),
+            "weight": (du * n, du_abs * n_abs), "bias": (du, du_abs)}
+    if y is not None:
+        dm, dm_abs = dr * g, dr_abs * g.abs()
+        full["y"] = back(post, dm * wp, dm_abs * wp.abs(), ny, ny_abs, ky, ky_rel)
+        full.update(gate=(dr * m, dr_abs * m_abs), post_weight=(dm * ny, dm_abs * ny_abs), post_bias=(dm, dm_abs))
+    given = dict(x=x, y=y, gate=gate, scale=scale, shift=shift, weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias)
+    for name, t in given.items():
+        if t is None:
+            continue
+        v, a = full[name]
+        if name in ("x", "y"):
+            val["g_" + name], tol["g_" + name] = v, 128 * E * a
+            continue
+        axes = (0, 1) if t.dim() == 1 else (1,)
+        rows = b * s if t.dim() == 1 else s
+        val["g_" + name], tol["g_" + name] = v.sum(axes), (128 + rows) * E * a.sum(axes)
+    return val, tol
+
+
+def norm_case(b, s, d, dtype, params, post, pre, gate, mod, affine, seed=0, y=True):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *sh: torch.randn(*sh, generator=g)  # noqa: E731
+    dt, pt = DTYPES[dtype], DTYPES[params]
+    t = dict(x=rnd(b, s, d).mul(2).to(dt), y=rnd(b, s, d).to(dt) if y else None)
+    kw = dict(gate=None if gate == "none" or not y else rnd(*((d,) if gate == "shared" else (b, d))).to(pt), post=post if y else "none", pre=pre,
+              scale=rnd(b, d).mul(.3).to(pt) if mod else None, shift=rnd(d).mul(.3).to(pt) if mod else None,
+              weight=(1 + .1 * rnd(d)).to(pt) if affine else None, bias=rnd(d).to(pt) if affine else None,
+              post_weight=(1 + .1 * rnd(d)).to(pt) if affine and post != "none" and y else None,
+              post_bias=rnd(d).to(pt) if affine and post != "none" and y else None, residual_scale=0.75)
+    grads = rnd(b, s, d).to(dt), rnd(b, s, d).to(dt)
+    cuda = lambda v: v.cuda() if isinstance(v, torch.Tensor) else v  # noqa: E731
+    return {k: cuda(v) for k, v in t.items()}, {k: cuda(v) for k, v in kw.items()}, tuple(cuda(v) for v in grads)
+
+
+NORM_CASES = [
+    # batch, seq, dim, dtype, params, post, pre, gate, modulate, affine
+    (1, 1, 1, "f32", "f32", "none", "layer", "shared", True, True),
+    (1, 1, 512, "bf16", "bf16", "rms", "rms", "sample", True, True),
+    (2, 3, 7, "f16", "f32", "layer", "layer", "sample", True, True),
+    (3, 5, 64, "f32", "f32", "layer", "rms", "shared", False, True),
+    (64, 1, 512, "f32", "f32", "none", "layer", "sample", True, False),
+    (2, 197, 512, "f32", "f32", "none", "layer", "sample", True, False),
+    (2, 130, 515, "f16", "f32", "layer", "layer", "shared", False, True),
+    (3, 70, 1024, "bf16", "f32", "rms", "layer", "none", True, True),
+    (2, 33, 1032, "bf16", "bf16", "rms", "rms", "sample", True, True),
+    (1, 300, 2048, "bf16", "bf16", "layer", "layer", "sample", True, True),
+    (2, 9, 3001, "f32", "f32", "rms", "layer", "shared", True, False),
+    (1, 17, 4096, "f16", "f16", "layer", "rms", "sample", False, True),
+    (1, 5, 8192, "f32", "f32", "rms", "rms", "sample", True, True),
+    (2, 3, 16384, "bf16", "bf16", "layer", "layer", "shared", True, True),
+    (1, 2, 16383, "bf16", "f32", "rms", "layer", "sample", True, True),
+    (700, 2, 40, "bf16", "bf16", "none", "rms", "sample", True, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", NORM_CASES, ids=lambda c: "-".join(map(str, c)))
+def test_gated_norm_and_gradients(case):
+    t, kw, (gr, gh) = norm_case(*case)
+    val, tol = norm64(t["x"], t["y"], **kw, grad_r=gr, grad_h=gh)
+    leaves = {k: v.clone().requires_grad_() for k, v in {**t, **kw}.items() if isinstance(v, torch.Tensor)}
+    opts = {k: leaves.get(k, v) for k, v in kw.items()}
+    r, h = ops().gated_norm(leaves["x"], leaves["y"], **opts)
+    for name, got in (("r", r), ("h", h)):
+        within(got, val[name], tol[name] + rounding(t["x"].dtype, val[name]), name)
+    for name, got in zip(leaves, torch.autograd.grad((r, h), list(leaves.values()), (gr, gh))):
+        want = val["g_" + name]
+        assert got.dtype == leaves[name].dtype
+        within(got, want, tol["g_" + name] + rounding(got.dtype, want), "gradient of " + name)
+    # no recorded graph: the same bits
+    r2, h2 = ops().gated_norm_fwd(t["x"], t["y"], **kw)
+    assert torch.equal(r2, r) and torch.equal(h2, h)
+    again = ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw)
+    first = ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw)
+    for name in again:
+        assert again[name] is None and first[name] is None or torch.equal(again[name], first[name]), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["r", "h"])
+def test_gated_norm_one_gradient_only_and_no_block(which):
+    t, kw, (gr, gh) = norm_case(2, 20, 96, "f32", "f32", "layer", "rms", "sample", True, True)
+    gr, gh = (gr, None) if which == "r" else (None, gh)
+    val, tol = norm64(t["x"], t["y"], **kw, grad_r=gr, grad_h=gh)
+    got = ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw)
+    for name, v in got.items():
+        within(v, val["g_" + name], tol["g_" + name] + E * val["g_" + name].abs(), name)
+    only = ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw, wanted=("y", "bias"))
+    assert {k for k, v in only.items() if v is not None} == {"y", "bias"}
+    assert torch.equal(only["y"], got["y"]) and torch.equal(only["bias"], got["bias"])
+    # a stack's first norm: no block in front
+    t, kw, (gr, gh) = norm_case(3, 11, 130, "bf16", "bf16", "none", "layer", "none", True, True, y=False)
+    val, tol = norm64(t["x"], **kw, grad_r=gr, grad_h=gh)
+    r, h = ops().gated_norm(t["x"], **kw)
+    u = half_step(torch.bfloat16)
+    within(h, val["h"], tol["h"] + u * val["h"].abs(), "h")
+    got = ops().gated_norm_vjp(gr, gh, t["x"], **kw)
+    for name in ("x", "scale", "shift", "weight", "bias"):
+        within(got[name], val["g_" + name], tol["g_" + name] + u * val["g_" + name].abs(), name)
+
+
+@pytest.mark.gpu
+def test_gated_norm_gradient_against_differences():
+    t, kw, (gr, gh) = norm_case(1, 3, 24, "f32", "f32", "layer", "layer", "sample", True, True)
+    got = ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw)
+    tensors = {"x": t["x"], "y": t["y"], **{k: v for k, v in kw.items() if isinstance(v, torch.Tensor)}}
+    rest = {k: v for k, v in kw.items() if not isinstance(v, torch.Tensor)}
+
+    def loss(ts):
+        ts = dict(ts)
+        val, _ = norm64(ts.pop("x"), ts.pop("y"), **ts, **rest)
+        return float((val["r"] * gr.double().cpu()).sum() + (val["h"] * gh.double().cpu()).sum())
+    g = torch.Generator().manual_seed(3)
+    for name, v in tensors.items():
+        way = torch.randn(v.shape, generator=g, dtype=torch.float64)
+        step = 1e-5
+        up, down = ({**{k: w.double().cpu() for k, w in tensors.items()}, name: v.double().cpu() + s * step * way} for s in (1, -1))
+        slope = (loss(up) - loss(down)) / (2 * step)
+        # the kernel's directional derivative: each term within its tolerance (1e-4 relative to the terms' magnitudes covers the
+        # 128 to 200 fp32 roundings, at most 1.2e-5, and the difference quotient's own step^2 ~ 1e-10 times a third derivative)
+        terms = got[name].double().cpu() * way
+        assert abs(float(terms.sum()) - slope) <= 1e-4 * float(terms.abs().sum()) + 1e-6, name
+
+
+@pytest.mark.gpu
+def test_gated_norm_strides_views_and_broadcast():
+    g = torch.Generator().manual_seed(5)
+    base = torch.randn(4, 3 * 11, 2 * 96, generator=g).bfloat16().cuda()
+    x, y = base[::2, 1::3, :96], base[1::2, ::3, 96:]                        # strided samples and rows
+    mod = torch.randn(2, 3 * 96, generator=g).bfloat16().cuda()
+    gate, scale, shift = mod.chunk(3, 1)                                   # rows 288 apart
+    r, h = ops().gated_norm_fwd(x, y, gate=gate, scale=scale, shift=shift, post="rms", pre="rms")
+    r2, h2 = ops().gated_norm_fwd(x.contiguous(), y.contiguous(), gate=gate.contiguous(), scale=scale.contiguous(), shift=shift.contiguous(),
+                                  post="rms", pre="rms")
+    assert torch.equal(r, r2) and torch.equal(h, h2)
+    # a misaligned view takes the element-wise loads: the same values up to the order of a row's sums
+    flat = torch.randn(1 + 2 * 11 * 96, generator=g).bfloat16().cuda()
+    xo = flat[1:].view(2, 11, 96)
+    val, tol = norm64(xo, None, pre="layer", scale=scale, shift=shift)
+    _, h3 = ops().gated_norm_fwd(xo, scale=scale, shift=shift)
+    within(h3, val["h"], tol["h"] + half_step(torch.bfloat16) * val["h"].abs(), "misaligned")
+    # broadcast inputs: an expanded x, an expanded gradient (stride 0), a gate expanded over the samples
+    one = torch.randn(1, 1, 96, generator=g).cuda()
+    xe, ge = one.expand(3, 5, 96), torch.ones(1, 1, 1).cuda().expand(3, 5, 96)
+    gx = torch.randn(96, generator=g).cuda().expand(3, 96).requires_grad_(False)
+    yy = torch.randn(3, 5, 96, generator=g).cuda()
+    val, tol = norm64(xe, yy, gate=gx, grad_r=ge, grad_h=ge)
+    got = ops().gated_norm_vjp(ge, ge, xe, yy, gate=gx)
+    for name in ("x", "y", "gate"):
+        within(got[name], val["g_" + name], tol["g_" + name] + E * val["g_" + name].abs(), name)
+    # one sample with a gate of its own: its gradient keeps the gate's shape
+    t, kw, (gr, gh) = norm_case(1, 9, 64, "f32", "f32", "none", "layer", "sample", False, False)
+    assert ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw)["gate"].shape == (1, 64)
+
+
+@pytest.mark.gpu
+def test_gated_norm_empty_rows_and_special_values():
+    x = torch.zeros(2, 0, 64, device="cuda")
+    r, h = ops().gated_norm(x, x)
+    assert r.shape == h.shape == (2, 0, 64)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    _, h = ops().gated_norm(x, x, weight=w)
+    assert torch.equal(torch.autograd.grad(h.sum(), w)[0], torch.zeros(64, device="cuda"))
+    # a row of equal values: no variance, eps alone; a NaN stays in its row
+    x = torch.full((1, 3, 64), 3.0, device="cuda")
+    x[0, 1, 5] = math.nan
+    _, h = ops().gated_norm(x)
+    assert torch.equal(h[0, 0], torch.zeros(64, device="cuda")) and torch.isnan(h[0, 1]).all() and torch.equal(h[0, 2], torch.zeros(64, device="cuda"))
+
+
+# ---- the 8-bit linear layer ---------------------------------------------------------------------------------------------------
+
+def quant_np(x):
+    x = np.asarray(x, np.float32)
+    top = np.abs(x).max(1)
+    some = top >= np.float32(1e-35)
+    inv = np.where(some, np.float32(127) / np.where(some, top, 1), 0).astype(np.float32)
+    return np.rint(x * inv[:, None]).astype(np.int64), np.where(some, top / np.float32(127), 0).astype(np.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,dtype", [(1, 1, "f32"), (3, 7, "f16"), (5, 128, "bf16"), (4, 263, "f16"), (2, 512, "f32"), (9, 2048, "bf16"),
+                                             (3, 2056, "f32"), (2, 8200, "bf16"), (2, 16384, "f32"), (1, 20001, "f16"), (1, 70000, "f32")])
+def test_quantize_rows(rows, cols, dtype):
+    g = torch.Generator().manual_seed(rows * cols)
+    x = (torch.randn(rows, cols, generator=g) * torch.exp(torch.randn(rows, 1, generator=g))).to(DTYPES[dtype])
+    x[-1] = 0 if rows > 1 else x[-1]
+    if cols > 4:
+        x[0, 1::2] = x[0, 0::2][: x[0, 1::2].numel()] * 0.5            # halves of a step
+    q, scale = ops().quantize_rows(x.cuda())
+    want, ws = quant_np(x.float().numpy())
+    assert q.shape == (rows, (cols + 127) // 128 * 128)
+    assert np.array_equal(q.cpu().numpy()[:, :cols], want) and not q[:, cols:].any()
+    assert np.array_equal(scale.cpu().numpy(), ws)
+
+
+@pytest.mark.gpu
+def test_quantize_rows_special_rows_and_strides():
+    base = torch.randn(4, 3, 200).cuda()
+    x = base[:, 1]
+    q, s = ops().quantize_rows(x)
+    q2, s2 = ops().quantize_rows(x.contiguous())
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+    q2, s2 = ops().quantize_rows(x.t().contiguous().t())
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+    x = x.clone()
+    x[0, 3], x[1, 4], x[2] = math.inf, math.nan, 1e-38
+    q, s = ops().quantize_rows(x)
+    assert torch.isnan(s[:2]).all() and s[2] == 0 and not q[:3].any() and s[3] == s2[3]
+    w, ws = ops().quantize_rows(torch.randn(16, 200).cuda())
+    c = ops().linear_i8(x, w, ws, torch.ones(16, device="cuda"))
+    assert torch.isnan(c[:2]).all() and torch.equal(c[2], torch.ones(16, device="cuda")) and torch.isfinite(c[3]).all()
+    assert ops().quantize_rows(x[:0])[0].shape == (0, 256) and ops().linear_i8(x[:0], w, ws).shape == (0, 16)
+
+
+def gemm64(qa, sa, qw, sw, bias, epi, resid, dtype):
+    """(value, tolerance): the integer sum is exact; its conversion, the two scales and the bias are four roundings, gelu's erf is
+    within 8.8e-8 of its own (csrc/common.hpp) and adds a handful, the residual one."""
+    acc = (qa.astype(np.int64) @ qw.astype(np.int64).T).astype(np.float64)
+    v = acc * sa.astype(np.float64)[:, None] * sw.astype(np.float64)
+    mag = np.abs(v) + (0 if bias is None else np.abs(bias))
+    v = v + (0 if bias is None else bias.astype(np.float64))
+    tol = 4 * E * mag
+    if epi == "gelu":
+        from scipy.special import erfc
+        x = v
+        v = 0.5 * x * erfc(-x / math.sqrt(2))
+        tol = 1.2 * tol + (8.8e-8 / 2 + 4 * E) * np.abs(x)       # |gelu'| <= 1.13
+    if epi == "resid":
+        r = resid.astype(np.float64)
+        v, tol = v + r, tol + E * (mag + np.abs(r))
+    return torch.from_numpy(v), torch.from_numpy(tol + rounding(dtype, torch.from_numpy(v)).numpy())
+
+
+GEMM_CASES = [(1, 1, 128), (1, 515, 256), (2, 1536, 512), (8, 8200, 1024), (16, 100, 4096), (17, 33, 640), (33, 1000, 384), (64, 512, 2176), (65, 64, 128),
+              (100, 515, 384), (197, 1536, 512), (300, 300, 1152), (1001, 515, 384), (2048, 1664, 256), (4099, 4100, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", GEMM_CASES)
+@pytest.mark.parametrize("dtype,epi", [("f32", "bias"), ("bf16", "resid"), ("f16", "gelu")])
+def test_gemm_i8(m, n, k, dtype, epi):
+    rng = np.random.default_rng(m * 7 + n)
+    qa, qw = rng.integers(-128, 128, (m, k)).astype(np.int8), rng.integers(-128, 128, (n, k)).astype(np.int8)
+    qa[0], qw[0] = -128, -128                                          # the largest sum
+    sa = (rng.random(m) / k).astype(np.float32)
+    sw = (rng.random(n) / 64).astype(np.float32)
+    bias = rng.standard_normal(n).astype(np.float32) if epi != "resid" or m % 2 else None
+    dt = DTYPES[dtype]
+    resid = torch.from_numpy(rng.standard_normal((m, n)).astype(np.float32)).to(dt) if epi == "resid" else None
+    want, tol = gemm64(qa, sa, qw, sw, bias, epi, None if resid is None else resid.float().numpy(), dt)
+    cuda = lambda a: None if a is None else torch.as_tensor(a).cuda()  # noqa: E731
+    got = ops().gemm_i8(cuda(qa), cuda(sa), cuda(qw), cuda(sw), cuda(bias), epi=epi, resid=cuda(resid), dtype=dt)
+    assert got.dtype == dt
+    within(got, want, tol + 1e-30, "C")
+
+
+@pytest.mark.gpu
+def test_gemm_i8_longest_k_and_views():
+    k = 130048
+    a = torch.full((2, k), -128, dtype=torch.int8, device="cuda")
+    one = torch.ones(2, device="cuda")
+    c = ops().gemm_i8(a, one, a, one)
+    assert torch.equal(c.cpu(), torch.full((2, 2), float(k * 16384)))
+    # weights whose rows stand 64 bytes apart from each other's end, activations out of a larger buffer, a strided residual
+    g = torch.Generator().manual_seed(1)
+    big = torch.randint(-127, 128, (300, 320), generator=g, dtype=torch.int8).cuda()
+    a, w = big[:70, :256], big[100:, 64:320]
+    sa, sw = torch.rand(70, generator=g).cuda(), torch.rand(200, generator=g).cuda()
+    resid = torch.randn(70, 2, 200, generator=g).cuda()[:, 1]
+    got = ops().gemm_i8(a, sa, w, sw, epi="resid", resid=resid)
+    assert torch.equal(got, ops().gemm_i8(a.contiguous(), sa, w.contiguous(), sw, epi="resid", resid=resid.contiguous()))
+    want, tol = gemm64(a.cpu().numpy(), sa.cpu().numpy(), w.cpu().numpy(), sw.cpu().numpy(), None, "resid", resid.cpu().numpy(), torch.float32)
+    within(got, want, tol, "views")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,dtype", [(1, 96, 100, "f32"), (40, 130, 263, "f16"), (200, 260, 512, "bf16")])
+def test_linear_i8(m, n, k, dtype):
+    g = torch.Generator().manual_seed(m)
+    x, w, bias = torch.randn(m, k, generator=g).to(DTYPES[dtype]), torch.randn(n, k, generator=g), torch.randn(n, generator=g)
+    qw, sw = ops().quantize_rows(w.cuda())
+    got = ops().linear_i8(x.cuda(), qw, sw, bias.cuda())
+    (qa, sa), (qn, sn) = quant_np(x.float().numpy()), quant_np(w.numpy())
+    want, tol = gemm64(qa, sa, qn, sn, bias.numpy(), "bias", None, DTYPES[dtype])
+    within(got, want, tol, "linear")
+
+
+# ---- shared-prefix attention ----------------------------------------------------------------------------------------------------
+
+def attention64(q, pk, pv, ok, ov, lens, causal, scale=None):
+    """(out, lse, tolerance of out without its own rounding, tolerance of lse).  P is rounded to 16 bits (half a step each), scores
+    are sums of `dim` products and meet the exponential through three more roundings, whose error is relative in p: (2 dim + 64
+    + 4 |score|) e covers both, the sums over the keys add one rounding a key of a lane (a sixteenth of them)."""
+    b, n, h, d = q.shape
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    f = lambda t: t.detach().double().cpu()  # noqa: E731
+    out, lse = torch.zeros(b, n, h, d, dtype=torch.float64), torch.full((b, h, n), -math.inf, dtype=torch.float64)
+    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+    hk = (pk if pk is not None else ok).shape[-2]
+    u = half_step(q.dtype)
+    none = torch.zeros(0, hk, d, dtype=torch.float64)
+    for i in range(b):
+        m = 0 if ok is None else int(ok.shape[1] if lens is None else min(max(int(lens[i]), 0), ok.shape[1]))
+        k = torch.cat([none if pk is None else f(pk), none if ok is None else f(ok[i, :m])])
+        v = torch.cat([none if pv is None else f(pv), none if ov is None else f(ov[i, :m])])
+        p = 0 if pk is None else pk.shape[0]
+        for t in range(n):
+            seen = p + (min(max(m - n + t + 1, 0), m) if causal else m)
+            if seen == 0:
+                continue
+            for j in range(h):
+                kk, vv, qq = k[:seen, j // (h // hk)], v[:seen, j // (h // hk)], f(q[i, t, j])
+                s = kk @ qq * scale
+                mag = (kk.abs() @ qq.abs() * scale).max() * 1.5
+                lse[i, j, t] = torch.logsumexp(s, 0)
+                w = torch.exp(s - lse[i, j, t])
+                out[i, t, j] = w @ vv
+                rel = (2 * d + 64) * E * mag / d * 2 + (64 + 4 * float(s.abs().max()) + seen / 16) * E
+                tol[i, t, j] = (w @ vv.abs()) * (u + 2 * rel)
+                ltol[i, j, t] = rel + 4 * E * lse[i, j, t].abs()
+    return out, lse, tol, ltol
+
+
+def attention_case(b, n, h, hk, d, p, o, dtype, seed=0, lens="ragged"):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *sh: torch.randn(*sh, generator=g).to(DTYPES[dtype]).cuda()  # noqa: E731
+    q = rnd(b, n, h, d)
+    pk, pv = (rnd(p, hk, d), rnd(p, hk, d)) if p else (None, None)
+    ok, ov = (rnd(b, o, hk, d), rnd(b, o, hk, d)) if o else (None, None)
+    length = None
+    if o and lens == "ragged":
+        length = torch.randint(0, o + 1, (b,), generator=g).to(torch.int32)
+        length[0], length[-1] = o, 0 if b > 1 else o
+        length = length.cuda()
+    return q, pk, pv, ok, ov, length
+
+
+ATTENTION_CASES = [
+    # batch, queries, heads, kv heads, dim, prefix, own
+    (1, 1, 1, 1, 64, 1, 0), (1, 1, 1, 1, 128, 0, 1), (2, 1, 4, 4, 128, 77, 32), (3, 1, 8, 2, 64, 0, 130), (5, 1, 6, 3, 128, 300, 40),
+    (2, 2, 4, 1, 64, 333, 70), (4, 3, 8, 2, 128, 1000, 17), (40, 1, 4, 2, 64, 700, 0), (33, 1, 10, 2, 128, 513, 9), (1, 1, 8, 1, 128, 5000, 3),
+    (3, 20, 4, 4, 64, 100, 20), (2, 30, 4, 2, 128, 300, 64), (1, 65, 2, 2, 128, 65, 65), (2, 197, 2, 1, 64, 196, 197), (1, 150, 4, 2, 128, 0, 300),
+    (6, 5, 4, 4, 128, 600, 300), (1, 17, 1, 1, 64, 2000, 500), (2, 9, 16, 2, 128, 257, 90),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", ATTENTION_CASES, ids=lambda c: "-".join(map(str, c)))
+def test_shared_prefix_attention(case, dtype, causal):
+    q, pk, pv, ok, ov, lens = attention_case(*case, dtype)
+    out, lse = ops().shared_prefix_attention(q, pk, pv, ok, ov, lens, causal=causal, return_lse=True)
+    want, wl, tol, ltol = attention64(q, pk, pv, ok, ov, lens, causal)
+    within(out, want, tol + rounding(q.dtype, want.abs() + tol), "out")
+    lse = lse.double().cpu()
+    assert torch.equal(torch.isinf(lse), torch.isinf(wl)) and (lse[torch.isinf(lse)] < 0).all()
+    fin = torch.isfinite(wl)
+    within(lse[fin], wl[fin], ltol[fin], "lse")
+    assert torch.equal(out, ops().shared_prefix_attention(q, pk, pv, ok, ov, lens, causal=causal))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,p", [(1, 40), (1, 600), (70, 40)])
+def test_shared_prefix_attention_never_reads_behind_a_length(n, p):
+    q, pk, pv, ok, ov, lens = attention_case(3, n, 4, 2, 128, p, 100, "bf16", seed=2)
+    lens = torch.tensor([100, 33, 0], dtype=torch.int32, device="cuda")
+    want = ops().shared_prefix_attention(q, pk, pv, ok, ov, lens)
+    for i, m in enumerate(lens.tolist()):
+        ok[i, m:], ov[i, m:] = math.nan, math.inf
+    assert torch.equal(ops().shared_prefix_attention(q, pk, pv, ok, ov, lens), want)
+    # lengths beyond the room and below zero count as the room and zero
+    assert torch.equal(ops().shared_prefix_attention(q, pk, pv, ok[:1].expand(3, -1, -1, -1), ov[:1].expand(3, -1, -1, -1),
+                                                     torch.tensor([100, 1000, -5], dtype=torch.int32, device="cuda"))[:1], want[:1])
+
+
+@pytest.mark.gpu
+def test_shared_prefix_attention_empty_rows_strides_and_scale():
+    # no prefix, own lengths below the queries: the first queries see nothing
+    q, _, _, ok, ov, _ = attention_case(2, 40, 4, 2, 64, 0, 50, "f16", seed=3)
+    lens = torch.tensor([50, 7], dtype=torch.int32, device="cuda")
+    out, lse = ops().shared_prefix_attention(q, None, None, ok, ov, lens, return_lse=True)
+    assert not out[1, :33].any() and (lse[1, :, :33] == -math.inf).all() and torch.isfinite(lse[1, :, 33:]).all()
+    # q, k, v as views of one projection's rows; keys with heads outside tokens
+    b, n, h, d = 2, 40, 4, 64
+    g = torch.Generator().manual_seed(4)
+    qkv = torch.randn(b, n, 3 * h * d, generator=g).half().cuda()
+    q, k, v = (t.view(b, n, h, d) for t in qkv.split(h * d, -1))
+    pre = torch.randn(h, 300, d, generator=g).half().cuda().transpose(0, 1)
+    got = ops().shared_prefix_attention(q, pre, pre, k, v, scale=0.3)
+    assert torch.equal(got, ops().shared_prefix_attention(q.contiguous(), pre.contiguous(), pre.contiguous(), k.contiguous(), v.contiguous(), scale=0.3))
+    want, _, tol, _ = attention64(q, pre, pre, k, v, None, True, 0.3)
+    within(got, want, tol + rounding(q.dtype, want.abs() + tol), "views")
+    # scores far apart: the largest key alone remains
+    big = torch.zeros(1, 1, 1, 64).half().cuda()
+    big[..., 0] = 200
+    keys = torch.zeros(70, 1, 64).half().cuda()
+    keys[:, 0, 0] = torch.arange(70).half().cuda() * 4
+    vals = torch.randn(70, 1, 64, generator=g).half().cuda()
+    assert torch.equal(ops().shared_prefix_attention(big, keys, vals)[0, 0, 0], vals[69, 0])
+    assert ops().shared_prefix_attention(q[:0], pre, pre, k[:0], v[:0]).shape == (0, n, h, d)
+    assert ops().shared_prefix_attention(q[:, :0], pre, pre, k, v).shape == (b, 0, h, d)
+    assert not ops().shared_prefix_attention(q, None, None, k[:, :0], v[:, :0]).any()
+
+
+# ---- a block of them, streams, graphs --------------------------------------------------------------------------------------------
+
+def block(x, y, mod, weights, prefix_k, prefix_v, lens, heads, kv_heads, dim):
+    """norm -> qkv in 8 bits -> attention behind the shared prefix -> projection in 8 bits -> gate, residual, norm."""
+    b, s, d = x.shape
+    gate, scale, shift = mod.chunk(3, 1)
+    r, h = ops().gated_norm_fwd(x, y, gate=gate, scale=scale, shift=shift, pre="rms")
+    qkv = ops().linear_i8(h.view(b * s, d), *weights["qkv"]).view(b, s, -1)
+    q, k, v = qkv.split([heads * dim, kv_heads * dim, kv_heads * dim], -1)
+    q, k, v = q.view(b, s, heads, dim), k.view(b, s, kv_heads, dim), v.view(b, s, kv_heads, dim)
+    o = ops().shared_prefix_attention(q, prefix_k, prefix_v, k, v, lens)
+    z = ops().linear_i8(o.view(b * s, heads * dim), *weights["out"]).view(b, s, d)
+    r2, h2 = ops().gated_norm_fwd(r, z, gate=gate, scale=scale, shift=shift, post="layer", pre="layer")
+    return dict(r=r, h=h, qkv=qkv, o=o, z=z, r2=r2, h2=h2)
+
+
+def block_inputs(seed=0, b=3, s=45, d=320, heads=4, kv_heads=2, dim=64, p=300):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *sh: torch.randn(*sh, generator=g).bfloat16().cuda()  # noqa: E731
+    weights = {}
+    for name, out, cols in (("qkv", (heads + 2 * kv_heads) * dim, d), ("out", d, heads * dim)):
+        w = torch.randn(out, cols, generator=g).cuda() / math.sqrt(cols)
+        weights[name] = (*ops().quantize_rows(w), torch.randn(out, generator=g).cuda())
+    lens = torch.tensor([s] * b, dtype=torch.int32, device="cuda")
+    return (rnd(b, s, d), rnd(b, s, d), rnd(b, 3 * d) * 0.3, weights, rnd(p, kv_heads, dim), rnd(p, kv_heads, dim), lens, heads, kv_heads, dim)
+
+
+@pytest.mark.gpu
+def test_block_of_the_operators():
+    args = block_inputs()
+    got = block(*args)
+    x, y, mod, weights, pk, pv, lens, heads, kv_heads, dim = args
+    b, s, d = x.shape
+    u = half_step(torch.bfloat16)
+    gate, scale, shift = mod.chunk(3, 1)
+    # every stage against its formula in 64 bits on what the stage before it gave
+    val, tol = norm64(x, y, gate=gate, scale=scale, shift=shift, pre="rms")
+    for n in ("r", "h"):
+        within(got[n], val[n], tol[n] + u * val[n].abs(), n)
+
+    def linear(inp, w):
+        qa, sa = quant_np(inp.reshape(b * s, -1).float().cpu().numpy())
+        qw = w[0].cpu().numpy()[:, :qa.shape[1]]
+        return gemm64(qa, sa, qw, w[1].cpu().numpy(), w[2].cpu().numpy(), "bias", None, torch.bfloat16)
+    within(got["qkv"].view(b * s, -1), *linear(got["h"], weights["qkv"]), "qkv")
+    q, k, v = got["qkv"].split([heads * dim, kv_heads * dim, kv_heads * dim], -1)
+    want, _, t, _ = attention64(q.view(b, s, heads, dim), pk, pv, k.view(b, s, kv_heads, dim), v.view(b, s, kv_heads, dim), lens, True)
+    within(got["o"], want, t + rounding(torch.bfloat16, want.abs() + t), "attention")
+    within(got["z"].view(b * s, -1), *linear(got["o"], weights["out"]), "projection")
+    val, tol = norm64(got["r"], got["z"], gate=gate, scale=scale, shift=shift, post="layer", pre="layer")
+    within(got["r2"], val["r"], tol["r"] + u * val["r"].abs(), "r2")
+    within(got["h2"], val["h"], tol["h"] + u * val["h"].abs(), "h2")
+
+
+@pytest.mark.gpu
+def test_block_on_side_streams_and_in_graphs():
+    args, other = block_inputs(), block_inputs(seed=9)
+    want, want2 = block(*args), block(*other)
+    gr, gh = torch.randn_like(args[0]), torch.randn_like(args[0])
+    gate, scale, shift = args[2].chunk(3, 1)
+    vjp = lambda a: ops().gated_norm_vjp(gr, gh, a[0], a[1], gate=a[2].chunk(3, 1)[0], scale=a[2].chunk(3, 1)[1], shift=a[2].chunk(3, 1)[2],  # noqa: E731
+                                         post="rms", pre="layer")
+    want_g, want_g2 = vjp(args), vjp(other)
+    # two calls at once on two streams
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s1):
+        a, ag = block(*args), vjp(args)
+    with torch.cuda.stream(s2):
+        c, cg = block(*other), vjp(other)
+    torch.cuda.synchronize()
+    for n in want:
+        assert torch.equal(a[n], want[n]) and torch.equal(c[n], want2[n]), n
+    for n in want_g:
+        if want_g[n] is not None:
+            assert torch.equal(ag[n], want_g[n]) and torch.equal(cg[n], want_g2[n]), n
+    # two graphs, replayed in turn with eager work between, on changing inputs
+    graphs = []
+    for inp in (args, other):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            res, grads = block(*inp), vjp(inp)
+        graphs.append((graph, res, grads, inp))
+    for turn in range(3):
+        for graph, res, grads, inp in graphs:
+            inp[0].copy_(torch.randn_like(inp[0]))
+            inp[6].fill_(45 - turn)
+            graph.replay()
+            eager, eager_g = block(*inp), vjp(inp)
+            torch.cuda.synchronize()
+            for n in eager:
+                assert torch.equal(res[n], eager[n]), (turn, n)
+            for n in eager_g:
+                assert eager_g[n] is None or torch.equal(grads[n], eager_g[n]), (turn, n)
+
+
+@pytest.mark.gpu
+def test_gated_norm_with_gradients_is_refused_under_capture():
+    x = torch.randn(1, 4, 64, device="cuda", requires_grad=True)
+    ops().gated_norm(x)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(native().NativeError, match="captured"):
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device="cuda")
+            ops().gated_norm(x)
+
+
+# ---- refusals (no GPU) --------------------------------------------------------------------------------------------------------------
+
+def test_block_operators_refuse_cpu_tensors_and_wrong_arguments():
+    o, err = ops(), native().NativeError
+    x = torch.zeros(1, 2, 8)
+    for call in (lambda: o.gated_norm(x), lambda: o.gated_norm_vjp(x, x, x), lambda: o.quantize_rows(x[0]),
+                 lambda: o.gemm_i8(torch.zeros(1, 128, dtype=torch.int8), torch.ones(1), torch.zeros(1, 128, dtype=torch.int8), torch.ones(1)),
+                 lambda: o.linear_i8(x[0], torch.zeros(4, 128, dtype=torch.int8), torch.ones(4)),
+                 lambda: o.shared_prefix_attention(torch.zeros(1, 1, 1, 64, dtype=torch.float16), None, None)):
+        with pytest.raises(err, match="HIP device"):
+            call()
+    with pytest.raises(err, match="no such inputs"):
+        o.gated_norm_vjp(x, x, x, wanted=("z",))
+
+
+@pytest.mark.gpu
+def test_block_operators_refuse_wrong_shapes_and_types():
+    o, err = ops(), native().NativeError
+    x = torch.zeros(2, 3, 64, device="cuda")
+    i8 = lambda *s: torch.zeros(*s, dtype=torch.int8, device="cuda")  # noqa: E731
+    one = lambda n: torch.ones(n, device="cuda")  # noqa: E731
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda")  # noqa: E731
+    bad = [lambda: o.gated_norm(x[0]), lambda: o.gated_norm(x.double()), lambda: o.gated_norm(x, x[:1]), lambda: o.gated_norm(x, x.half()),
+           lambda: o.gated_norm(x, gate=one(64)), lambda: o.gated_norm(x, x, gate=one(63)), lambda: o.gated_norm(x, x, gate=one(64).half()),
+           lambda: o.gated_norm(x, weight=torch.ones(2, 64, device="cuda")), lambda: o.gated_norm(x, pre="none"), lambda: o.gated_norm(x, post="rms"),
+           lambda: o.gated_norm(x, x, post_weight=one(64)), lambda: o.gated_norm(x, eps=0.0), lambda: o.gated_norm(x, eps=math.nan),
+           lambda: o.gated_norm(x, residual_scale=math.inf), lambda: o.gated_norm(x, weight=torch.ones(64)),
+           lambda: o.gated_norm(torch.zeros(1, 1, 16385, device="cuda")),
+           lambda: o.gated_norm_vjp(x[:1], None, x),
+           lambda: o.quantize_rows(x), lambda: o.quantize_rows(x[0].double()), lambda: o.quantize_rows(torch.zeros(1, 130049, device="cuda")),
+           lambda: o.quantize_rows(torch.zeros(2, 0, device="cuda")),
+           lambda: o.gemm_i8(i8(2, 64), one(2), i8(2, 64), one(2)), lambda: o.gemm_i8(i8(2, 128), one(2), i8(2, 256), one(2)),
+           lambda: o.gemm_i8(i8(2, 128), one(3), i8(2, 128), one(2)), lambda: o.gemm_i8(i8(2, 128), one(2), i8(2, 128), one(2), epi="relu"),
+           lambda: o.gemm_i8(i8(2, 128), one(2), i8(2, 128), one(2), epi="resid"), lambda: o.gemm_i8(i8(2, 128), one(2), i8(2, 128), one(2).half()),
+           lambda: o.gemm_i8(i8(2, 128), one(2), i8(2, 128), one(2), resid=one(4).view(2, 2)),
+           lambda: o.gemm_i8(i8(2, 128), one(2), i8(0, 128), one(0)),
+           lambda: o.linear_i8(x[0], i8(4, 64), one(4)),
+           lambda: o.shared_prefix_attention(h(1, 1, 2, 64), None, None), lambda: o.shared_prefix_attention(h(1, 1, 2, 32), h(4, 2, 32), h(4, 2, 32)),
+           lambda: o.shared_prefix_attention(h(1, 1, 3, 64), h(4, 2, 64), h(4, 2, 64)), lambda: o.shared_prefix_attention(h(1, 1, 2, 64), h(4, 2, 64), None),
+           lambda: o.shared_prefix_attention(h(1, 1, 2, 64), h(4, 2, 64), h(5, 2, 64)), lambda: o.shared_prefix_attention(h(1, 1, 2, 64).float(), None, None),
+           lambda: o.shared_prefix_attention(h(1, 1, 2, 64), h(4, 2, 64).bfloat16(), h(4, 2, 64)),
+           lambda: o.shared_prefix_attention(h(2, 1, 2, 64), None, None, h(1, 4, 2, 64), h(1, 4, 2, 64)),
+           lambda: o.shared_prefix_attention(h(1, 1, 2, 64), h(4, 2, 64), h(4, 2, 64), scale=-1.0),
+           lambda: o.shared_prefix_attention(h(1, 1, 2, 64), None, None, h(1, 4, 2, 64), h(1, 4, 2, 64), torch.ones(1, dtype=torch.int64, device="cuda")),
+           lambda: o.shared_prefix_attention(h(1, 1, 2, 64), None, None, h(1, 4, 2, 64), h(1, 4, 2, 64), torch.ones(1, dtype=torch.int32))]
+    for i, call in enumerate(bad):
+        with pytest.raises(err):
+            call()
+            pytest.fail(f"call {i} was accepted")
+
+
+def test_c_entries_refuse_before_any_launch():
+    """Bad descriptors come back as CMDI_E_INVALID with a text (pointers that are never followed; no device here)."""
+    n = native()
+    lib, E_INVALID, P = n.load(), -1, 0x1000
+
+    def norm(**over):
+        d = n.GatedNormDesc(batch=1, seq=1, dim=8, post=0, pre=2, residual_scale=1.0, eps=1e-5, d_x=P, x_stride=(8, 8), y_stride=(8, 8))
+        for k, v in over.items():
+            setattr(d, k, (C.c_int64 * 2)(*v) if k.endswith("_stride") and isinstance(v, tuple) else v)
+        return d
+    bad = [dict(batch=-1), dict(batch=1 << 16, seq=1 << 15), dict(dim=0), dict(dim=16385), dict(dtype=3), dict(param_dtype=1), dict(post=3), dict(post=-1),
+           dict(pre=0), dict(eps=0.0), dict(eps=-1.0), dict(residual_scale=math.nan), dict(d_x=0), dict(post=1), dict(d_gate=P), dict(d_x=P + 2),
+           dict(d_post_weight=P, d_y=P), dict(x_stride=(-8, 8)), dict(d_scale=P, scale_stride=-1), dict(d_weight=P + 1)]
+    for over in bad:
+        assert lib.cmdi_gated_norm_fwd(C.byref(norm(**over)), P, P, 0) == E_INVALID, over
+        assert lib.cmdi_last_error(), over
+    assert lib.cmdi_gated_norm_fwd(None, P, P, 0) == E_INVALID
+    assert lib.cmdi_gated_norm_fwd(C.byref(norm()), P, 0, 0) == E_INVALID
+    assert lib.cmdi_gated_norm_fwd(C.byref(norm()), P + 2, P, 0) == E_INVALID
+    assert lib.cmdi_gated_norm_fwd(C.byref(norm(batch=0, d_x=0)), 0, 0, 0) == 0
+    gd = lambda **kw: n.GatedNormGrads(**kw)  # noqa: E731
+    for over, grads in ((dict(), gd(d_gy=P)), (dict(), gd(d_gweight=P)), (dict(d_y=P), gd(d_ggate=P)), (dict(d_weight=P), gd(d_gweight=P)),
+                        (dict(d_weight=P), gd(d_gweight=P, d_work=P, work_bytes=4)), (dict(), gd(d_gr=P + 1)),
+                        (dict(d_weight=P, seq=0), gd(d_gweight=P))):
+        assert lib.cmdi_gated_norm_vjp(C.byref(norm(**over)), C.byref(grads), 0) == E_INVALID, (over,)
+    assert lib.cmdi_gated_norm_vjp(C.byref(norm()), None, 0) == E_INVALID
+    assert lib.cmdi_gated_norm_vjp_workspace(C.byref(norm(dim=0)), C.byref(gd())) == E_INVALID
+    assert lib.cmdi_gated_norm_vjp_workspace(C.byref(norm()), C.byref(gd(d_gx=P))) == 0
+    assert lib.cmdi_gated_norm_vjp_workspace(C.byref(norm(d_weight=P)), C.byref(gd(d_gweight=P))) > 0
+
+    ok = dict(x=P, dtype=0, rows=1, cols=8, ld=8, q=P, kp=128, scale=P)
+    for over in (dict(dtype=5), dict(rows=-1), dict(rows=(1 << 22) + 1), dict(cols=0), dict(ld=-1), dict(kp=4), dict(kp=130), dict(kp=130176, cols=130100),
+                 dict(x=0), dict(q=0), dict(scale=0), dict(q=P + 8), dict(x=P + 1), dict(scale=P + 2)):
+        assert lib.cmdi_quant_rows_i8(*{**ok, **over}.values(), 0) == E_INVALID, over
+    assert lib.cmdi_quant_rows_i8(*{**ok, "rows": 0, "x": 0}.values(), 0) == 0
+
+    ok = dict(a=P, sa=P, w=P, sw=P, bias=0, resid=0, c=P, m=1, n=1, k=128, lda=128, ldw=128, ldc=1, ldr=1, dtype=0, epi=0)
+    for over in (dict(dtype=4), dict(epi=2), dict(epi=3), dict(m=-1), dict(n=0), dict(k=64), dict(k=200), dict(k=130176, lda=130176, ldw=130176), dict(lda=64),
+                 dict(ldw=136), dict(lda=(1 << 22) + 16), dict(ldc=0), dict(a=0), dict(sa=0), dict(w=0), dict(sw=0), dict(c=0), dict(a=P + 8), dict(w=P + 4),
+                 dict(c=P + 1), dict(bias=P + 2), dict(epi=3, resid=P, ldr=0), dict(m=1 << 30, n=1 << 20, ldc=1 << 20)):
+        assert lib.cmdi_gemm_i8(*{**ok, **over}.values(), 0) == E_INVALID, over
+    assert lib.cmdi_gemm_i8(*{**ok, "m": 0, "a": 0}.values(), 0) == 0
+
+    def attn(**over):
+        d = n.PrefixAttentionDesc(batch=1, queries=1, heads=2, kv_heads=1, dim=64, prefix=4, own_max=4, dtype=1, scale=1.0, d_q=P, d_prefix_k=P,
+                                  d_prefix_v=P, d_own_k=P, d_own_v=P)
+        d.prefix_k_stride = d.prefix_v_stride = (C.c_int64 * 2)(64, 64)
+        d.q_stride = d.own_k_stride = d.own_v_stride = (C.c_int64 * 3)(256, 64, 64)
+        for k, v in over.items():
+            setattr(d, k, (C.c_int64 * len(v))(*v) if isinstance(v, tuple) else v)
+        return d
+    for over in (dict(batch=-1), dict(queries=-1), dict(prefix=-1), dict(own_max=-1), dict(heads=0), dict(kv_heads=0), dict(heads=3, kv_heads=2), dict(dim=96),
+                 dict(dtype=0), dict(scale=0.0), dict(scale=math.inf), dict(scale=-1.0), dict(batch=1 << 16, queries=1 << 15), dict(prefix=(1 << 31) - 8),
+                 dict(d_q=0), dict(d_prefix_v=0), dict(d_own_k=0), dict(d_q=P + 8), dict(q_stride=(256, 64, 4)), dict(prefix_k_stride=(-64, 64)),
+                 dict(own_v_stride=(0, (1 << 23) + 8, 64))):
+        assert lib.cmdi_prefix_attention(C.byref(attn(**over)), P, 0, P, 1 << 40, 0) == E_INVALID, over
+        assert lib.cmdi_prefix_attention_workspace(C.byref(attn(**over))) == E_INVALID, over
+    assert lib.cmdi_prefix_attention(C.byref(attn()), 0, 0, 0, 0, 0) == E_INVALID
+    assert lib.cmdi_prefix_attention(C.byref(attn()), P, P + 2, 0, 0, 0) == E_INVALID
+    assert lib.cmdi_prefix_attention(C.byref(attn(prefix=100000)), P, 0, 0, 0, 0) == E_INVALID      # workspace missing
+    assert lib.cmdi_prefix_attention_workspace(C.byref(attn(prefix=0, own_max=0))) == 0
+    assert lib.cmdi_prefix_attention(C.byref(attn(queries=0, d_q=0)), 0, 0, 0, 0, 0) == 0
+    assert lib.cmdi_prefix_attention(None, P, 0, 0, 0, 0) == E_INVALID
