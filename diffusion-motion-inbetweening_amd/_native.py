@@ -138,13 +138,15 @@ SIGNATURES = {
     "cmdi_clip_encode_text": (C.c_int, [_VP, _VP, _I32, _VP, _VP]),
     "cmdi_pack_x6": (C.c_int, [_VP, _VP, _I64, _I32, _VP]),
     "cmdi_gemm_x6": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _I32, _VP]),
-    "cmdi_gated_norm_fwd": (C.c_int, [C.POINTER(GatedNormDesc), _VP, _VP, _VP]),
-    "cmdi_gated_norm_vjp": (C.c_int, [C.POINTER(GatedNormDesc), C.POINTER(GatedNormGrads), _VP]),
-    "cmdi_gated_norm_vjp_workspace": (_I64, [C.POINTER(GatedNormDesc), C.POINTER(GatedNormGrads)]),
+    # descriptors of the block operators: a structure above by reference, or bytes of the same layout (ops.py)
+    "cmdi_gated_norm_fwd": (C.c_int, [_VP, _VP, _VP, _VP]),
+    "cmdi_gated_norm_vjp": (C.c_int, [_VP, _VP, _VP]),
+    "cmdi_gated_norm_vjp_workspace": (_I64, [_VP, _VP]),
     "cmdi_quant_rows_i8": (C.c_int, [_VP, _I32, _I64, _I32, _I64, _VP, _I32, _VP, _VP]),
     "cmdi_gemm_i8": (C.c_int, [_VP] * 7 + [_I32] * 3 + [_I64] * 4 + [_I32] * 2 + [_VP]),
-    "cmdi_prefix_attention": (C.c_int, [C.POINTER(PrefixAttentionDesc), _VP, _VP, _VP, _I64, _VP]),
-    "cmdi_prefix_attention_workspace": (_I64, [C.POINTER(PrefixAttentionDesc)]),
+    "cmdi_linear_i8": (C.c_int, [_VP, _I32, _I32, _I32, _I64, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _I64, _I64, _I64, _I32, _VP, _I64, _VP]),
+    "cmdi_prefix_attention": (C.c_int, [_VP, _VP, _VP, _VP, _I64, _VP]),
+    "cmdi_prefix_attention_workspace": (_I64, [_VP]),
     "cmdi_philox4x32_10": (None, [C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
     "cmdi_workspace_bytes": (_I64, [_VP]),
     "cmdi_pipeline_parts": (C.c_int, [_VP]),

@@ -123,6 +123,30 @@ int64_t prefix_blocks(const PrefixAttnArgs& a, const PrefixAttnPlan& p) {
     return most;
 }
 
+// argument checks of the product, then (go) its launch
+int gemm_i8_checked(const void* d_a, const float* d_a_scale, const void* d_w, const float* d_w_scale, const float* d_bias, const void* d_resid,
+                 void* d_c, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldw, int64_t ldc, int64_t ldr, int32_t dtype, int32_t epi,
+                 cmdi_stream stream, bool go) {
+    if (!dt_known(dtype)) return fail(CMDI_E_INVALID, "dtype must be CMDI_DT_F32, CMDI_DT_BF16 or CMDI_DT_F16");
+    if (epi != 0 && epi != 1 && epi != 3) return fail(CMDI_E_INVALID, "epi must be 0 (bias), 1 (bias+gelu) or 3 (bias+residual)");
+    if (m < 0 || n < 1 || k < kI8KAlign || k % kI8KAlign != 0 || k > kI8MaxK) return fail(CMDI_E_INVALID, "m >= 0, n >= 1, k a multiple of 128 up to 130048");
+    if (lda < k || ldw < k || lda % 16 != 0 || ldw % 16 != 0 || lda > (1 << 22) || ldw > (1 << 22))
+        return fail(CMDI_E_INVALID, "lda and ldw must be multiples of 16 from k to 2^22");
+    if (ldc < n || (epi == 3 && ldr < n)) return fail(CMDI_E_INVALID, "ldc and ldr must be at least n");
+    if (m == 0) return CMDI_OK;
+    if (!d_a || !d_a_scale || !d_w || !d_w_scale || !d_c) return fail(CMDI_E_INVALID, "null tensor");
+    if (epi == 3 && !d_resid) return fail(CMDI_E_INVALID, "residual epilogue needs d_resid");
+    if (!at16(d_a) || !at16(d_w)) return fail(CMDI_E_INVALID, "a and w must be 16-byte aligned");
+    if (!at_elem(d_c, dtype) || !at_elem(d_resid, dtype) || !at_elem(d_a_scale, CMDI_DT_F32) || !at_elem(d_w_scale, CMDI_DT_F32) || !at_elem(d_bias, CMDI_DT_F32))
+        return fail(CMDI_E_INVALID, "a tensor is not aligned to its element");
+    if ((int64_t)((m + 63) / 64) * ((n + 63) / 64) > kMaxBlocks) return fail(CMDI_E_INVALID, "m * n too large");
+    GemmI8Args p{static_cast<const int8_t*>(d_a), static_cast<const int8_t*>(d_w), d_a_scale, d_w_scale, d_bias, epi == 3 ? d_resid : nullptr, d_c,
+                 m, n, k, lda, ldw, ldc, ldr, dtype, epi};
+    if (!go) return CMDI_OK;
+    HIPCHK(launch_gemm_i8(p, static_cast<hipStream_t>(stream)));
+    return CMDI_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -183,23 +207,23 @@ int cmdi_quant_rows_i8(const void* d_x, int32_t dtype, int64_t rows, int32_t col
 int cmdi_gemm_i8(const void* d_a, const float* d_a_scale, const void* d_w, const float* d_w_scale, const float* d_bias, const void* d_resid,
                  void* d_c, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldw, int64_t ldc, int64_t ldr, int32_t dtype, int32_t epi,
                  cmdi_stream stream) {
-    if (!dt_known(dtype)) return fail(CMDI_E_INVALID, "dtype must be CMDI_DT_F32, CMDI_DT_BF16 or CMDI_DT_F16");
-    if (epi != 0 && epi != 1 && epi != 3) return fail(CMDI_E_INVALID, "epi must be 0 (bias), 1 (bias+gelu) or 3 (bias+residual)");
-    if (m < 0 || n < 1 || k < kI8KAlign || k % kI8KAlign != 0 || k > kI8MaxK) return fail(CMDI_E_INVALID, "m >= 0, n >= 1, k a multiple of 128 up to 130048");
-    if (lda < k || ldw < k || lda % 16 != 0 || ldw % 16 != 0 || lda > (1 << 22) || ldw > (1 << 22))
-        return fail(CMDI_E_INVALID, "lda and ldw must be multiples of 16 from k to 2^22");
-    if (ldc < n || (epi == 3 && ldr < n)) return fail(CMDI_E_INVALID, "ldc and ldr must be at least n");
-    if (m == 0) return CMDI_OK;
-    if (!d_a || !d_a_scale || !d_w || !d_w_scale || !d_c) return fail(CMDI_E_INVALID, "null tensor");
-    if (epi == 3 && !d_resid) return fail(CMDI_E_INVALID, "residual epilogue needs d_resid");
-    if (!at16(d_a) || !at16(d_w)) return fail(CMDI_E_INVALID, "a and w must be 16-byte aligned");
-    if (!at_elem(d_c, dtype) || !at_elem(d_resid, dtype) || !at_elem(d_a_scale, CMDI_DT_F32) || !at_elem(d_w_scale, CMDI_DT_F32) || !at_elem(d_bias, CMDI_DT_F32))
-        return fail(CMDI_E_INVALID, "a tensor is not aligned to its element");
-    if ((int64_t)((m + 63) / 64) * ((n + 63) / 64) > kMaxBlocks) return fail(CMDI_E_INVALID, "m * n too large");
-    GemmI8Args p{static_cast<const int8_t*>(d_a), static_cast<const int8_t*>(d_w), d_a_scale, d_w_scale, d_bias, epi == 3 ? d_resid : nullptr, d_c,
-                 m, n, k, lda, ldw, ldc, ldr, dtype, epi};
-    HIPCHK(launch_gemm_i8(p, static_cast<hipStream_t>(stream)));
-    return CMDI_OK;
+    return gemm_i8_checked(d_a, d_a_scale, d_w, d_w_scale, d_bias, d_resid, d_c, m, n, k, lda, ldw, ldc, ldr, dtype, epi, stream, true);
+}
+
+int cmdi_linear_i8(const void* d_x, int32_t dtype, int32_t m, int32_t cols, int64_t ldx, const void* d_w, const float* d_w_scale,
+                   const float* d_bias, const void* d_resid, void* d_c, int32_t n, int32_t kp, int64_t ldw, int64_t ldc, int64_t ldr,
+                   int32_t epi, void* d_work, int64_t work_bytes, cmdi_stream stream) {
+    if (m < 0 || cols < 1 || kp != (int64_t)(cols + (int64_t)kI8KAlign - 1) / kI8KAlign * kI8KAlign)
+        return fail(CMDI_E_INVALID, "m >= 0, cols >= 1, kp = cols rounded up to 128");
+    if (m > 0 && (!d_work || !at16(d_work) || work_bytes < (int64_t)m * (kp + 4)))
+        return fail(CMDI_E_INVALID, "workspace must be 16-byte aligned and hold m * (kp + 4) bytes");
+    int8_t* q = static_cast<int8_t*>(d_work);
+    float* scale = reinterpret_cast<float*>(q + (int64_t)m * kp);
+    // the product's own checks first (m = 0: they need no tensors), so that a refused call has launched nothing
+    const int rc = gemm_i8_checked(q, scale, d_w, d_w_scale, d_bias, d_resid, d_c, m, n, kp, kp, ldw, ldc, ldr, dtype, epi, nullptr, false);
+    if (rc != CMDI_OK || m == 0) return rc;
+    if (int e = cmdi_quant_rows_i8(d_x, dtype, m, cols, ldx, q, kp, scale, stream)) return e;
+    return gemm_i8_checked(q, scale, d_w, d_w_scale, d_bias, d_resid, d_c, m, n, kp, kp, ldw, ldc, ldr, dtype, epi, stream, true);
 }
 
 int64_t cmdi_prefix_attention_workspace(const cmdi_prefix_attention_desc* d) {

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -22,104 +23,113 @@ from . import _native as N
 __all__ = ["gated_norm", "gated_norm_fwd", "gated_norm_vjp", "quantize_rows", "gemm_i8", "linear_i8", "shared_prefix_attention"]
 
 _EPI = {"bias": 0, "gelu": 1, "resid": 3}
+_CONTIGUOUS = torch.contiguous_format
+# the descriptors' C layouts (native alignment): packing one costs a quarter of a microsecond, a ctypes structure two
+_NORM_DESC = struct.Struct("@7i2f2P4q3P3q4P")
+_NORM_GRADS = struct.Struct("@2P4q10Pq")
+_PREFIX_DESC = struct.Struct("@9if5P13qP")
 
 
 def _refuse(what: str):
     raise N.NativeError(what)
 
 
-def _on_device(t: torch.Tensor, name: str) -> torch.device:
+def _on_device(t: torch.Tensor, name: str) -> int:
+    """The HIP device's index of a tensor."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         _refuse(f"{name} must be on a HIP device (there is no CPU path), got {t.device}")
-    return t.device
+    return t.get_device()
 
 
-def _same_device(device: torch.device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            _refuse(f"{name} is on {t.device}, the call's tensors on {device}")
+def _elsewhere(name: str, t: torch.Tensor, device: int):
+    _refuse(f"{name} is on {t.device}, the call's tensors on cuda:{device}")
 
 
-class _On:
-    """The tensors' device made current for the launches (nothing to do where it is already)."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.before)
+def _launch(device: int, entry, *args):
+    """entry(*args, current stream of `device`) with that device current; raises what the entry reports."""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch._C._cuda_getDevice() == device:
+        rc = entry(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args, stream)
+    if rc:
+        N.check(rc)
 
 
 # ---- gated norm -------------------------------------------------------------------------------------------------------------
 
-def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """t as [batch, seq, dim] rows that the kernels can read in place (contiguous columns), or a contiguous copy."""
-    if t.dim() != 3:
-        _refuse(f"{name} must be [batch, seq, dim], got {tuple(t.shape)}")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
-        _refuse(f"{name} must be {tuple(like.shape)} {like.dtype}, got {tuple(t.shape)} {t.dtype}")
-    return t if t.shape[2] == 1 or t.stride(2) == 1 else t.contiguous()
+def _rows(t: torch.Tensor, name: str, like: torch.Tensor, device: int) -> torch.Tensor:
+    """t as rows like x's that the kernels can read in place (contiguous columns), or a contiguous copy."""
+    if t.shape != like.shape or t.dtype != like.dtype:
+        _refuse(f"{name} must be {list(like.shape)} {like.dtype}, got {list(t.shape)} {t.dtype}")
+    if t.get_device() != device:
+        _elsewhere(name, t, device)
+    return t if t.stride()[2] == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def _param(t: Optional[torch.Tensor], name: str, x: torch.Tensor, dtype, per_sample: bool) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    b, _, d = x.shape
-    if t.dtype != dtype:
-        _refuse(f"{name} must be {dtype} like the other parameters, got {t.dtype}")
-    if t.shape != (d,) and not (per_sample and t.shape == (b, d)):
-        _refuse(f"{name} must be [{d}]{f' or [{b}, {d}]' if per_sample else ''}, got {tuple(t.shape)}")
-    if (d > 1 and t.stride(-1) != 1) or (t.dim() == 2 and t.stride(0) == 0):
-        t = t.contiguous()
-    return t
-
-
-def _stride(t: Optional[torch.Tensor]) -> int:
-    # a [1, dim] parameter still belongs to its sample (its gradient is [1, dim]): any stride but 0 says so
-    return 0 if t is None or t.dim() == 1 else max(1, t.stride(0)) if t.shape[0] > 1 else t.shape[1]
+_PARAMS = ("gate", "scale", "shift", "weight", "bias", "post_weight", "post_bias")
 
 
 def _norm_desc(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps):
-    """(desc, the tensors it points at in the order x, y, gate, scale, shift, weight, bias, post_weight, post_bias)."""
+    """(packed descriptor, the tensors it points at in the order x, y, *_PARAMS, device)."""
     device = _on_device(x, "x")
-    if x.dtype not in N.CMDI_DT:
-        _refuse(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    dtype, shape = x.dtype, x.shape
+    code = N.CMDI_DT.get(dtype)
+    if code is None or len(shape) != 3:
+        _refuse(f"x must be [batch, seq, dim] float32, bfloat16 or float16, got {list(shape)} {dtype}")
     if post not in N.CMDI_NORMS or pre not in ("rms", "layer"):
         _refuse(f"post must be 'none', 'rms' or 'layer' and pre 'rms' or 'layer', got {post!r}, {pre!r}")
-    x = _rows(x, "x")
+    b, s, d = shape
+    xs = x.stride()
+    if xs[2] != 1 and d != 1:
+        x = x.contiguous()
+        xs = x.stride()
+    tensors, ptrs, strides, pdt = [x, y], [], [], None
     if y is not None:
-        y = _rows(y, "y", x)
-    params = dict(gate=gate, scale=scale, shift=shift, weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias)
-    _same_device(device, y=y, **params)
-    dtypes = {t.dtype for t in params.values() if t is not None}
-    dtype = dtypes.pop() if dtypes else x.dtype
-    if dtypes or dtype not in (x.dtype, torch.float32):
-        _refuse(f"gate, scale, shift, weights and biases must all be float32 or all {x.dtype}")
-    p = {k: _param(t, k, x, dtype, k in ("gate", "scale", "shift")) for k, t in params.items()}
-    b, s, d = x.shape
-    desc = N.GatedNormDesc(b, s, d, N.CMDI_DT[x.dtype], N.CMDI_DT[dtype], N.CMDI_NORMS[post], N.CMDI_NORMS[pre], float(residual_scale),
-                           float(eps), N.ptr(x), N.ptr(y), (C.c_int64 * 2)(x.stride(0), x.stride(1)),
-                           (C.c_int64 * 2)(*((y.stride(0), y.stride(1)) if y is not None else (0, 0))), N.ptr(p["gate"]), N.ptr(p["scale"]),
-                           N.ptr(p["shift"]), _stride(p["gate"]), _stride(p["scale"]), _stride(p["shift"]), N.ptr(p["weight"]), N.ptr(p["bias"]),
-                           N.ptr(p["post_weight"]), N.ptr(p["post_bias"]))
-    return desc, (x, y, *p.values())
+        tensors[1] = y = _rows(y, "y", x, device)
+        ys, yp = y.stride(), y.data_ptr()
+    else:
+        ys, yp = (0, 0), 0
+    for i, t in enumerate((gate, scale, shift, weight, bias, post_weight, post_bias)):
+        step = 0
+        if t is not None:
+            if pdt is None:
+                pdt = t.dtype
+            ts = t.shape
+            if t.dtype != pdt or (pdt != dtype and pdt != torch.float32):
+                _refuse(f"gate, scale, shift, weights and biases must all be float32 or all {dtype}, got {_PARAMS[i]} {t.dtype}")
+            if t.get_device() != device:
+                _elsewhere(_PARAMS[i], t, device)
+            if len(ts) == 1 and ts[0] == d:
+                if t.stride()[0] != 1 and d > 1:
+                    t = t.contiguous()
+            elif i < 3 and len(ts) == 2 and ts[0] == b and ts[1] == d:
+                st = t.stride()
+                if (st[1] != 1 and d > 1) or st[0] == 0:
+                    t = t.contiguous()
+                    st = t.stride()
+                # a [1, dim] parameter still belongs to its sample (its gradient is [1, dim]): any stride but 0 says so
+                step = st[0] if b > 1 else d
+            else:
+                _refuse(f"{_PARAMS[i]} must be [{d}]{f' or [{b}, {d}]' if i < 3 else ''}, got {list(ts)}")
+            ptrs.append(t.data_ptr())
+        else:
+            ptrs.append(0)
+        tensors.append(t)
+        strides.append(step)
+    desc = _NORM_DESC.pack(b, s, d, code, code if pdt is None or pdt == dtype else 0, N.CMDI_NORMS[post], N.CMDI_NORMS[pre], residual_scale, eps,
+                           x.data_ptr(), yp, xs[0], xs[1], ys[0], ys[1], *ptrs[:3], *strides[:3], *ptrs[3:])
+    return desc, tensors, device
 
 
-def _norm_fwd(args, kw):
-    desc, tensors = _norm_desc(*args, **kw)
+def _norm_fwd(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps):
+    desc, tensors, device = _norm_desc(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps)
     x = tensors[0]
-    r, h = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with _On(x.device) as stream:
-        N.check(N.load().cmdi_gated_norm_fwd(C.byref(desc), N.ptr(r), N.ptr(h), stream))
+    r, h = torch.empty_like(x, memory_format=_CONTIGUOUS), torch.empty_like(x, memory_format=_CONTIGUOUS)
+    _launch(device, N.load().cmdi_gated_norm_fwd, desc, r.data_ptr(), h.data_ptr())
     return r, h
 
 
@@ -127,25 +137,24 @@ _NORM_INPUTS = ("x", "y", "gate", "scale", "shift", "weight", "bias", "post_weig
 
 
 def _norm_vjp(args, kw, gr, gh, wanted):
-    desc, tensors = _norm_desc(*args, **kw)
+    desc, tensors, device = _norm_desc(*args, **kw)
     x = tensors[0]
-    _same_device(x.device, grad_r=gr, grad_h=gh)
-    gr, gh = (None if g is None else _rows(g, n, x) for g, n in ((gr, "grad_r"), (gh, "grad_h")))
-    empty = x.numel() == 0
-    out = {n: None if t is None or n not in wanted else torch.zeros(t.shape, dtype=t.dtype, device=t.device) if empty else
-           torch.empty(t.shape, dtype=t.dtype, device=t.device) for n, t in zip(_NORM_INPUTS, tensors)}
-    if empty:
+    if gr is not None:
+        gr = _rows(gr, "grad_r", x, device)
+    if gh is not None:
+        gh = _rows(gh, "grad_h", x, device)
+    make = torch.zeros_like if x.numel() == 0 else torch.empty_like
+    out = {n: None if t is None or n not in wanted else make(t, memory_format=_CONTIGUOUS) for n, t in zip(_NORM_INPUTS, tensors)}
+    if x.numel() == 0:
         return out
-    pair = lambda g: (C.c_int64 * 2)(*((g.stride(0), g.stride(1)) if g is not None else (0, 0)))  # noqa: E731
-    grads = N.GatedNormGrads(N.ptr(gr), N.ptr(gh), pair(gr), pair(gh), *(N.ptr(out[n]) for n in _NORM_INPUTS), 0, 0)
+    rs, hs = (0, 0) if gr is None else gr.stride()[:2], (0, 0) if gh is None else gh.stride()[:2]
     lib = N.load()
-    need = lib.cmdi_gated_norm_vjp_workspace(C.byref(desc), C.byref(grads))
+    grads = [N.ptr(gr), N.ptr(gh), *rs, *hs, *(N.ptr(t) for t in out.values())]
+    need = lib.cmdi_gated_norm_vjp_workspace(desc, _NORM_GRADS.pack(*grads, 0, 0))
     if need < 0:
         N.check(int(need))
     work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    grads.d_work, grads.work_bytes = N.ptr(work), need
-    with _On(x.device) as stream:
-        N.check(lib.cmdi_gated_norm_vjp(C.byref(desc), C.byref(grads), stream))
+    _launch(device, lib.cmdi_gated_norm_vjp, desc, _NORM_GRADS.pack(*grads, N.ptr(work), need))
     return out
 
 
@@ -155,7 +164,7 @@ class _GatedNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.kw = kw
         ctx.save_for_backward(*args)
-        return _norm_fwd(args, kw)
+        return _norm_fwd(*args, **kw)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -178,19 +187,21 @@ def gated_norm(x, y=None, *, gate=None, residual_scale=1.0, post="none", post_we
     weight, bias, post_weight, post_bias [dim]; the parameters all float32 or all of x's type.  post 'none' | 'rms' | 'layer', pre
     'rms' | 'layer'.  Differentiable (once) in every tensor; a call that would record a backward pass while its stream is
     being captured is refused: capture gated_norm_fwd and gated_norm_vjp."""
-    args = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
-    kw = dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        if torch.cuda.is_current_stream_capturing():
-            _refuse("gated_norm with gradients cannot be captured: use gated_norm_fwd and gated_norm_vjp inside a graph")
-        return _GatedNorm.apply(kw, *args)
-    return _norm_fwd(args, kw)
+    if torch.is_grad_enabled():
+        args = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
+        for t in args:
+            if t is not None and t.requires_grad:
+                _on_device(x, "x")
+                if torch.cuda.is_current_stream_capturing():
+                    _refuse("gated_norm with gradients cannot be captured: use gated_norm_fwd and gated_norm_vjp inside a graph")
+                return _GatedNorm.apply(dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps), *args)
+    return _norm_fwd(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps)
 
 
 def gated_norm_fwd(x, y=None, *, gate=None, residual_scale=1.0, post="none", post_weight=None, post_bias=None, pre="layer", weight=None, bias=None,
                    scale=None, shift=None, eps=1e-5):
     """gated_norm without a backward pass -> (r, h)."""
-    return _norm_fwd((x, y, gate, scale, shift, weight, bias, post_weight, post_bias), dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps))
+    return _norm_fwd(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps)
 
 
 def gated_norm_vjp(grad_r, grad_h, x, y=None, *, gate=None, residual_scale=1.0, post="none", post_weight=None, post_bias=None, pre="layer", weight=None,
@@ -206,29 +217,60 @@ def gated_norm_vjp(grad_r, grad_h, x, y=None, *, gate=None, residual_scale=1.0, 
 
 # ---- the linear layer in 8-bit integers ---------------------------------------------------------------------------------------
 
+def _float_rows(x: torch.Tensor):
+    """(x [rows, cols] with contiguous columns, its type's code, device)."""
+    device = _on_device(x, "x")
+    code = N.CMDI_DT.get(x.dtype)
+    if code is None or x.dim() != 2:
+        _refuse(f"x must be [rows, cols] float32, bfloat16 or float16, got {list(x.shape)} {x.dtype}")
+    return x if x.stride()[1] == 1 or x.shape[1] == 1 else x.contiguous(), code, device
+
+
 def quantize_rows(x: torch.Tensor):
     """Rows of x [rows, cols] in 8 bits -> (q int8 [rows, cols rounded up to 128] with zeros behind the columns, scale float32
     [rows]); x ~ q * scale.  For weights [out, in] once, for activations [tokens, in] in every call."""
-    device = _on_device(x, "x")
-    if x.dim() != 2 or x.dtype not in N.CMDI_DT:
-        _refuse(f"x must be [rows, cols] float32, bfloat16 or float16, got {tuple(x.shape)} {x.dtype}")
+    x, code, device = _float_rows(x)
     rows, cols = x.shape
-    if cols > 1 and x.stride(1) != 1:
-        x = x.contiguous()
     kp = (cols + 127) // 128 * 128
-    q = torch.empty((rows, kp), dtype=torch.int8, device=device)
-    scale = torch.empty((rows,), dtype=torch.float32, device=device)
-    with _On(device) as stream:
-        N.check(N.load().cmdi_quant_rows_i8(N.ptr(x), N.CMDI_DT[x.dtype], rows, cols, x.stride(0), N.ptr(q), kp, N.ptr(scale), stream))
+    q = torch.empty((rows, kp), dtype=torch.int8, device=x.device)
+    scale = torch.empty((rows,), dtype=torch.float32, device=x.device)
+    _launch(device, N.load().cmdi_quant_rows_i8, x.data_ptr(), code, rows, cols, x.stride()[0], q.data_ptr(), kp, scale.data_ptr())
     return q, scale
 
 
-def _bytes_rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    if t.dim() != 2 or t.dtype != torch.int8:
-        _refuse(f"{name} must be int8 [rows, k], got {tuple(t.shape)} {t.dtype}")
-    if t.stride(1) != 1 or t.stride(0) % 16 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
+def _bytes_rows(t: torch.Tensor, name: str, device: int) -> torch.Tensor:
+    if t.dtype != torch.int8 or t.dim() != 2:
+        _refuse(f"{name} must be int8 [rows, k], got {list(t.shape)} {t.dtype}")
+    if t.get_device() != device:
+        _elsewhere(name, t, device)
+    st = t.stride()
+    if st[1] != 1 or st[0] % 16 or st[0] < t.shape[1] or t.data_ptr() % 16:
         t = t.contiguous()
     return t
+
+
+def _scales(t: torch.Tensor, name: str, size: int, device: int) -> torch.Tensor:
+    if t.dtype != torch.float32 or t.shape != (size,):
+        _refuse(f"{name} must be float32 [{size}], got {list(t.shape)} {t.dtype}")
+    if t.get_device() != device:
+        _elsewhere(name, t, device)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _epilogue(epi, resid, m: int, n: int, dtype, device: int):
+    """(code, resid that the kernels can read in place, its row stride)."""
+    code = _EPI.get(epi)
+    if code is None or (code == 3) != (resid is not None):
+        _refuse(f"epi must be 'bias', 'gelu' or 'resid', the last with a resid tensor, got {epi!r}")
+    if resid is None:
+        return code, None, n
+    if resid.shape != (m, n) or resid.dtype != dtype:
+        _refuse(f"resid must be [{m}, {n}] {dtype}, got {list(resid.shape)} {resid.dtype}")
+    if resid.get_device() != device:
+        _elsewhere("resid", resid, device)
+    if (n > 1 and resid.stride()[1] != 1) or (m > 1 and resid.stride()[0] < n):
+        resid = resid.contiguous()
+    return code, resid, resid.stride()[0] if m > 1 else n
 
 
 def gemm_i8(a, a_scale, w, w_scale, bias=None, *, epi="bias", resid=None, dtype=torch.float32) -> torch.Tensor:
@@ -236,59 +278,64 @@ def gemm_i8(a, a_scale, w, w_scale, bias=None, *, epi="bias", resid=None, dtype=
     quantize_rows pads it), the sum exact in 32-bit integers.  epi 'bias', 'gelu' or 'resid' (+ resid [M, N] of `dtype`); C of
     `dtype`."""
     device = _on_device(a, "a")
-    _same_device(device, a_scale=a_scale, w=w, w_scale=w_scale, bias=bias, resid=resid)
-    if epi not in _EPI or (epi == "resid") != (resid is not None):
-        _refuse(f"epi must be 'bias', 'gelu' or 'resid', the last with a resid tensor, got {epi!r}")
-    if dtype not in N.CMDI_DT:
+    out = N.CMDI_DT.get(dtype)
+    if out is None:
         _refuse(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-    a, w = _bytes_rows(a, "a"), _bytes_rows(w, "w")
+    a, w = _bytes_rows(a, "a", device), _bytes_rows(w, "w", device)
     (m, k), n = a.shape, w.shape[0]
     if w.shape[1] != k:
         _refuse(f"a has {k} columns, w {w.shape[1]}")
-    for name, t, size in (("a_scale", a_scale, m), ("w_scale", w_scale, n), ("bias", bias, n)):
-        if t is not None and (t.shape != (size,) or t.dtype != torch.float32):
-            _refuse(f"{name} must be float32 [{size}], got {tuple(t.shape)} {t.dtype}")
-    a_scale, w_scale = a_scale.contiguous(), w_scale.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if resid is not None:
-        if resid.shape != (m, n) or resid.dtype != dtype:
-            _refuse(f"resid must be [{m}, {n}] {dtype}, got {tuple(resid.shape)} {resid.dtype}")
-        if (n > 1 and resid.stride(1) != 1) or (m > 1 and resid.stride(0) < n):
-            resid = resid.contiguous()
-    c = torch.empty((m, n), dtype=dtype, device=device)
-    with _On(device) as stream:
-        N.check(N.load().cmdi_gemm_i8(N.ptr(a), N.ptr(a_scale), N.ptr(w), N.ptr(w_scale), N.ptr(bias), N.ptr(resid), N.ptr(c), m, n, k,
-                                      max(a.stride(0), k) if m > 1 else k, max(w.stride(0), k) if n > 1 else k, n,
-                                      n if resid is None or m <= 1 else resid.stride(0), N.CMDI_DT[dtype], _EPI[epi], stream))
+    a_scale, w_scale = _scales(a_scale, "a_scale", m, device), _scales(w_scale, "w_scale", n, device)
+    if bias is not None:
+        bias = _scales(bias, "bias", n, device)
+    code, resid, ldr = _epilogue(epi, resid, m, n, dtype, device)
+    c = torch.empty((m, n), dtype=dtype, device=a.device)
+    _launch(device, N.load().cmdi_gemm_i8, a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), N.ptr(bias), N.ptr(resid), c.data_ptr(),
+            m, n, k, a.stride()[0] if m > 1 else k, w.stride()[0] if n > 1 else k, n, ldr, out, code)
     return c
 
 
 def linear_i8(x, w, w_scale, bias=None, *, epi="bias", resid=None) -> torch.Tensor:
     """A linear layer in 8-bit integers: rows of x [M, in] are quantised in the call, (w, w_scale) = quantize_rows(weight [out, in])
-    once -> [M, out] of x's type.  epi 'bias', 'gelu' or 'resid' (+ resid [M, out])."""
-    _on_device(x, "x")
-    if x.dim() != 2 or x.dtype not in N.CMDI_DT:
-        _refuse(f"x must be [rows, cols] float32, bfloat16 or float16, got {tuple(x.shape)} {x.dtype}")
-    if w.dim() != 2 or w.shape[1] != (x.shape[1] + 127) // 128 * 128:
-        _refuse(f"w must be quantize_rows of a weight [out, {x.shape[1]}], got {tuple(w.shape)}")
-    q, scale = quantize_rows(x)
-    return gemm_i8(q, scale, w, w_scale, bias, epi=epi, resid=resid, dtype=x.dtype)
+    once -> [M, out] of x's type.  epi 'bias', 'gelu' or 'resid' (+ resid [M, out]); the same bits as gemm_i8 behind
+    quantize_rows."""
+    x, dt, device = _float_rows(x)
+    w = _bytes_rows(w, "w", device)
+    (m, cols), (n, kp) = x.shape, w.shape
+    if kp != (cols + 127) // 128 * 128:
+        _refuse(f"w must be quantize_rows of a weight [out, {cols}], got {list(w.shape)}")
+    w_scale = _scales(w_scale, "w_scale", n, device)
+    if bias is not None:
+        bias = _scales(bias, "bias", n, device)
+    code, resid, ldr = _epilogue(epi, resid, m, n, x.dtype, device)
+    where = x.device
+    c = torch.empty((m, n), dtype=x.dtype, device=where)
+    need = m * (kp + 4)                       # cmdi_linear_i8's scratch: the rows in 8 bits, then their scales
+    work = torch.empty(need, dtype=torch.uint8, device=where)
+    _launch(device, N.load().cmdi_linear_i8, x.data_ptr(), dt, m, cols, x.stride()[0], w.data_ptr(), w_scale.data_ptr(), N.ptr(bias), N.ptr(resid),
+            c.data_ptr(), n, kp, w.stride()[0] if n > 1 else kp, n, ldr, code, work.data_ptr(), need)
+    return c
 
 
 # ---- shared-prefix attention ----------------------------------------------------------------------------------------------------
 
-def _heads(t: torch.Tensor, name: str, shape, dtype) -> torch.Tensor:
-    """t of `shape` with rows of contiguous, 16-byte aligned dims that the kernels can read in place, or a contiguous copy."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+def _heads(t: torch.Tensor, name: str, shape, dtype, device: int, limit=1 << 62):
+    """(t of `shape` with rows of contiguous, 16-byte aligned dims that the kernels can read in place, or a contiguous copy; its
+    address; its strides without the last).  A dimension of one element may carry any stride: 0 stands for it."""
+    if t.shape != shape or t.dtype != dtype:
         _refuse(f"{name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]) or t.stride(-3) > 1 << 23):
+    if t.get_device() != device:
+        _elsewhere(name, t, device)
+    for again in (False, True):
+        st, at = t.stride(), t.data_ptr()
+        fine = st[-1] == 1 and at % 16 == 0
+        if 1 in shape:
+            st = [0 if n == 1 else s for n, s in zip(shape, st)]
+        for s in st[:-1]:
+            fine = fine and s % 8 == 0
+        if again or (fine and st[-3] <= limit) or not t.numel():
+            return t, at, st[:-1]
         t = t.contiguous()
-    return t
-
-
-def _strides(t: Optional[torch.Tensor], n: int):
-    # a dimension of one element may carry any stride: its own does not matter
-    return (C.c_int64 * n)(*([0] * n if t is None else [0 if t.shape[i] <= 1 else t.stride(i) for i in range(n)]))
 
 
 def shared_prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None, *, causal=True, scale=None, return_lse=False):
@@ -301,41 +348,52 @@ def shared_prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_l
     kv_heads.  scale None: 1 / sqrt(dim).  -> out [batch, queries, heads, dim], with return_lse also the log-sums float32 [batch,
     heads, queries].  A query that sees no key gives 0 and -inf."""
     device = _on_device(q, "q")
-    if q.dim() != 4 or q.dtype not in (torch.bfloat16, torch.float16):
-        _refuse(f"q must be [batch, queries, heads, dim] bfloat16 or float16, got {tuple(q.shape)} {q.dtype}")
+    dtype, shape = q.dtype, q.shape
+    if len(shape) != 4 or dtype not in (torch.bfloat16, torch.float16):
+        _refuse(f"q must be [batch, queries, heads, dim] bfloat16 or float16, got {list(shape)} {dtype}")
     if (prefix_k is None) != (prefix_v is None) or (own_k is None) != (own_v is None):
         _refuse("keys and values come together")
-    if prefix_k is None and own_k is None:
-        _refuse("no keys: give a prefix, own keys or both")
-    _same_device(device, prefix_k=prefix_k, prefix_v=prefix_v, own_k=own_k, own_v=own_v, own_len=own_len)
-    b, n, h, d = q.shape
-    kv = prefix_k if prefix_k is not None else own_k
-    if kv.dim() != (3 if prefix_k is not None else 4):
-        _refuse("prefix keys must be [prefix, kv_heads, dim], own keys [batch, own_max, kv_heads, dim]")
-    hk = kv.shape[-2]
+    b, n, h, d = shape
+    pk = pv = ok = ov = p = o = 0
+    ps = pvs = (0, 0)
+    os_ = ovs = (0, 0, 0)
+    hk = None
     if prefix_k is not None:
-        prefix_k, prefix_v = (_heads(t, m, (prefix_k.shape[0], hk, d), q.dtype) for t, m in ((prefix_k, "prefix_k"), (prefix_v, "prefix_v")))
+        if prefix_k.dim() != 3:
+            _refuse(f"prefix_k must be [prefix, kv_heads, dim], got {list(prefix_k.shape)}")
+        p, hk = prefix_k.shape[:2]
+        prefix_k, pk, ps = _heads(prefix_k, "prefix_k", (p, hk, d), dtype, device, 1 << 23)
+        prefix_v, pv, pvs = _heads(prefix_v, "prefix_v", (p, hk, d), dtype, device, 1 << 23)
     if own_k is not None:
         if own_k.dim() != 4:
-            _refuse(f"own_k must be [batch, own_max, kv_heads, dim], got {tuple(own_k.shape)}")
-        own_k, own_v = (_heads(t, m, (b, own_k.shape[1], hk, d), q.dtype) for t, m in ((own_k, "own_k"), (own_v, "own_v")))
+            _refuse(f"own_k must be [batch, own_max, kv_heads, dim], got {list(own_k.shape)}")
+        o = own_k.shape[1]
+        hk = own_k.shape[2] if hk is None else hk
+        own_k, ok, os_ = _heads(own_k, "own_k", (b, o, hk, d), dtype, device, 1 << 23)
+        own_v, ov, ovs = _heads(own_v, "own_v", (b, o, hk, d), dtype, device, 1 << 23)
+    if hk is None:
+        _refuse("no keys: give a prefix, own keys or both")
+    lens = 0
     if own_len is not None:
         if own_k is None or own_len.shape != (b,) or own_len.dtype != torch.int32:
-            _refuse(f"own_len must be int32 [{b}] beside own keys, got {tuple(own_len.shape)} {own_len.dtype}")
-        own_len = own_len.contiguous()
-    if q.numel() and (q.stride(-1) != 1 or q.data_ptr() % 16 or any(s % 8 for s in q.stride()[:-1])):
-        q = q.contiguous()
-    desc = N.PrefixAttentionDesc(b, n, h, hk, d, 0 if prefix_k is None else prefix_k.shape[0], 0 if own_k is None else own_k.shape[1], int(bool(causal)),
-                                 N.CMDI_DT[q.dtype], 1.0 / math.sqrt(d) if scale is None else float(scale), N.ptr(q), N.ptr(prefix_k), N.ptr(prefix_v),
-                                 N.ptr(own_k), N.ptr(own_v), _strides(q, 3), _strides(prefix_k, 2), _strides(prefix_v, 2), _strides(own_k, 3),
-                                 _strides(own_v, 3), N.ptr(own_len))
-    out = torch.empty((b, n, h, d), dtype=q.dtype, device=device)
-    lse = torch.empty((b, h, n), dtype=torch.float32, device=device) if return_lse else None
+            _refuse(f"own_len must be int32 [{b}] beside own keys, got {list(own_len.shape)} {own_len.dtype}")
+        if own_len.get_device() != device:
+            _elsewhere("own_len", own_len, device)
+        own_len = own_len if own_len.is_contiguous() else own_len.contiguous()
+        lens = own_len.data_ptr()
+    q, qp, qs = _heads(q, "q", shape, dtype, device)
+    desc = _PREFIX_DESC.pack(b, n, h, hk, d, p, o, 1 if causal else 0, N.CMDI_DT[dtype], 1.0 / math.sqrt(d) if scale is None else scale, qp, pk, pv, ok, ov,
+                             *qs, *ps, *pvs, *os_, *ovs, lens)
+    out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device) if return_lse else None
     lib = N.load()
-    with _On(device) as stream:
-        need = lib.cmdi_prefix_attention_workspace(C.byref(desc))
-        if need < 0:
-            N.check(int(need))
-        work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        N.check(lib.cmdi_prefix_attention(C.byref(desc), N.ptr(out), N.ptr(lse), N.ptr(work), need, stream))
+    if torch._C._cuda_getDevice() == device:
+        need = lib.cmdi_prefix_attention_workspace(desc)
+    else:
+        with torch.cuda.device(device):
+            need = lib.cmdi_prefix_attention_workspace(desc)
+    if need < 0:
+        N.check(int(need))
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _launch(device, lib.cmdi_prefix_attention, desc, out.data_ptr(), N.ptr(lse), N.ptr(work), need)
     return (out, lse) if return_lse else out

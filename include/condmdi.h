@@ -303,6 +303,12 @@ int cmdi_gemm_i8(const void* d_a, const float* d_a_scale, const void* d_w, const
                  const void* d_resid, void* d_c, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldw, int64_t ldc,
                  int64_t ldr, int32_t dtype, int32_t epi, cmdi_stream stream);
 
+/* The whole layer, the same bits as the two calls above: quantises x [m, cols] (ldx elements between rows) into d_work, then the
+ * product with w [n, kp], kp = cols rounded up to 128, into c of x's `dtype`.  d_work: m * (kp + 4) bytes, 16-byte aligned. */
+int cmdi_linear_i8(const void* d_x, int32_t dtype, int32_t m, int32_t cols, int64_t ldx, const void* d_w, const float* d_w_scale,
+                   const float* d_bias, const void* d_resid, void* d_c, int32_t n, int32_t kp, int64_t ldw, int64_t ldc,
+                   int64_t ldr, int32_t epi, void* d_work, int64_t work_bytes, cmdi_stream stream);
+
 /* out[b, i, h] = softmax_j(scale q[b, i, h] . k_j) v_j over the prefix's keys [prefix] and sample b's own keys
  * j < visible(b, i): own_len[b], or with `causal` own_len[b] - queries + i + 1 (the queries are the newest of the own tokens).
  * A row that sees no key is 0 with lse -inf; keys behind a length are never read.  bf16 or f16, dim 64 or 128, heads a multiple

@@ -386,6 +386,8 @@ def test_linear_i8(m, n, k, dtype):
     (qa, sa), (qn, sn) = quant_np(x.float().numpy()), quant_np(w.numpy())
     want, tol = gemm64(qa, sa, qn, sn, bias.numpy(), "bias", None, DTYPES[dtype])
     within(got, want, tol, "linear")
+    q, scale = ops().quantize_rows(x.cuda())
+    assert torch.equal(got, ops().gemm_i8(q, scale, qw, sw, bias.cuda(), dtype=got.dtype))
 
 
 # ---- shared-prefix attention ----------------------------------------------------------------------------------------------------
@@ -665,6 +667,21 @@ def test_block_operators_refuse_wrong_shapes_and_types():
             pytest.fail(f"call {i} was accepted")
 
 
+def test_packed_descriptors_have_the_structures_layout():
+    n, o = native(), ops()
+    assert o._NORM_DESC.size == C.sizeof(n.GatedNormDesc) and o._NORM_GRADS.size == C.sizeof(n.GatedNormGrads)
+    assert o._PREFIX_DESC.size == C.sizeof(n.PrefixAttentionDesc)
+    for packer, kind in ((o._NORM_DESC, n.GatedNormDesc), (o._NORM_GRADS, n.GatedNormGrads), (o._PREFIX_DESC, n.PrefixAttentionDesc)):
+        flat = []
+        d = kind()
+        for i, (name, t) in enumerate(kind._fields_):
+            many = getattr(t, "_length_", 0)
+            values = [float(100 * i + j) if t is C.c_float else 100 * i + j + 1 for j in range(max(1, many))]
+            setattr(d, name, t(*values) if many else values[0])
+            flat += values
+        assert packer.pack(*flat) == bytes(d), kind
+
+
 def test_c_entries_refuse_before_any_launch():
     """Bad descriptors come back as CMDI_E_INVALID with a text (pointers that are never followed; no device here)."""
     n = native()
@@ -707,6 +724,12 @@ def test_c_entries_refuse_before_any_launch():
                  dict(c=P + 1), dict(bias=P + 2), dict(epi=3, resid=P, ldr=0), dict(m=1 << 30, n=1 << 20, ldc=1 << 20)):
         assert lib.cmdi_gemm_i8(*{**ok, **over}.values(), 0) == E_INVALID, over
     assert lib.cmdi_gemm_i8(*{**ok, "m": 0, "a": 0}.values(), 0) == 0
+
+    ok = dict(x=P, dtype=0, m=1, cols=100, ldx=100, w=P, sw=P, bias=0, resid=0, c=P, n=1, kp=128, ldw=128, ldc=1, ldr=1, epi=0, work=P, work_bytes=132)
+    for over in (dict(dtype=4), dict(m=-1), dict(cols=0), dict(cols=129), dict(kp=256), dict(ldx=-1), dict(w=0), dict(sw=0), dict(c=0), dict(n=0), dict(ldw=64),
+                 dict(ldc=0), dict(epi=3), dict(epi=2), dict(work=0), dict(work=P + 8), dict(work_bytes=131), dict(x=0), dict(x=P + 1)):
+        assert lib.cmdi_linear_i8(*{**ok, **over}.values(), 0) == E_INVALID, over
+    assert lib.cmdi_linear_i8(*{**ok, "m": 0, "x": 0, "work": 0, "c": 0}.values(), 0) == 0
 
     def attn(**over):
         d = n.PrefixAttentionDesc(batch=1, queries=1, heads=2, kv_heads=1, dim=64, prefix=4, own_max=4, dtype=1, scale=1.0, d_q=P, d_prefix_k=P,
