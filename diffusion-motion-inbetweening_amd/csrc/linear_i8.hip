@@ -90,20 +90,27 @@ __global__ __launch_bounds__(256) void quant_rows_i8_kernel(const QuantRowsArgs 
 }
 
 // ---- product -------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float finish(int acc, float sa, float sw, float bias) { return (float)acc * sa * sw + bias; }
+
 template <class T>
-__device__ __forceinline__ void finish(const GemmI8Args& p, int row, int col, int acc, float sa, float sw, float bias) {
-    float v = (float)acc * sa * sw + bias;
+__device__ __forceinline__ void finish_at(const GemmI8Args& p, int row, int col, int acc, float sa, float sw, float bias) {
+    float v = finish(acc, sa, sw, bias);
     if (p.epi == 1) v = gelu_erf(v);
     if (p.epi == 3) v += Elem<T>::up(static_cast<const T*>(p.resid)[(int64_t)row * p.ldr + col]);
     static_cast<T*>(p.c)[(int64_t)row * p.ldc + col] = Elem<T>::down(v);
 }
 
 // Tiles: WM x WN waves, a wave owns TM x TN fragments of 32 x 32 (v_mfma_i32_32x32x32_i8).  K runs in steps of 128 columns
-// through two LDS stages filled by LDS-DMA: the next step's requests are out while this one is multiplied, one barrier a step.
-// A row of a stage is 128 bytes = eight 16-byte slots; slot t of row r holds columns 16 (t ^ (r & 7)): the 8 rows of a wave's
-// read phase hit 8 different slots.  Rows behind the matrix repeat its last one and are not stored.
+// through two LDS stages filled by LDS-DMA.  A row of a stage is 128 bytes = eight 16-byte slots; slot t of row r holds columns
+// 16 (t ^ (r >> 1 & 7)), which spreads the rows of a read's lane group over all banks.  Rows behind the matrix repeat its last
+// one and are not stored.
+//
+// A step is four substeps of 32 columns; the fragments of the next substep are read while this one multiplies.  The step's one
+// barrier sits before its LAST substep: by then every wave has that substep's fragments in registers, so stage s may be
+// overwritten (requests of step s + 2 go out) and, with the wait in front of it, step s + 1 has landed and its first fragments are
+// read under the last products: the matrix pipe waits for other waves once a step, never for LDS.
 template <class T, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmI8Args p, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_tile_kernel(const GemmI8Args p, int tiles_m, int tiles_n, int vec) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
     constexpr int PIECES = (BM + BN) / 8 / NW;       // 1-KiB pieces (8 rows) a wave brings per step
     static_assert((BM / 8) % NW == 0 && (BN / 8) % NW == 0, "a piece lies in one operand for every wave");
@@ -124,15 +131,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmI8
         const int r = (is_a ? pc : pc - BM / 8) * 8 + (lane >> 3);
         const int last = (is_a ? p.m - m0 : p.n - n0) - 1;
         const int rr = r < last ? r : last;
-        off[i] = (unsigned)(rr * (is_a ? p.lda : p.ldw)) + (((lane & 7) ^ (r & 7)) << 4);
+        off[i] = (unsigned)(rr * (is_a ? p.lda : p.ldw)) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
     }
     const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.a + (int64_t)m0 * p.lda), 0, 0x7fffffff, 0x00020000);
     const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.w + (int64_t)n0 * p.ldw), 0, 0x7fffffff, 0x00020000);
     auto bring = [&](int step, int stage) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int pc = i * NW + wave;
-            char* dst = lds + stage * STAGE + pc * 1024;
+            char* dst = lds + stage * STAGE + (i * NW + wave) * 1024;
             if (i * NW < BM / 8)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)dst, 16, (int)off[i], step * 128, 0, 0);
             else
@@ -148,46 +154,101 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_i8_tile_kernel(const GemmI8
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
 
-    const int steps = p.k / 128;
-    bring(0, 0);
-    const int arow = (wm * TM * 32 + l31) * 128, brow = (BM + wn * TN * 32 + l31) * 128, sw = l31 & 7;
-    for (int s = 0; s < steps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                             // step s is in LDS, and every wave has left step s - 1
-        if (s + 1 < steps) bring(s + 1, (s + 1) & 1);
-        const char* st = lds + (s & 1) * STAGE;
+    const int arow = (wm * TM * 32 + l31) * 128, brow = (BM + wn * TN * 32 + l31) * 128, sw = (l31 >> 1) & 7;
+    i32x4 fa[2][TM], fb[2][TN];
+    auto read = [&](const char* st, int ks, int buf) {
+        const int slot = ((ks * 2 + hi) ^ sw) << 4;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            const int slot = ((ks * 2 + hi) ^ sw) << 4;
-            i32x4 fa[TM], fb[TN];
+        for (int i = 0; i < TM; ++i) fa[buf][i] = *reinterpret_cast<const i32x4*>(st + arow + i * 32 * 128 + slot);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const i32x4*>(st + arow + i * 32 * 128 + slot);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const i32x4*>(st + brow + j * 32 * 128 + slot);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int col = n0 + (wn * TN + j) * 32 + l31;
-        if (col >= p.n) continue;
-        const float ws = p.w_scale[col], bias = p.bias ? p.bias[col] : 0.f;
+        for (int j = 0; j < TN; ++j) fb[buf][j] = *reinterpret_cast<const i32x4*>(st + brow + j * 32 * 128 + slot);
+    };
+    auto multiply = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = m0 + (wm * TM + i) * 32 + mfma32_row(r, lane);
-                if (row < p.m) finish<T>(p, row, col, acc[i][j][r], p.a_scale[row], ws, bias);
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[buf][i], fb[buf][j], acc[i][j], 0, 0, 0);
+    };
+
+    const int steps = p.k / 128;
+    bring(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (steps > 1) bring(1, 1);
+    read(lds, 0, 0);
+    for (int s = 0; s < steps; ++s) {
+        const char* st = lds + (s & 1) * STAGE;
+        read(st, 1, 1);
+        multiply(0);
+        read(st, 2, 0);
+        multiply(1);
+        read(st, 3, 1);
+        multiply(0);
+        if (s + 1 < steps) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (s + 2 < steps) bring(s + 2, s & 1);
+            read(lds + ((s + 1) & 1) * STAGE, 0, 0);
+        }
+        multiply(1);
+    }
+
+    // ---- epilogue: 32 rows of the wave's columns at a time through its own slice of LDS, so that a lane stores 16 consecutive
+    // bytes of a row; its columns, their scales and their bias stay the same for all rows ----
+    constexpr int W = Elem<T>::W, COLS = 32 * TN, PITCH = COLS + 4, LPR = COLS / W, RPI = 64 / LPR;
+    static_assert(NW * 32 * PITCH * 4 <= 2 * STAGE, "the strips fit the stages");
+    __syncthreads();
+    int* strip = reinterpret_cast<int*>(lds) + wave * 32 * PITCH;
+    const int col = n0 + wn * COLS + (lane % LPR) * W;
+    float ws[W], bias[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const int c = col + i < p.n ? col + i : p.n - 1;
+        ws[i] = p.w_scale[c];
+        bias[i] = p.bias ? p.bias[c] : 0.f;
+    }
+    const bool whole = vec && col + W <= p.n;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) strip[mfma32_row(r, lane) * PITCH + j * 32 + l31] = acc[i][j][r];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // one wave writes and reads: no barrier
+#pragma unroll 4
+        for (int it = 0; it < 32 / RPI; ++it) {
+            const int lr = it * RPI + lane / LPR, row = m0 + (wm * TM + i) * 32 + lr;
+            if (row >= p.m) continue;
+            const float sa = p.a_scale[row];
+            const int* at = strip + lr * PITCH + (lane % LPR) * W;
+            if (whole) {
+                float v[W];
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[e] = finish(at[e], sa, ws[e], bias[e]);
+                if (p.epi == 1) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) v[e] = gelu_erf(v[e]);
+                }
+                if (p.epi == 3) {
+                    float r[W];
+                    load_vec<T, W>(static_cast<const T*>(p.resid) + (int64_t)row * p.ldr + col, r);
+#pragma unroll
+                    for (int e = 0; e < W; ++e) v[e] += r[e];
+                }
+                store_vec<T, W>(static_cast<T*>(p.c) + (int64_t)row * p.ldc + col, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    if (col + e < p.n) finish_at<T>(p, row, col + e, at[e], sa, ws[e], bias[e]);
             }
+        }
+        asm volatile("" ::: "memory");
     }
 }
 
 // Few rows (M <= 16 MT): the weights' bytes are the time.  A block takes 16 weight rows, its 4 waves split K and read their
-// weights straight into the registers of v_mfma_i32_16x16x64_i8 (weights as its rows, activations as its columns), 8 steps of 64
-// columns in flight; the waves' sums join through LDS.
+// weights straight into the registers of v_mfma_i32_16x16x64_i8 (weights as its rows, activations as its columns), 8 or 16 steps of
+// 64 columns in flight; the waves' sums join through LDS.
 template <class T, int MT>
 __global__ __launch_bounds__(256) void gemm_i8_rows_kernel(const GemmI8Args p) {
     __shared__ i32x4 part[4][MT][64];
@@ -206,7 +267,7 @@ __global__ __launch_bounds__(256) void gemm_i8_rows_kernel(const GemmI8Args p) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
     const int steps = p.k / 64;
-    constexpr int U = 8;
+    constexpr int U = MT == 1 ? 16 : 8;
     for (int s0 = wave * U; s0 < steps; s0 += 4 * U) {
         i32x4 fw[U];
         const int n = steps - s0 < U ? steps - s0 : U;
@@ -243,7 +304,7 @@ __global__ __launch_bounds__(256) void gemm_i8_rows_kernel(const GemmI8Args p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int col = n0 + 4 * kg + r;
-            if (col < p.n) finish<T>(p, row, col, s[r], sa, p.w_scale[col], p.bias ? p.bias[col] : 0.f);
+            if (col < p.n) finish_at<T>(p, row, col, s[r], sa, p.w_scale[col], p.bias ? p.bias[col] : 0.f);
         }
     }
 }
@@ -261,8 +322,11 @@ hipError_t launch_tile(const GemmI8Args& p, hipStream_t stream) {
             done = 1;
         }
     }
+    constexpr int W = Elem<T>::W;
+    const auto wide = [&](const void* t, int64_t ld) { return (reinterpret_cast<uintptr_t>(t) & 15) == 0 && ld % W == 0; };
+    const int vec = wide(p.c, p.ldc) && (p.epi != 3 || wide(p.resid, p.ldr));
     const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-    kernel<<<dim3((unsigned)tm * tn), dim3(64 * WM * WN), LDS, stream>>>(p, tm, tn);
+    kernel<<<dim3((unsigned)tm * tn), dim3(64 * WM * WN), LDS, stream>>>(p, tm, tn, vec);
     return hipGetLastError();
 }
 
@@ -274,7 +338,7 @@ hipError_t launch_typed(const GemmI8Args& p, hipStream_t stream) {
     if (p.m <= 64) { gemm_i8_rows_kernel<T, 4><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
     const int cus = device_cu_count();
     auto tiles = [&](int bm, int bn) { return (int64_t)((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn); };
-    if (tiles(256, 256) >= cus) return launch_tile<T, 4, 2, 2, 4>(p, stream);
+    if (tiles(256, 256) >= cus && p.k >= 1024) return launch_tile<T, 4, 4, 2, 2>(p, stream);
     if (tiles(128, 128) >= cus) return launch_tile<T, 2, 2, 2, 2>(p, stream);
     return launch_tile<T, 1, 1, 2, 2>(p, stream);
 }

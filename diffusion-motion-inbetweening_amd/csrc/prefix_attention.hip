@@ -49,11 +49,13 @@ template <> struct Mma<_Float16> {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
-// A key row of a stage is DIM elements in 16-byte slots; slot t of key k is stored at t ^ swz(k).  K's reads (16 keys, one slot)
-// and V's transposed reads (8 keys, two neighbouring slots) both spread over all 64 banks.
+// A key row of a stage is DIM elements in 16-byte slots; slot t of key k is stored at t ^ swz(k).  A ds_read_b128 serves lanes
+// {0-3, 12-15, 20-27} and so on together: keys {0-3, 12-15} at one slot and {4-11} at its neighbour, so the swizzles of the first
+// eight have to be four whole pairs; a transposed read takes 8 keys at two neighbouring slots, whose pairs have to differ.
 template <int DIM>
 __device__ __forceinline__ int swz(int k) {
-    return DIM == 128 ? ((k & 7) << 1) | ((k >> 3) & 1) : (((k >> 1) & 3) << 1) | ((k >> 3) & 1);
+    const int high = (k >> 3) & 1;
+    return DIM == 128 ? (((k & 7) ^ (high << 2)) << 1) | high : ((((k >> 1) & 3) ^ (high << 1)) << 1) | high;
 }
 
 // One item: a tile of rows over a chunk of keys.  BYWAVE: at most 16 rows, every wave takes every fourth 32-key tile through its
