@@ -135,15 +135,16 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
     }
     const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.a + (int64_t)m0 * p.lda), 0, 0x7fffffff, 0x00020000);
     const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.w + (int64_t)n0 * p.ldw), 0, 0x7fffffff, 0x00020000);
+    auto bring_one = [&](int i, int step, int stage) {
+        char* dst = lds + stage * STAGE + (i * NW + wave) * 1024;
+        if (i * NW < BM / 8)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)dst, 16, (int)off[i], step * 128, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)dst, 16, (int)off[i], step * 128, 0, 0);
+    };
     auto bring = [&](int step, int stage) {
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            char* dst = lds + stage * STAGE + (i * NW + wave) * 1024;
-            if (i * NW < BM / 8)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)dst, 16, (int)off[i], step * 128, 0, 0);
-            else
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)dst, 16, (int)off[i], step * 128, 0, 0);
-        }
+        for (int i = 0; i < PIECES; ++i) bring_one(i, step, stage);
     };
 
     i32x16 acc[TM][TN];
@@ -163,35 +164,62 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
 #pragma unroll
         for (int j = 0; j < TN; ++j) fb[buf][j] = *reinterpret_cast<const i32x4*>(st + brow + j * 32 * 128 + slot);
     };
-    auto multiply = [&](int buf) {
+    // the products of one substep; FROM < TO: pieces [FROM, TO) of `step`'s request go out between them, evenly
+    auto multiply = [&](int buf, auto from, auto to, int step, int stage) {
+        constexpr int FROM = decltype(from)::value, TO = decltype(to)::value;
+        int piece = FROM;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[buf][i], fb[buf][j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < TN; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[buf][i], fb[buf][j], acc[i][j], 0, 0, 0);
+                if constexpr (TO > FROM) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int done = FROM + (TO - FROM) * (i * TN + j + 1) / (TM * TN);
+#pragma unroll
+                    for (; piece < done; ++piece) bring_one(piece, step, stage);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
     };
+    constexpr std::integral_constant<int, 0> N0{};
+    constexpr std::integral_constant<int, PIECES / 2> NH{};
+    constexpr std::integral_constant<int, PIECES> NP{};
 
     const int steps = p.k / 128;
+    // substeps 0 .. 2 of step s (second half of the request of s + 1 under the first), then the barrier and substep 3 with the first
+    // half of the request of s + 2
+    auto step = [&](int s, auto half1, auto more1, auto more2) {
+        const char* st = lds + (s & 1) * STAGE;
+        read(st, 1, 1);
+        if constexpr (decltype(half1)::value) multiply(0, NH, NP, s + 1, (s + 1) & 1);
+        else multiply(0, N0, N0, 0, 0);
+        read(st, 2, 0);
+        multiply(1, N0, N0, 0, 0);
+        read(st, 3, 1);
+        multiply(0, N0, N0, 0, 0);
+        if constexpr (decltype(more1)::value) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            read(lds + ((s + 1) & 1) * STAGE, 0, 0);
+        }
+        if constexpr (decltype(more2)::value) multiply(1, N0, NH, s + 2, s & 1);
+        else multiply(1, N0, N0, 0, 0);
+    };
+    constexpr std::true_type YES{};
+    constexpr std::false_type NO{};
     bring(0, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    if (steps > 1) bring(1, 1);
-    read(lds, 0, 0);
-    for (int s = 0; s < steps; ++s) {
-        const char* st = lds + (s & 1) * STAGE;
-        read(st, 1, 1);
-        multiply(0);
-        read(st, 2, 0);
-        multiply(1);
-        read(st, 3, 1);
-        multiply(0);
-        if (s + 1 < steps) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            if (s + 2 < steps) bring(s + 2, s & 1);
-            read(lds + ((s + 1) & 1) * STAGE, 0, 0);
-        }
-        multiply(1);
+    if (steps > 1) {
+#pragma unroll
+        for (int i = 0; i < PIECES / 2; ++i) bring_one(i, 1, 1);
     }
+    read(lds, 0, 0);
+    int s = 0;
+    for (; s + 2 < steps; ++s) step(s, YES, YES, YES);
+    if (s + 1 < steps) { step(s, YES, YES, NO); ++s; }
+    step(s, NO, NO, NO);
 
     // ---- epilogue: 32 rows of the wave's columns at a time through its own slice of LDS, so that a lane stores 16 consecutive
     // bytes of a row; its columns, their scales and their bias stay the same for all rows ----
@@ -338,7 +366,7 @@ hipError_t launch_typed(const GemmI8Args& p, hipStream_t stream) {
     if (p.m <= 64) { gemm_i8_rows_kernel<T, 4><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
     const int cus = device_cu_count();
     auto tiles = [&](int bm, int bn) { return (int64_t)((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn); };
-    if (tiles(256, 256) >= cus && p.k >= 1024) return launch_tile<T, 4, 4, 2, 2>(p, stream);
+    if (tiles(256, 256) >= cus && p.k >= 1024) return launch_tile<T, 4, 2, 2, 4>(p, stream);
     if (tiles(128, 128) >= cus) return launch_tile<T, 2, 2, 2, 2>(p, stream);
     return launch_tile<T, 1, 1, 2, 2>(p, stream);
 }
