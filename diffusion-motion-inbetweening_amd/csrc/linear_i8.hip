@@ -101,15 +101,15 @@ __device__ __forceinline__ void finish_at(const GemmI8Args& p, int row, int col,
 }
 
 // Tiles: WM x WN waves, a wave owns TM x TN fragments of 32 x 32 (v_mfma_i32_32x32x32_i8).  K runs in steps of 128 columns
-// through two LDS stages filled by LDS-DMA.  A row of a stage is 128 bytes = eight 16-byte slots; slot t of row r holds columns
+// through NST LDS stages filled by LDS-DMA.  A row of a stage is 128 bytes = eight 16-byte slots; slot t of row r holds columns
 // 16 (t ^ (r >> 1 & 7)), which spreads the rows of a read's lane group over all banks.  Rows behind the matrix repeat its last
-// one and are not stored.
+// one and are not stored.  NST stages: two where the products of a step cover a request's way, four where a step is short.
 //
 // A step is four substeps of 32 columns; the fragments of the next substep are read while this one multiplies.  The step's one
 // barrier sits before its LAST substep: by then every wave has that substep's fragments in registers, so stage s may be
 // overwritten (requests of step s + 2 go out) and, with the wait in front of it, step s + 1 has landed and its first fragments are
 // read under the last products: the matrix pipe waits for other waves once a step, never for LDS.
-template <class T, int TM, int TN, int WM, int WN>
+template <class T, int TM, int TN, int WM, int WN, int NST>
 __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_tile_kernel(const GemmI8Args p, int tiles_m, int tiles_n, int vec) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
     constexpr int PIECES = (BM + BN) / 8 / NW;       // 1-KiB pieces (8 rows) a wave brings per step
@@ -122,6 +122,33 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
     const int band = id / (8 * tiles_n), in = id % (8 * tiles_n);
     const int bh = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
     const int m0 = (band * 8 + in % bh) * BM, n0 = (in / bh) * BN;
+
+    // the epilogue's scales and bias, asked for first of all where the registers allow it: its lane's W columns and 32 / RPI rows of
+    // each strip
+    constexpr bool EARLY = TM * TN <= 4;
+    constexpr int W = Elem<T>::W, COLS = 32 * TN, PITCH = COLS + 4, LPR = COLS / W, RPI = 64 / LPR;
+    const int col = n0 + wn * COLS + (lane % LPR) * W;
+    float ws[W], bias[W], sa[EARLY ? TM : 1][32 / RPI];
+    auto scales = [&]() {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int c = col + i < p.n ? col + i : p.n - 1;
+            ws[i] = p.w_scale[c];
+            bias[i] = p.bias ? p.bias[c] : 0.f;
+        }
+    };
+    auto row_scales = [&](int i, float (&out)[32 / RPI]) {
+#pragma unroll
+        for (int it = 0; it < 32 / RPI; ++it) {
+            const int row = m0 + (wm * TM + i) * 32 + it * RPI + lane / LPR;
+            out[it] = p.a_scale[row < p.m ? row : p.m - 1];
+        }
+    };
+    if constexpr (EARLY) {
+        scales();
+#pragma unroll
+        for (int i = 0; i < TM; ++i) row_scales(i, sa[i]);
+    }
 
     unsigned off[PIECES];
 #pragma unroll
@@ -164,77 +191,64 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
 #pragma unroll
         for (int j = 0; j < TN; ++j) fb[buf][j] = *reinterpret_cast<const i32x4*>(st + brow + j * 32 * 128 + slot);
     };
-    // the products of one substep; FROM < TO: pieces [FROM, TO) of `step`'s request go out between them, evenly
-    auto multiply = [&](int buf, auto from, auto to, int step, int stage) {
-        constexpr int FROM = decltype(from)::value, TO = decltype(to)::value;
-        int piece = FROM;
+    // the products of one substep; where `go`, pieces [from, to) of `step`'s request go out between them, evenly
+    auto multiply = [&](int buf, int from, int to, bool go, int step, int stage) {
+        int piece = from;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[buf][i], fb[buf][j], acc[i][j], 0, 0, 0);
-                if constexpr (TO > FROM) {
+                const int done = from + (to - from) * (i * TN + j + 1) / (TM * TN);
+                if (done > piece) {
                     __builtin_amdgcn_sched_barrier(0);
-                    const int done = FROM + (TO - FROM) * (i * TN + j + 1) / (TM * TN);
+                    if (go) {
 #pragma unroll
-                    for (; piece < done; ++piece) bring_one(piece, step, stage);
+                        for (int k = piece; k < done; ++k) bring_one(k, step, stage);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
+                    piece = done;
                 }
             }
     };
-    constexpr std::integral_constant<int, 0> N0{};
-    constexpr std::integral_constant<int, PIECES / 2> NH{};
-    constexpr std::integral_constant<int, PIECES> NP{};
 
     const int steps = p.k / 128;
-    // substeps 0 .. 2 of step s (second half of the request of s + 1 under the first), then the barrier and substep 3 with the first
-    // half of the request of s + 2
-    auto step = [&](int s, auto half1, auto more1, auto more2) {
-        const char* st = lds + (s & 1) * STAGE;
-        read(st, 1, 1);
-        if constexpr (decltype(half1)::value) multiply(0, NH, NP, s + 1, (s + 1) & 1);
-        else multiply(0, N0, N0, 0, 0);
-        read(st, 2, 0);
-        multiply(1, N0, N0, 0, 0);
-        read(st, 3, 1);
-        multiply(0, N0, N0, 0, 0);
-        if constexpr (decltype(more1)::value) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            read(lds + ((s + 1) & 1) * STAGE, 0, 0);
-        }
-        if constexpr (decltype(more2)::value) multiply(1, N0, NH, s + 2, s & 1);
-        else multiply(1, N0, N0, 0, 0);
-    };
-    constexpr std::true_type YES{};
-    constexpr std::false_type NO{};
-    bring(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    if (steps > 1) {
 #pragma unroll
-        for (int i = 0; i < PIECES / 2; ++i) bring_one(i, 1, 1);
-    }
+    for (int i = 0; i < NST; ++i)
+        if (i < steps) bring(i, i);
+    if (steps >= NST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * PIECES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
     read(lds, 0, 0);
-    int s = 0;
-    for (; s + 2 < steps; ++s) step(s, YES, YES, YES);
-    if (s + 1 < steps) { step(s, YES, YES, NO); ++s; }
-    step(s, NO, NO, NO);
+    int at = 0;                                       // s % NST
+    for (int s = 0; s < steps; ++s) {
+        const char* st = lds + at * STAGE;
+        const int next = at + 1 == NST ? 0 : at + 1;
+        read(st, 1, 1);
+        // two stages: the second half of the request of s + 1 goes out here (step 1's went out whole in front of the loop)
+        if constexpr (NST == 2) multiply(0, PIECES / 2, PIECES, s > 0 && s + 1 < steps, s + 1, next);
+        else multiply(0, 0, 0, false, 0, 0);
+        read(st, 2, 0);
+        multiply(1, 0, 0, false, 0, 0);
+        read(st, 3, 1);
+        multiply(0, 0, 0, false, 0, 0);
+        if (s + 1 < steps) {
+            // step s + 1 has landed once at most the NST - 2 requests behind it are out
+            if (s + NST <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * PIECES) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            read(lds + next * STAGE, 0, 0);
+        }
+        multiply(1, 0, NST == 2 ? PIECES / 2 : PIECES, s + NST < steps, s + NST, at);      // into the stage just left
+        at = next;
+    }
 
     // ---- epilogue: 32 rows of the wave's columns at a time through its own slice of LDS, so that a lane stores 16 consecutive
     // bytes of a row; its columns, their scales and their bias stay the same for all rows ----
-    constexpr int W = Elem<T>::W, COLS = 32 * TN, PITCH = COLS + 4, LPR = COLS / W, RPI = 64 / LPR;
-    static_assert(NW * 32 * PITCH * 4 <= 2 * STAGE, "the strips fit the stages");
+    static_assert(NW * 32 * PITCH * 4 <= NST * STAGE, "the strips fit the stages");
     __syncthreads();
     int* strip = reinterpret_cast<int*>(lds) + wave * 32 * PITCH;
-    const int col = n0 + wn * COLS + (lane % LPR) * W;
-    float ws[W], bias[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-        const int c = col + i < p.n ? col + i : p.n - 1;
-        ws[i] = p.w_scale[c];
-        bias[i] = p.bias ? p.bias[c] : 0.f;
-    }
+    if constexpr (!EARLY) scales();
     const bool whole = vec && col + W <= p.n;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
@@ -242,17 +256,17 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) strip[mfma32_row(r, lane) * PITCH + j * 32 + l31] = acc[i][j][r];
+        if constexpr (!EARLY) row_scales(i, sa[0]);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // one wave writes and reads: no barrier
-#pragma unroll 4
+#pragma unroll
         for (int it = 0; it < 32 / RPI; ++it) {
             const int lr = it * RPI + lane / LPR, row = m0 + (wm * TM + i) * 32 + lr;
             if (row >= p.m) continue;
-            const float sa = p.a_scale[row];
             const int* at = strip + lr * PITCH + (lane % LPR) * W;
             if (whole) {
                 float v[W];
 #pragma unroll
-                for (int e = 0; e < W; ++e) v[e] = finish(at[e], sa, ws[e], bias[e]);
+                for (int e = 0; e < W; ++e) v[e] = finish(at[e], sa[EARLY ? i : 0][it], ws[e], bias[e]);
                 if (p.epi == 1) {
 #pragma unroll
                     for (int e = 0; e < W; ++e) v[e] = gelu_erf(v[e]);
@@ -267,80 +281,64 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
             } else {
 #pragma unroll
                 for (int e = 0; e < W; ++e)
-                    if (col + e < p.n) finish_at<T>(p, row, col + e, at[e], sa, ws[e], bias[e]);
+                    if (col + e < p.n) finish_at<T>(p, row, col + e, at[e], sa[EARLY ? i : 0][it], ws[e], bias[e]);
             }
         }
         asm volatile("" ::: "memory");
     }
 }
 
-// Few rows (M <= 16 MT): the weights' bytes are the time.  A block takes 16 weight rows, its 4 waves split K and read their
-// weights straight into the registers of v_mfma_i32_16x16x64_i8 (weights as its rows, activations as its columns), 8 or 16 steps of
+// Few rows (M <= 16): the weights' bytes are the time.  A block takes 16 weight rows, its 4 waves split K and read their
+// weights straight into the registers of v_mfma_i32_16x16x64_i8 (weights as its rows, activations as its columns), 16 steps of
 // 64 columns in flight; the waves' sums join through LDS.
-template <class T, int MT>
+template <class T>
 __global__ __launch_bounds__(256) void gemm_i8_rows_kernel(const GemmI8Args p) {
-    __shared__ i32x4 part[4][MT][64];
+    __shared__ i32x4 part[4][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l15 = lane & 15, kg = lane >> 4;
     const int n0 = blockIdx.x * 16;
-    const int wr = n0 + l15 < p.n ? n0 + l15 : p.n - 1;
+    const int wr = n0 + l15 < p.n ? n0 + l15 : p.n - 1, ar = l15 < p.m ? l15 : p.m - 1;
     const int8_t* w = p.w + (int64_t)wr * p.ldw + kg * 16;
-    const int8_t* a[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int r = t * 16 + l15 < p.m ? t * 16 + l15 : p.m - 1;
-        a[t] = p.a + (int64_t)r * p.lda + kg * 16;
-    }
-    i32x4 acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+    const int8_t* a = p.a + (int64_t)ar * p.lda + kg * 16;
+    i32x4 acc{0, 0, 0, 0};
     const int steps = p.k / 64;
-    constexpr int U = MT == 1 ? 16 : 8;
+    constexpr int U = 16;
     for (int s0 = wave * U; s0 < steps; s0 += 4 * U) {
-        i32x4 fw[U];
         const int n = steps - s0 < U ? steps - s0 : U;
         if (n == U) {
+            i32x4 fw[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) fw[u] = *reinterpret_cast<const i32x4*>(w + (int64_t)(s0 + u) * 64);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const i32x4 fa = *reinterpret_cast<const i32x4*>(a[t] + (int64_t)(s0 + u) * 64);
-                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fa, acc[t], 0, 0, 0);
-                }
+            for (int u = 0; u < U; ++u) {
+                const i32x4 fa = *reinterpret_cast<const i32x4*>(a + (int64_t)(s0 + u) * 64);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], fa, acc, 0, 0, 0);
+            }
         } else {
             for (int u = 0; u < n; ++u) {
                 const i32x4 f = *reinterpret_cast<const i32x4*>(w + (int64_t)(s0 + u) * 64);
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const i32x4 fa = *reinterpret_cast<const i32x4*>(a[t] + (int64_t)(s0 + u) * 64);
-                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, fa, acc[t], 0, 0, 0);
-                }
+                const i32x4 fa = *reinterpret_cast<const i32x4*>(a + (int64_t)(s0 + u) * 64);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, fa, acc, 0, 0, 0);
             }
         }
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    part[wave][lane] = acc;
     __syncthreads();
-    // lane of fragment t: activation row 16 t + l15, weight rows 4 kg + r
-    for (int t = wave; t < MT; t += 4) {
-        const i32x4 s = part[0][t][lane] + part[1][t][lane] + part[2][t][lane] + part[3][t][lane];
-        const int row = t * 16 + l15;
-        if (row >= p.m) continue;
-        const float sa = p.a_scale[row];
+    if (wave != 0 || l15 >= p.m) return;
+    // this lane: activation row l15, weight rows 4 kg + r
+    const i32x4 s = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    const float sa = p.a_scale[l15];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int col = n0 + 4 * kg + r;
-            if (col < p.n) finish_at<T>(p, row, col, s[r], sa, p.w_scale[col], p.bias ? p.bias[col] : 0.f);
-        }
+    for (int r = 0; r < 4; ++r) {
+        const int col = n0 + 4 * kg + r;
+        if (col < p.n) finish_at<T>(p, l15, col, s[r], sa, p.w_scale[col], p.bias ? p.bias[col] : 0.f);
     }
 }
 
-template <class T, int TM, int TN, int WM, int WN>
+template <class T, int TM, int TN, int WM, int WN, int NST>
 hipError_t launch_tile(const GemmI8Args& p, hipStream_t stream) {
-    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, LDS = 2 * (BM + BN) * 128;
-    auto* kernel = gemm_i8_tile_kernel<T, TM, TN, WM, WN>;
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, LDS = NST * (BM + BN) * 128;
+    auto* kernel = gemm_i8_tile_kernel<T, TM, TN, WM, WN, NST>;
     if (LDS > 64 * 1024) {
         static PerDevice<int> set;
         int& done = set.get();
@@ -360,15 +358,25 @@ hipError_t launch_tile(const GemmI8Args& p, hipStream_t stream) {
 
 template <class T>
 hipError_t launch_typed(const GemmI8Args& p, hipStream_t stream) {
-    const dim3 g16((unsigned)((p.n + 15) / 16));
-    if (p.m <= 16) { gemm_i8_rows_kernel<T, 1><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
-    if (p.m <= 32) { gemm_i8_rows_kernel<T, 2><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
-    if (p.m <= 64) { gemm_i8_rows_kernel<T, 4><<<g16, 256, 0, stream>>>(p); return hipGetLastError(); }
+    // Measured on an MI355X (us, 8-bit operands, bf16 out unless said):
+    //   rows kernel / 64 x 64 tile:          16 x 8192 x 4096: 9.1 / 12.7        32 x 8192 x 4096: 14.1 / 12.7
+    //   64 x 64, four stages / two stages:   65 x 8192 x 4096: 11.8 / 17.4       512 x 4096 x 4096: 15.5 / 17.8
+    //   128 x 128, three stages / 64 x 64:   1024 x 4096 x 4096: 23.6 / 30.1     512 x 4096 x 4096 (half a chip of tiles): 20.6 / 15.5
+    //   128 x 128, two stages / three:       2048 x 4096 x 4096: 39.7 / 44.8     12608 x 1536 x 512 fp32 out: 29.2 / 36.8
+    //   256 x 256 / 128 x 128, two stages:   4096^3: 64 / 75    8192 x 8192 x 512: 62 / 81    2048 x 4096 x 4096 (half a chip): 50 / 40
+    //                                        12608 x 1536 x 512 fp32 out (300 tiles, a round and a sixth): 33.9 / 29.2
     const int cus = device_cu_count();
-    auto tiles = [&](int bm, int bn) { return (int64_t)((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn); };
-    if (tiles(256, 256) >= cus && p.k >= 1024) return launch_tile<T, 4, 2, 2, 4>(p, stream);
-    if (tiles(128, 128) >= cus) return launch_tile<T, 2, 2, 2, 2>(p, stream);
-    return launch_tile<T, 1, 1, 2, 2>(p, stream);
+    auto tiles = [&](int side) { return (int64_t)((p.m + side - 1) / side) * ((p.n + side - 1) / side); };
+    const int64_t t256 = tiles(256), t128 = tiles(128);
+    if (p.m <= 16) {
+        gemm_i8_rows_kernel<T><<<dim3((unsigned)((p.n + 15) / 16)), 256, 0, stream>>>(p);
+        return hipGetLastError();
+    }
+    // one block a CU: worth it where its rounds are at least three quarters full
+    if (t256 >= cus && 4 * t256 >= 3 * ((t256 + cus - 1) / cus) * cus) return launch_tile<T, 4, 2, 2, 4, 2>(p, stream);
+    if (t128 >= 2 * cus) return launch_tile<T, 2, 2, 2, 2, 2>(p, stream);
+    if (t128 >= cus) return launch_tile<T, 2, 2, 2, 2, 3>(p, stream);
+    return launch_tile<T, 1, 1, 2, 2, 4>(p, stream);
 }
 
 }  // namespace
