@@ -58,22 +58,51 @@ __device__ __forceinline__ int swz(int k) {
     return DIM == 128 ? (((k & 7) ^ (high << 2)) << 1) | high : ((((k >> 1) & 3) ^ (high << 1)) << 1) | high;
 }
 
-// One item: a tile of rows over a chunk of keys.  BYWAVE: at most 16 rows, every wave takes every fourth 32-key tile through its
-// own LDS ring, and the waves join at the end; otherwise wave w owns rows [16 RT w, +16 RT) and all share 64-key stages.
+// 16 bytes a lane from `offset` behind the descriptor's base to LDS, lane after lane.  (The host's pass over this file knows no
+// 16-byte form of the builtin.)
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, char* to, int offset) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
+#endif
+}
+
+// Maximum / sum over the four lane groups that share a row (lanes 16 apart).
+__device__ __forceinline__ float over_groups_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float over_groups_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+template <int DIM, bool BYWAVE>
+constexpr int lds_bytes() {
+    // by rows: two stages of 64 keys and 64 values; by wave: each of the four has two stages of 32 values
+    return BYWAVE ? 4 * 2 * 32 * DIM * 2 : 2 * 2 * 64 * DIM * 2;
+}
+
+// One item: a tile of rows over a chunk of keys.
+//   By rows: wave w owns rows [16 RT w, +16 RT); K and V come in 64-key stages through LDS (LDS-DMA), two of each.  The scores of
+//   stage s + 1 are multiplied while the softmax of stage s runs, so the matrix units work under the exponentials.
+//   BYWAVE: at most 16 rows (few queries): a wave takes every fourth 32-key tile, its K straight into registers, its V through its own
+//   two LDS slots, no barrier until the four waves join at the end.
+// A row's maximum is moved only when a score passes it by 2^8: until then its p stay below 256, which changes no relative
+// rounding and saves the exchange between the lanes and the rescaling of o.
 template <class T, int DIM, int RT, bool BYWAVE>
-__global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(const PrefixAttnArgs a, const PrefixAttnLaunch L, int slots) {
-    constexpr int KT = BYWAVE ? 32 : 64, ROWB = DIM * 2, TILE = KT * ROWB, STAGE = 2 * TILE, KB = KT / 16, DB = DIM / 16, DS = DIM / 32;
+__device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int slots, int block, int blocks, char* lds_all) {
+    constexpr int KT = BYWAVE ? 32 : 64, ROWB = DIM * 2, TILE = KT * ROWB, KB = KT / 16, DB = DIM / 16, DS = DIM / 32;
     constexpr int SLOTS = DIM / 8, RPP = 64 / SLOTS;              // 16-byte slots of a key row; key rows of a 1-KiB piece
-    constexpr int PIECES = KT / RPP / (BYWAVE ? 1 : 4);           // pieces of K (and as many of V) a wave brings per stage
+    constexpr int PIECES = KT / RPP / (BYWAVE ? 1 : 4);           // pieces of a tile that a wave brings
     static_assert(!BYWAVE || RT == 1, "");
-    extern __shared__ __attribute__((aligned(16))) char lds_all[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l15 = lane & 15, g = lane >> 4;
-    char* lds = lds_all + (BYWAVE ? wave * 2 * STAGE : 0);
+    // by rows: K slots at 0, 1, V slots at 2, 3 tiles; by wave: the wave's two V slots
+    char* lds = lds_all + (BYWAVE ? wave * 2 * TILE : 0);
 
     // ---- which item ----
     const int grp = a.heads / a.kv_heads;
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int id = xcd_remap(block, blocks);
     const int tile = id % L.tiles, rest = id / L.tiles;
     const int chunk = rest % L.chunks, bh = rest / L.chunks;
     const int hk = bh % a.kv_heads, b0 = bh / a.kv_heads;         // packed: b0 = 0, the sample comes from the row
@@ -83,7 +112,6 @@ __global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(
     // ---- rows of this lane: column l15 of each of the wave's RT row tiles ----
     int row_b[RT], row_i[RT], row_h[RT], vis[RT];
     bool row_ok[RT];
-    int vis_top = 0, vis_low = 0x7fffffff;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         int r = tile * BM + (BYWAVE ? 0 : wave * RT * 16) + t * 16 + l15;
@@ -95,60 +123,74 @@ __global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(
         row_b[t] = L.packed ? q / a.queries : b0;
         vis[t] = 0;
     }
-    int own_tiles_end = 0;                                        // own keys this block has to look at
+    int vis_top = 0, vis_low = 0;                                 // own keys that the block's last and first row see
     if (L.k_end > a.prefix) {                                     // (never for packed rows)
         int len = a.own_len ? a.own_len[b0] : a.own_max;
         len = len < 0 ? 0 : len > a.own_max ? a.own_max : len;
+        auto sees = [&](int i) {
+            const int v = a.causal ? len - a.queries + i + 1 : len;
+            return v < 0 ? 0 : v > len ? len : v;
+        };
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            int v = a.causal ? len - a.queries + row_i[t] + 1 : len;
-            vis[t] = v < 0 ? 0 : v > len ? len : v;
-        }
-        const int last = (tile + 1) * BM < n_rows ? (tile + 1) * BM - 1 : n_rows - 1;
-        int v = a.causal ? len - a.queries + last / grp + 1 : len;
-        vis_top = v < 0 ? 0 : v > len ? len : v;
-        v = a.causal ? len - a.queries + (tile * BM) / grp + 1 : len;
-        vis_low = v < 0 ? 0 : v > len ? len : v;
-        own_tiles_end = vis_top;
+        for (int t = 0; t < RT; ++t) vis[t] = sees(row_i[t]);
+        vis_top = sees(((tile + 1) * BM < n_rows ? (tile + 1) * BM - 1 : n_rows - 1) / grp);
+        vis_low = sees(tile * BM / grp);
     }
     const int c0 = L.k_begin + chunk * L.chunk;
     const int c1 = c0 + L.chunk < L.k_end ? c0 + L.chunk : L.k_end;
     const int p0 = c0, p1 = c1 < a.prefix ? c1 : a.prefix;        // prefix keys [p0, p1)
     const int o0 = c0 > a.prefix ? c0 - a.prefix : 0;             // own keys [o0, o1)
-    const int o1 = c1 - a.prefix < own_tiles_end ? c1 - a.prefix : own_tiles_end;
+    const int o1 = c1 - a.prefix < vis_top ? c1 - a.prefix : vis_top;
     const int np = p1 > p0 ? (p1 - p0 + KT - 1) / KT : 0;
     const int no = o1 > o0 ? (o1 - o0 + KT - 1) / KT : 0;
     const int stages = np + no;
 
-    // ---- bringing a stage: LDS-DMA through a descriptor that ends with the stage's last valid key, so that keys behind it read
-    // as zeros whatever lies there ----
+    // ---- a stage's keys or values, through a descriptor that ends with the stage's last valid key: keys behind it read as zeros
+    // whatever lies there ----
     const char* pk = static_cast<const char*>(a.pk) + (int64_t)hk * a.pk_hs * 2;
     const char* pv = static_cast<const char*>(a.pv) + (int64_t)hk * a.pv_hs * 2;
     const char* ok = static_cast<const char*>(a.ok) + ((int64_t)b0 * a.ok_bs + (int64_t)hk * a.ok_hs) * 2;
     const char* ov = static_cast<const char*>(a.ov) + ((int64_t)b0 * a.ov_bs + (int64_t)hk * a.ov_hs) * 2;
-    const int w4 = BYWAVE ? 0 : wave;
-    auto bring = [&](int s, int slot) {
+    auto rows_of = [&](int s, bool values, int64_t& stride) {
         const bool own = s >= np;
         const int k0 = own ? o0 + (s - np) * KT : p0 + s * KT;
-        const int left = (own ? o1 : p1) - k0;
-        const int valid = left < KT ? left : KT;
-        const int64_t ks = own ? a.ok_ss : a.pk_ss, vs = own ? a.ov_ss : a.pv_ss;
-        const char* kb = (own ? ok : pk) + (int64_t)k0 * ks * 2;
-        const char* vb = (own ? ov : pv) + (int64_t)k0 * vs * 2;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kb), 0, (int)((valid - 1) * ks * 2 + ROWB), 0x00020000);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vb), 0, (int)((valid - 1) * vs * 2 + ROWB), 0x00020000);
+        const int left = (own ? o1 : p1) - k0, valid = left < KT ? left : KT;
+        stride = own ? (values ? a.ov_ss : a.ok_ss) : (values ? a.pv_ss : a.pk_ss);
+        const char* base = (own ? (values ? ov : ok) : (values ? pv : pk)) + (int64_t)k0 * stride * 2;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)((valid - 1) * stride * 2 + ROWB), 0x00020000);
+    };
+    const int w4 = BYWAVE ? 0 : wave;
+    auto bring = [&](int s, bool values, char* to) {
+        int64_t stride;
+        const auto r = rows_of(s, values, stride);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int pc = i + w4 * PIECES;
-            const int key = pc * RPP + lane / SLOTS;
-            const int t = (lane % SLOTS) ^ swz<DIM>(key);
-            char* dst = lds + slot * STAGE + pc * 1024;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)dst, 16, (int)(key * (int)ks * 2 + t * 16), 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(dst + TILE), 16, (int)(key * (int)vs * 2 + t * 16), 0, 0, 0);
+            const int pc = i + w4 * PIECES, key = pc * RPP + lane / SLOTS, t = (lane % SLOTS) ^ swz<DIM>(key);
+            dma16(r, to + pc * 1024, key * (int)stride * 2 + t * 16);
         }
     };
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    s8 kreg[2][BYWAVE ? KB : 1][DS];                              // by wave: the K operand, this tile's and the next one's
+    auto load_k = [&](int s, int buf) {
+        int64_t stride;
+        const auto r = rows_of(s, false, stride);
+#pragma unroll
+        for (int kb = 0; kb < (BYWAVE ? KB : 0); ++kb)
+#pragma unroll
+            for (int d = 0; d < DS; ++d)
+                kreg[buf][kb][d] = __builtin_bit_cast(s8, (u4)__builtin_amdgcn_raw_buffer_load_b128(r, (kb * 16 + l15) * (int)stride * 2 + (32 * d + 8 * g) * 2, 0, 0));
+    };
     const int first = BYWAVE ? wave : 0, step = BYWAVE ? 4 : 1;
-    if (first < stages) bring(first, 0);
+    if (first < stages) {
+        if constexpr (BYWAVE) {
+            load_k(first, 0);
+            bring(first, true, lds);
+        } else {
+            bring(0, false, lds);
+            bring(0, true, lds + 2 * TILE);
+            if (stages > 1) bring(1, false, lds + TILE);
+        }
+    }
 
     // ---- Q as the B operand: lane (row l15, dims 32 s + 8 g ..) ----
     s8 q[RT][DS];
@@ -171,43 +213,29 @@ __global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(
     const float scale2 = a.scale * kLog2e;
     const int kswz = swz<DIM>(l15), krow = l15 * ROWB;            // K: key l15 of a 16-key block
     const int vkey = 4 * g + (l15 >> 2);                          // V: this lane's source key of a 16-key block
-    const int vrow = TILE + vkey * ROWB + (l15 & 1) * 8, vsl = ((l15 & 3) >> 1) ^ swz<DIM>(vkey);
+    const int vrow = vkey * ROWB + (l15 & 1) * 8, vsl = ((l15 & 3) >> 1) ^ swz<DIM>(vkey);
 
-    int slot = 0;
-    for (int s = first; s < stages; s += step) {
-        if constexpr (BYWAVE) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the other slot's reads are done
-            if (s + step < stages) {
-                bring(s + step, slot ^ 1);
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PIECES) : "memory");
-            } else {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();                                      // stage s is in LDS, and every wave has left stage s - 1
-            if (s + 1 < stages) bring(s + 1, slot ^ 1);
-        }
-        const char* st = lds + slot * STAGE;
-        slot ^= 1;
-        // ---- scores ----
-        f32x4 sc[KB][RT];
+    auto scores = [&](const char* kt, int buf, f32x4 (&sc)[KB][RT]) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int t = 0; t < RT; ++t) sc[kb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int d = 0; d < DS; ++d) {
-                const s8 kf = *reinterpret_cast<const s8*>(st + kb * 16 * ROWB + krow + (((4 * d + g) ^ kswz) << 4));
+                s8 kf;
+                if constexpr (BYWAVE) kf = kreg[buf][kb][d];
+                else kf = *reinterpret_cast<const s8*>(kt + kb * 16 * ROWB + krow + (((4 * d + g) ^ kswz) << 4));
 #pragma unroll
                 for (int t = 0; t < RT; ++t) sc[kb][t] = Mma<T>::mul(kf, q[t][d], sc[kb][t]);
             }
         }
-        // ---- masks: keys behind the chunk's end, own keys a row does not see ----
+    };
+    // masks, and the running maximum brought above the scores less 2^8
+    auto settle = [&](int s, f32x4 (&sc)[KB][RT]) {
         const bool own = s >= np;
         const int k0 = own ? o0 + (s - np) * KT : p0 + s * KT;
         const int end = own ? o1 : p1;
-        if (k0 + KT > end || (own && k0 + KT > vis_low)) {
+        if (k0 + KT > end || (own && k0 + KT > vis_low)) {        // keys behind the chunk's end, own keys a row does not see
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 const int lim = own && vis[t] < end ? vis[t] : end;
@@ -218,27 +246,35 @@ __global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(
                         if (k0 + kb * 16 + 4 * g + r >= lim) sc[kb][t][r] = -INFINITY;
             }
         }
-        // ---- running maximum and sum; P^T as the B operand of each 32-key block ----
-        s8 p[KB / 2][RT];
+        float top[RT];
+        bool move = false;
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            float top = sc[0][t][0];
+            top[t] = sc[0][t][0];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[kb][t][r]);
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m[t], top * scale2);
-            const float base = mn == -INFINITY ? 0.f : mn;        // nothing seen yet: every p is 2^-inf = 0
-            if (__any(mn > m[t])) {
-                const float k = exp2f(m[t] - base);
+                for (int r = 0; r < 4; ++r) top[t] = fmaxf(top[t], sc[kb][t][r]);
+            top[t] *= scale2;
+            move |= top[t] > m[t] + 8.f;
+        }
+        if (__any(move)) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const float mn = fmaxf(m[t], over_groups_max(top[t]));
+                const float k = mn == -INFINITY ? 0.f : exp2f(m[t] - mn);
                 l[t] *= k;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) o[t][d] *= k;
+                m[t] = mn;
             }
-            m[t] = mn;
-            float sum = 0.f;
+        }
+    };
+    // P^T as the B operand of each 32-key block, its sum into l
+    auto weights = [&](const f32x4 (&sc)[KB][RT], s8 (&p)[KB / 2][RT]) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const float base = m[t] == -INFINITY ? 0.f : m[t];    // nothing seen yet: every p is 2^-inf = 0
 #pragma unroll
             for (int kb = 0; kb < KB; kb += 2) {
                 float e[8];
@@ -247,35 +283,82 @@ __global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(
                     e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][t][r], scale2, -base));
                     e[4 + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb + 1][t][r], scale2, -base));
                 }
-                sum += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                struct { unsigned u[4]; } pk4;
+                l[t] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                struct { unsigned u[4]; } w;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) pk4.u[r] = Mma<T>::pack(e[2 * r], e[2 * r + 1]);
-                p[kb / 2][t] = __builtin_bit_cast(s8, pk4);
+                for (int r = 0; r < 4; ++r) w.u[r] = Mma<T>::pack(e[2 * r], e[2 * r + 1]);
+                p[kb / 2][t] = __builtin_bit_cast(s8, w);
             }
-            l[t] += sum;
         }
-        // ---- O^T += V^T P^T ----
+    };
+    auto values = [&](const char* vt, const s8 (&p)[KB / 2][RT]) {
 #pragma unroll
         for (int kk = 0; kk < KB / 2; ++kk)
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const char* at = st + kk * 32 * ROWB + vrow + ((vsl ^ (2 * d)) << 4);
+                const char* at = vt + kk * 32 * ROWB + vrow + ((vsl ^ (2 * d)) << 4);
                 const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
                 const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + 16 * ROWB));
                 const s8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int t = 0; t < RT; ++t) o[t][d] = Mma<T>::mul(v, p[kk][t], o[t][d]);
             }
+    };
+
+    s8 p[KB / 2][RT];
+    if constexpr (BYWAVE) {
+        auto one = [&](int s, int buf) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the other slot's reads are done
+            const bool more = s + step < stages;
+            if (more) {
+                load_k(s + step, buf ^ 1);
+                bring(s + step, true, lds + (buf ^ 1) * TILE);
+            }
+            f32x4 sc[KB][RT];
+            scores(nullptr, buf, sc);
+            settle(s, sc);
+            weights(sc, p);
+            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES + KB * DS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            values(lds + buf * TILE, p);
+        };
+        for (int s = first; s < stages; s += 2 * step) {
+            one(s, 0);
+            if (s + step < stages) one(s + step, 1);
+        }
+    } else if (stages > 0) {
+        f32x4 sc[KB][RT];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        scores(lds, 0, sc);
+        for (int s = 0; s < stages; ++s) {
+            const int at = s & 1;
+            // K of s + 1 and V of s are in LDS, and every wave has left K of s and V of s - 1
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (s + 2 < stages) bring(s + 2, false, lds + at * TILE);
+            if (s + 1 < stages) bring(s + 1, true, lds + (2 + (at ^ 1)) * TILE);
+            settle(s, sc);
+            if (s + 1 < stages) {
+                f32x4 nx[KB][RT];
+                scores(lds + (at ^ 1) * TILE, 0, nx);
+                weights(sc, p);
+                values(lds + (2 + at) * TILE, p);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) sc[kb][t] = nx[kb][t];
+            } else {
+                weights(sc, p);
+                values(lds + (2 + at) * TILE, p);
+            }
+        }
     }
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        l[t] += __shfl_xor(l[t], 16, 64);
-        l[t] += __shfl_xor(l[t], 32, 64);
-    }
+    for (int t = 0; t < RT; ++t) l[t] = over_groups_sum(l[t]);
 
     if constexpr (BYWAVE) {                                       // the four waves' results join in order
-        __syncthreads();                                          // the ring is free
+        __syncthreads();                                          // the rings are free
         float* jo = reinterpret_cast<float*>(lds_all);            // [4][16 rows][DIM + 4]
         float* jm = jo + 4 * 16 * (DIM + 4);                      // [4][16], then the sums
 #pragma unroll
@@ -321,88 +404,87 @@ __global__ __launch_bounds__(256, RT == 4 ? 1 : 2) void prefix_attention_kernel(
             if (a.lse && g == 0) a.lse[((int64_t)row_b[t] * a.heads + row_h[t]) * a.queries + row_i[t]] = lse2 * kLn2;
         } else {
             const int64_t rows = (int64_t)a.batch * a.queries * a.heads, at = (int64_t)(L.slot0 + chunk) * rows + row;
-            if (some) {
-                float* out = a.work + at * DIM + 4 * g;
+            float* out = a.work + at * DIM + 4 * g;
 #pragma unroll
-                for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(out + 16 * d) = o[t][d] * inv;
-            }
+            for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4*>(out + 16 * d) = some ? o[t][d] * inv : f32x4{0.f, 0.f, 0.f, 0.f};
             if (g == 0) (a.work + (int64_t)slots * rows * DIM)[at] = lse2;
         }
     }
 }
 
-// Joins a row's partial results: out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  One wave a row; a partial result
-// without keys has no o (never written) and is passed over.
+// The first `n0` blocks work on launch A, the others on B: the packed prefix and the own keys run beside each other.  KIND 0: by
+// wave, 1, 2: by rows.
+template <class T, int DIM, int KIND_A, int KIND_B>
+__global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const PrefixAttnArgs a, const PrefixAttnLaunch A, const PrefixAttnLaunch B, int n0,
+                                                                  int slots) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int block = blockIdx.x;
+    if constexpr (KIND_A == KIND_B) {
+        const bool second = block >= n0;
+        const PrefixAttnLaunch L = second ? B : A;
+        attend<T, DIM, KIND_A == 0 ? 1 : KIND_A, KIND_A == 0>(a, L, slots, second ? block - n0 : block, second ? (int)gridDim.x - n0 : n0, lds);
+    } else if (block < n0) {
+        attend<T, DIM, KIND_A == 0 ? 1 : KIND_A, KIND_A == 0>(a, A, slots, block, n0, lds);
+    } else {
+        attend<T, DIM, KIND_B == 0 ? 1 : KIND_B, KIND_B == 0>(a, B, slots, block - n0, (int)gridDim.x - n0, lds);
+    }
+}
+
+// Joins a row's partial results: out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  One wave a row, a lane a partial
+// result's weight (at most 64), then a lane two columns or one.
 template <class T, int DIM>
 __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const PrefixAttnArgs a, int slots, int rows) {
     constexpr int W = DIM / 64;
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= rows) return;
-    const float* lse = a.work + (int64_t)slots * rows * DIM + row;
-    float top = -INFINITY;
-    bool odd = false;
-    for (int s = 0; s < slots; ++s) {
-        const float v = lse[(int64_t)s * rows];
-        top = fmaxf(top, v);
-        odd |= v != v;
-    }
-    float sum = 0.f, acc[W];
+    const float mine = lane < slots ? a.work[(int64_t)slots * rows * DIM + (int64_t)lane * rows + row] : -INFINITY;
+    const float top = wave_highest(mine), base = top == -INFINITY ? 0.f : top;
+    const float k = exp2f(mine - base);                           // NaN stays NaN
+    const float sum = wave_total(k);
+    float acc[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.f;
+    const float* o = a.work + (int64_t)row * DIM + lane * W;
+#pragma unroll 8
     for (int s = 0; s < slots; ++s) {
-        const float v = lse[(int64_t)s * rows];
-        if (v == -INFINITY) continue;
-        const float k = exp2f(v - top);
-        float o[W];
-        load_vec<float, W>(a.work + ((int64_t)s * rows + row) * DIM + lane * W, o);
-        sum += k;
+        float v[W];
+        load_vec<float, W>(o + (int64_t)s * rows * DIM, v);
+        const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k), s));
 #pragma unroll
-        for (int i = 0; i < W; ++i) acc[i] += k * o[i];
+        for (int i = 0; i < W; ++i) acc[i] += ks * v[i];
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int i = 0; i < W; ++i) acc[i] = odd ? __builtin_nanf("") : acc[i] * inv;
+    for (int i = 0; i < W; ++i) acc[i] *= inv;
     store_vec<T, W>(static_cast<T*>(a.out) + (int64_t)row * DIM + lane * W, acc);
     if (a.lse && lane == 0) {
         const int h = row % a.heads, bq = row / a.heads, b = bq / a.queries, i = bq % a.queries;
-        a.lse[((int64_t)b * a.heads + h) * a.queries + i] = odd ? __builtin_nanf("") : sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+        a.lse[((int64_t)b * a.heads + h) * a.queries + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
 }
 
-template <class T, int DIM, int RT, bool BYWAVE>
-hipError_t launch_one(const PrefixAttnArgs& a, const PrefixAttnLaunch& l, int slots, hipStream_t stream) {
-    constexpr int LDS = BYWAVE ? 4 * 2 * 2 * 32 * DIM * 2 : 2 * 2 * 64 * DIM * 2;
-    static_assert(!BYWAVE || LDS >= (4 * 16 * (DIM + 4) + 128) * 4, "the join fits the ring");
-    auto* kernel = prefix_attention_kernel<T, DIM, RT, BYWAVE>;
-    static PerDevice<int> set;
-    int& done = set.get();
-    if (LDS > 64 * 1024 && !done) {
-        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-        if (e != hipSuccess) return e;
-        done = 1;
-    }
-    const int64_t blocks = (int64_t)(l.packed ? 1 : a.batch) * a.kv_heads * l.tiles * l.chunks;
-    kernel<<<dim3((unsigned)blocks), 256, LDS, stream>>>(a, l, slots);
+template <class T, int DIM, int KIND_A, int KIND_B>
+hipError_t launch_kinds(const PrefixAttnArgs& a, const PrefixAttnPlan& p, hipStream_t stream) {
+    constexpr int LA = lds_bytes<DIM, KIND_A == 0>(), LB = lds_bytes<DIM, KIND_B == 0>(), LDS = LA > LB ? LA : LB;
+    static_assert((KIND_A != 0 && KIND_B != 0) || LDS >= (4 * 16 * (DIM + 4) + 128) * 4, "the join fits the rings");
+    static_assert(LDS <= 64 * 1024, "no attribute needed");
+    auto blocks = [&](const PrefixAttnLaunch& l) { return (int64_t)(l.packed ? 1 : a.batch) * a.kv_heads * l.tiles * l.chunks; };
+    const int64_t n0 = blocks(p.l[0]), n1 = p.n > 1 ? blocks(p.l[1]) : 0;
+    prefix_attention_kernel<T, DIM, KIND_A, KIND_B><<<dim3((unsigned)(n0 + n1)), 256, LDS, stream>>>(a, p.l[0], p.l[1], (int)n0, p.slots);
     return hipGetLastError();
 }
 
 template <class T, int DIM>
 hipError_t launch_dim(const PrefixAttnArgs& a, const PrefixAttnPlan& p, hipStream_t stream) {
-    for (int i = 0; i < p.n; ++i) {
-        hipError_t e;
-        switch (p.l[i].kind) {
-            case 0: e = launch_one<T, DIM, 1, true>(a, p.l[i], p.slots, stream); break;
-            case 1: e = launch_one<T, DIM, 1, false>(a, p.l[i], p.slots, stream); break;
-            default: e = launch_one<T, DIM, 2, false>(a, p.l[i], p.slots, stream); break;
-        }
-        if (e != hipSuccess) return e;
-    }
-    if (p.slots > 1) {
-        const int rows = a.batch * a.queries * a.heads;
-        prefix_attention_join_kernel<T, DIM><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, stream>>>(a, p.slots, rows);
-        return hipGetLastError();
-    }
-    return hipSuccess;
+    const int ka = p.l[0].kind, kb = p.n > 1 ? p.l[1].kind : ka;   // the packed prefix has at least the own keys' rows: ka >= kb
+    hipError_t e;
+    if (ka == 0) e = launch_kinds<T, DIM, 0, 0>(a, p, stream);
+    else if (ka == 1) e = kb == 0 ? launch_kinds<T, DIM, 1, 0>(a, p, stream) : launch_kinds<T, DIM, 1, 1>(a, p, stream);
+    else e = kb == 0 ? launch_kinds<T, DIM, 2, 0>(a, p, stream) : kb == 1 ? launch_kinds<T, DIM, 2, 1>(a, p, stream) : launch_kinds<T, DIM, 2, 2>(a, p, stream);
+    if (e != hipSuccess || p.slots == 1) return e;
+    const int rows = a.batch * a.queries * a.heads;
+    prefix_attention_join_kernel<T, DIM><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, stream>>>(a, p.slots, rows);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -422,9 +504,10 @@ PrefixAttnPlan prefix_attention_plan(const PrefixAttnArgs& a, int cus) {
         l.tiles = (int)((rows + bm - 1) / bm);
         const int64_t items = (int64_t)(packed ? 1 : a.batch) * a.kv_heads * l.tiles;
         const int keys = k_end - k_begin, unit = 128;
-        // fill the chip (two blocks a CU) with chunks of at least 256 keys
+        // fill the chip (two blocks a CU) with chunks of at least 256 keys (512 for the widest tiles, whose partial results are the
+        // largest); at most 32 of them, so that a wave of the join holds all weights
         int64_t n = (2 * cus + items - 1) / items;
-        n = std::min<int64_t>(n, std::max(1, keys / 256));
+        n = std::min<int64_t>(n, std::max(1, keys / (l.kind == 2 ? 512 : 256)));
         n = std::min<int64_t>(n, 32);
         l.chunk = (int)std::max<int64_t>(unit, ((keys + n - 1) / n + unit - 1) / unit * unit);   // no keys at all: one empty chunk
         l.chunks = std::max(1, (keys + l.chunk - 1) / l.chunk);
@@ -435,8 +518,10 @@ PrefixAttnPlan prefix_attention_plan(const PrefixAttnArgs& a, int cus) {
     if (a.batch > 1 && a.prefix >= 256 && rows_own < 64) {
         add(true, 0, a.prefix);
         if (a.own_max > 0) add(false, a.prefix, a.prefix + a.own_max);
+        else plan.l[1] = plan.l[0];
     } else {
         add(false, 0, a.prefix + a.own_max);
+        plan.l[1] = plan.l[0];
     }
     return plan;
 }
