@@ -78,26 +78,27 @@ __device__ __forceinline__ float over_groups_sum(float v) {
 
 template <int DIM, bool BYWAVE>
 constexpr int lds_bytes() {
-    // by rows: two stages of 64 keys and 64 values; by wave: each of the four has two stages of 32 values
-    return BYWAVE ? 4 * 2 * 32 * DIM * 2 : 2 * 2 * 64 * DIM * 2;
+    // by rows: three stages of 64 keys, two of 64 values; by wave: each of the four has two stages of 32 values
+    return BYWAVE ? 4 * 2 * 32 * DIM * 2 : 5 * 64 * DIM * 2;
 }
 
 // One item: a tile of rows over a chunk of keys.
-//   By rows: wave w owns rows [16 RT w, +16 RT); K and V come in 64-key stages through LDS (LDS-DMA), two of each.  The scores of
-//   stage s + 1 are multiplied while the softmax of stage s runs, so the matrix units work under the exponentials.
+//   By rows: wave w owns rows [16 RT w, +16 RT); K and V come in 64-key stages through LDS (LDS-DMA, three stages of K, two of V).
+//   A stage is two units of 32 keys; the scores of the next unit are multiplied while the softmax of this one runs, so the matrix
+//   units work under the exponentials.
 //   BYWAVE: at most 16 rows (few queries): a wave takes every fourth 32-key tile, its K straight into registers, its V through its own
 //   two LDS slots, no barrier until the four waves join at the end.
 // A row's maximum is moved only when a score passes it by 2^8: until then its p stay below 256, which changes no relative
 // rounding and saves the exchange between the lanes and the rescaling of o.
 template <class T, int DIM, int RT, bool BYWAVE>
 __device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int slots, int block, int blocks, char* lds_all) {
-    constexpr int KT = BYWAVE ? 32 : 64, ROWB = DIM * 2, TILE = KT * ROWB, KB = KT / 16, DB = DIM / 16, DS = DIM / 32;
+    constexpr int KT = BYWAVE ? 32 : 64, ROWB = DIM * 2, TILE = KT * ROWB, KB = 2, DB = DIM / 16, DS = DIM / 32;
     constexpr int SLOTS = DIM / 8, RPP = 64 / SLOTS;              // 16-byte slots of a key row; key rows of a 1-KiB piece
     constexpr int PIECES = KT / RPP / (BYWAVE ? 1 : 4);           // pieces of a tile that a wave brings
     static_assert(!BYWAVE || RT == 1, "");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l15 = lane & 15, g = lane >> 4;
-    // by rows: K slots at 0, 1, V slots at 2, 3 tiles; by wave: the wave's two V slots
+    // by rows: K slots at 0 .. 2, V slots at 3, 4 tiles; by wave: the wave's two V slots
     char* lds = lds_all + (BYWAVE ? wave * 2 * TILE : 0);
 
     // ---- which item ----
@@ -187,7 +188,7 @@ __device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttn
             bring(first, true, lds);
         } else {
             bring(0, false, lds);
-            bring(0, true, lds + 2 * TILE);
+            bring(0, true, lds + 3 * TILE);
             if (stages > 1) bring(1, false, lds + TILE);
         }
     }
@@ -230,12 +231,12 @@ __device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttn
             }
         }
     };
-    // masks, and the running maximum brought above the scores less 2^8
-    auto settle = [&](int s, f32x4 (&sc)[KB][RT]) {
+    // masks of unit `u` of stage s, and the running maximum brought above the scores less 2^8
+    auto settle = [&](int s, int u, f32x4 (&sc)[KB][RT]) {
         const bool own = s >= np;
-        const int k0 = own ? o0 + (s - np) * KT : p0 + s * KT;
+        const int k0 = (own ? o0 + (s - np) * KT : p0 + s * KT) + 32 * u;
         const int end = own ? o1 : p1;
-        if (k0 + KT > end || (own && k0 + KT > vis_low)) {        // keys behind the chunk's end, own keys a row does not see
+        if (k0 + 32 > end || (own && k0 + 32 > vis_low)) {        // keys behind the chunk's end, own keys a row does not see
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
                 const int lim = own && vis[t] < end ? vis[t] : end;
@@ -270,42 +271,50 @@ __device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttn
             }
         }
     };
-    // P^T as the B operand of each 32-key block, its sum into l
-    auto weights = [&](const f32x4 (&sc)[KB][RT], s8 (&p)[KB / 2][RT]) {
+    // P^T as the B operand of the unit's products, its sum into l
+    auto weights = [&](const f32x4 (&sc)[KB][RT], s8 (&p)[RT]) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             const float base = m[t] == -INFINITY ? 0.f : m[t];    // nothing seen yet: every p is 2^-inf = 0
+            float e[8];
 #pragma unroll
-            for (int kb = 0; kb < KB; kb += 2) {
-                float e[8];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][t][r], scale2, -base));
-                    e[4 + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb + 1][t][r], scale2, -base));
-                }
-                l[t] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                struct { unsigned u[4]; } w;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) w.u[r] = Mma<T>::pack(e[2 * r], e[2 * r + 1]);
-                p[kb / 2][t] = __builtin_bit_cast(s8, w);
+            for (int r = 0; r < 4; ++r) {
+                e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[0][t][r], scale2, -base));
+                e[4 + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[1][t][r], scale2, -base));
             }
+            l[t] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+            struct { unsigned u[4]; } w;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w.u[r] = Mma<T>::pack(e[2 * r], e[2 * r + 1]);
+            p[t] = __builtin_bit_cast(s8, w);
         }
     };
-    auto values = [&](const char* vt, const s8 (&p)[KB / 2][RT]) {
+    // O^T += V^T P^T over 32 keys.  AHEAD fragments are on their way from LDS at any time, the first ones asked for before the softmax
+    // ends (as the compiler orders it alone, each product waits for its own read)
+    constexpr int AHEAD = 4;
+    s8 vf[AHEAD];
+    auto v_frag = [&](const char* vt, int d) {
+        const char* at = vt + vrow + ((vsl ^ (2 * d)) << 4);
+        const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
+        const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + 16 * ROWB));
+        return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    auto values_ahead = [&](const char* vt) {
 #pragma unroll
-        for (int kk = 0; kk < KB / 2; ++kk)
+        for (int d = 0; d < AHEAD; ++d) vf[d] = v_frag(vt, d);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto values = [&](const char* vt, const s8 (&p)[RT]) {
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const char* at = vt + kk * 32 * ROWB + vrow + ((vsl ^ (2 * d)) << 4);
-                const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)at);
-                const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + 16 * ROWB));
-                const s8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int d = 0; d < DB; ++d) {
 #pragma unroll
-                for (int t = 0; t < RT; ++t) o[t][d] = Mma<T>::mul(v, p[kk][t], o[t][d]);
-            }
+            for (int t = 0; t < RT; ++t) o[t][d] = Mma<T>::mul(vf[d % AHEAD], p[t], o[t][d]);
+            if (d + AHEAD < DB) vf[d % AHEAD] = v_frag(vt, d + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
-    s8 p[KB / 2][RT];
+    s8 p[RT];
     if constexpr (BYWAVE) {
         auto one = [&](int s, int buf) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the other slot's reads are done
@@ -316,10 +325,11 @@ __device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttn
             }
             f32x4 sc[KB][RT];
             scores(nullptr, buf, sc);
-            settle(s, sc);
+            settle(s, 0, sc);
             weights(sc, p);
             if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES + KB * DS) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            values_ahead(lds + buf * TILE);
             values(lds + buf * TILE, p);
         };
         for (int s = first; s < stages; s += 2 * step) {
@@ -327,31 +337,40 @@ __device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttn
             if (s + step < stages) one(s + step, 1);
         }
     } else if (stages > 0) {
-        f32x4 sc[KB][RT];
+        f32x4 sc[KB][RT], nx[KB][RT];
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         scores(lds, 0, sc);
+        const char* kt = lds;                                     // K of stage s, s + 1; V of s
+        char* kn = lds + TILE;
+        char* k2 = lds + 2 * TILE;
+        char* vt = lds + 3 * TILE;
+        char* vn = lds + 4 * TILE;
         for (int s = 0; s < stages; ++s) {
-            const int at = s & 1;
-            // K of s + 1 and V of s are in LDS, and every wave has left K of s and V of s - 1
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (s + 2 < stages) bring(s + 2, false, lds + at * TILE);
-            if (s + 1 < stages) bring(s + 1, true, lds + (2 + (at ^ 1)) * TILE);
-            settle(s, sc);
-            if (s + 1 < stages) {
-                f32x4 nx[KB][RT];
-                scores(lds + (at ^ 1) * TILE, 0, nx);
-                weights(sc, p);
-                values(lds + (2 + at) * TILE, p);
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) sc[kb][t] = nx[kb][t];
-            } else {
-                weights(sc, p);
-                values(lds + (2 + at) * TILE, p);
+            // K of s + 1 and V of s are in LDS, and every wave has left K and V of s - 1
+            if (s > 0) {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
             }
+            if (s + 2 < stages) bring(s + 2, false, k2);
+            if (s + 1 < stages) bring(s + 1, true, vn);
+            settle(s, 0, sc);
+            scores(kt + 32 * ROWB, 0, nx);
+            weights(sc, p);
+            values_ahead(vt);
+            values(vt, p);
+            settle(s, 1, nx);
+            scores(kn, 0, sc);                                    // (the last stage: what lies there, not used)
+            weights(nx, p);
+            values_ahead(vt + 32 * ROWB);
+            values(vt + 32 * ROWB, p);
+            char* was = const_cast<char*>(kt);
+            kt = kn;
+            kn = k2;
+            k2 = was;
+            was = vt;
+            vt = vn;
+            vn = was;
         }
     }
 #pragma unroll
@@ -467,7 +486,17 @@ template <class T, int DIM, int KIND_A, int KIND_B>
 hipError_t launch_kinds(const PrefixAttnArgs& a, const PrefixAttnPlan& p, hipStream_t stream) {
     constexpr int LA = lds_bytes<DIM, KIND_A == 0>(), LB = lds_bytes<DIM, KIND_B == 0>(), LDS = LA > LB ? LA : LB;
     static_assert((KIND_A != 0 && KIND_B != 0) || LDS >= (4 * 16 * (DIM + 4) + 128) * 4, "the join fits the rings");
-    static_assert(LDS <= 64 * 1024, "no attribute needed");
+    static_assert(LDS <= 80 * 1024, "two blocks a CU");
+    if (LDS > 64 * 1024) {
+        static PerDevice<int> set;
+        int& done = set.get();
+        if (!done) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_attention_kernel<T, DIM, KIND_A, KIND_B>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+            if (e != hipSuccess) return e;
+            done = 1;
+        }
+    }
     auto blocks = [&](const PrefixAttnLaunch& l) { return (int64_t)(l.packed ? 1 : a.batch) * a.kv_heads * l.tiles * l.chunks; };
     const int64_t n0 = blocks(p.l[0]), n1 = p.n > 1 ? blocks(p.l[1]) : 0;
     prefix_attention_kernel<T, DIM, KIND_A, KIND_B><<<dim3((unsigned)(n0 + n1)), 256, LDS, stream>>>(a, p.l[0], p.l[1], (int)n0, p.slots);
