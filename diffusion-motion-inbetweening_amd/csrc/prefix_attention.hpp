@@ -21,7 +21,7 @@ struct PrefixAttnArgs {
 // has several partial results.
 struct PrefixAttnLaunch {
     int32_t packed;                      // rows of all samples together (prefix keys only)
-    int32_t kind;                        // 0: a wave a key tile, at most 16 rows;  1, 2: tiles of 64, 128 rows, 16 or 32 a wave
+    int32_t by_wave;                     // at most 32 rows: a wave a key tile;  else tiles of 128 rows, 32 a wave
     int32_t k_begin, k_end;              // range on the axis [prefix keys | own keys]
     int32_t chunk, chunks, tiles, slot0;
 };
