@@ -58,19 +58,21 @@ __device__ __forceinline__ int swz(int k) {
     return DIM == 128 ? ((k & 3) << 2) | ((k >> 2) & 3) : (((k >> 1) & 3) << 1) | ((k >> 3) & 1);
 }
 
-// 16 bytes a lane from `offset` behind the descriptor's base to LDS at `to`, lane after lane.  In assembly because the compiler
+// 16 bytes a lane from `offset` behind the descriptor's base to LDS at `to` + PLUS, lane after lane.  In assembly because the compiler
 // puts a wait for ALL requests in front of the next transposed LDS read when it knows of one: the waits below count them instead.
 // (It has no result register; a wait that the compiler counts for its own loads only gets longer by requests it does not know of.)
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void dma16(u4 descriptor, char* to, int offset) {
-    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)to;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(offset), "s"(descriptor) : "memory", "m0");
+template <int PLUS>
+__device__ __forceinline__ void dma16(u4 descriptor, unsigned to, int offset) {
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(descriptor), "n"(PLUS)
+                 : "memory", "m0", "scc");
 }
 // a raw buffer: `bytes` from `base`, accesses behind them return zeros
 __device__ __forceinline__ u4 buffer(const char* base, int bytes) {
     const uint64_t at = reinterpret_cast<uint64_t>(base);
     return u4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, (unsigned)bytes, 0x00020000u};
 }
+__device__ __forceinline__ unsigned lds_at(const char* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 
 template <int DIM, bool BYWAVE>
 constexpr int lds_bytes() {
@@ -78,393 +80,491 @@ constexpr int lds_bytes() {
     return BYWAVE ? 4 * 2 * 32 * DIM * 2 : 5 * 64 * DIM * 2;
 }
 
-// The item's keys, tile by tile: its part of the prefix, then its part of the own keys.  A walker stands at one tile; a step costs
-// a handful of scalar instructions but where it crosses into the own keys.
-struct Segment { const char *k, *v; int ks, vs, n; };             // first key's addresses, bytes between keys, number of keys
-template <int KT>
-struct Walker {
-    int tile, at;                                                 // tile number; first key of the tile within its segment
-    bool own;
-    __device__ __forceinline__ void go(int t, int prefix_tiles) {
-        tile = t;
-        own = t >= prefix_tiles;
-        at = (own ? t - prefix_tiles : t) * KT;
+// Which rows and which keys an item has.
+template <int BM, int KT>
+struct Item {
+    int chunk, n_rows, row0, hk, b0;      // row0: the wave's first row
+    bool row_ok;                          // this lane's row exists (else it repeats the last one)
+    int row_b, row_i, row_h, vis;         // the lane's sample, query, head; own keys it sees
+    int vis_low;                          // own keys that the wave's first row sees
+    int c0, p1, o0, o1;                   // prefix keys [c0, p1), own keys [o0, o1)
+    int np, tiles;                        // tiles of KT keys: prefix ones, all
+
+    __device__ __forceinline__ Item(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int block, int blocks, int first_row, int l31) {
+        const int grp = a.heads / a.kv_heads;
+        const int id = xcd_remap(block, blocks);
+        const int tile = id % L.tiles, rest = id / L.tiles;
+        const int bh = rest / L.chunks;
+        chunk = rest % L.chunks;
+        hk = bh % a.kv_heads;
+        b0 = bh / a.kv_heads;                                     // packed: 0, the sample comes from the row
+        n_rows = (L.packed ? a.batch : 1) * a.queries * grp;
+        row0 = tile * BM + first_row;
+        row_ok = row0 + l31 < n_rows;
+        const int r = row_ok ? row0 + l31 : n_rows - 1;
+        const int rq = r / grp;
+        row_h = hk * grp + r - rq * grp;
+        row_b = L.packed ? rq / a.queries : b0;
+        row_i = L.packed ? rq - row_b * a.queries : rq;
+        vis = vis_low = 0;
+        int vis_top = 0;                                          // own keys that the block's last row sees
+        if (L.k_end > a.prefix) {                                 // (never for packed rows)
+            int len = a.own_len ? a.own_len[b0] : a.own_max;
+            len = len < 0 ? 0 : len > a.own_max ? a.own_max : len;
+            auto sees = [&](int i) {
+                const int v = a.causal ? len - a.queries + i + 1 : len;
+                return v < 0 ? 0 : v > len ? len : v;
+            };
+            vis = sees(row_i);
+            vis_top = sees(((tile + 1) * BM < n_rows ? (tile + 1) * BM - 1 : n_rows - 1) / grp);
+            vis_low = sees(row0 / grp);
+        }
+        c0 = L.k_begin + chunk * L.chunk;
+        const int c1 = c0 + L.chunk < L.k_end ? c0 + L.chunk : L.k_end;
+        p1 = c1 < a.prefix ? c1 : a.prefix;
+        o0 = c0 > a.prefix ? c0 - a.prefix : 0;
+        o1 = c1 - a.prefix < vis_top ? c1 - a.prefix : vis_top;
+        np = p1 > c0 ? (p1 - c0 + KT - 1) / KT : 0;
+        tiles = np + (o1 > o0 ? (o1 - o0 + KT - 1) / KT : 0);
     }
 };
 
-// One item: a tile of rows over a chunk of keys.
-//   By rows: wave w owns 32 of 128 rows; K and V come in 64-key tiles through LDS (LDS-DMA, a ring of three tiles of K, of two of V).
-//   A tile is two units of 32 keys; the scores of the next unit are multiplied while the softmax of this one runs, so the matrix
-//   units work under the exponentials.
-//   BYWAVE: at most 32 rows (few queries): a wave takes every fourth 32-key tile, its K straight into registers, its V through its own
-//   two LDS tiles, no barrier until the four waves join at the end.
-// A row's maximum is moved only when a score passes it by 2^8: until then its p stay below 256, which changes no relative
-// rounding and saves the exchange between the lanes and the rescaling of o.
-template <class T, int DIM, bool BYWAVE>
-__device__ __forceinline__ void attend(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int slots, int block, int blocks, char* lds_all) {
-    constexpr int KT = BYWAVE ? 32 : 64, ROWB = DIM * 2, TILE = KT * ROWB, DS = DIM / 16, DB = DIM / 32;
-    constexpr int SLOTS = DIM / 8, RPP = 64 / SLOTS;              // 16-byte slots of a key row; key rows of a 1-KiB piece
-    constexpr int PIECES = KT / RPP / (BYWAVE ? 1 : 4);           // pieces of a tile that a wave brings
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l31 = lane & 31, hi = lane >> 5;
-    char* lds = lds_all + (BYWAVE ? wave * 2 * TILE : 0);
-
-    // ---- which item ----
-    const int grp = a.heads / a.kv_heads;
-    const int id = xcd_remap(block, blocks);
-    const int tile = id % L.tiles, rest = id / L.tiles;
-    const int chunk = rest % L.chunks, bh = rest / L.chunks;
-    const int hk = bh % a.kv_heads, b0 = bh / a.kv_heads;         // packed: b0 = 0, the sample comes from the row
-    const int n_rows = (L.packed ? a.batch : 1) * a.queries * grp;
-    constexpr int BM = BYWAVE ? 32 : 128;
-    const int row0 = tile * BM + (BYWAVE ? 0 : wave * 32);
-    const bool busy = row0 < n_rows;                              // this wave has rows (it brings keys in any case)
-    const bool row_ok = row0 + l31 < n_rows;
-    const int r = row_ok ? row0 + l31 : n_rows - 1;               // this lane's row
-    const int rq = r / grp, row_h = hk * grp + r - rq * grp, row_b = L.packed ? rq / a.queries : b0;
-    const int row_i = L.packed ? rq - row_b * a.queries : rq;
-
-    // ---- own keys that the lane's row, the block's last row and the wave's first one see ----
-    int vis = 0, vis_top = 0, vis_low = 0;
-    if (L.k_end > a.prefix) {                                     // (never for packed rows)
-        int len = a.own_len ? a.own_len[b0] : a.own_max;
-        len = len < 0 ? 0 : len > a.own_max ? a.own_max : len;
-        auto sees = [&](int i) {
-            const int v = a.causal ? len - a.queries + i + 1 : len;
-            return v < 0 ? 0 : v > len ? len : v;
-        };
-        vis = sees(row_i);
-        vis_top = sees(((tile + 1) * BM < n_rows ? (tile + 1) * BM - 1 : n_rows - 1) / grp);
-        vis_low = sees(row0 / grp);
+// A walk over an item's keys or values, tile by tile: its part of the prefix, then of the own keys.  `left` keys from `at` on are in
+// the segment.  A tile is read through a descriptor that ends with the segment's last key: what lies behind it reads as zeros.
+template <class I, int DIM, int KT>
+struct Walk {
+    const char* at;
+    int left, stride;                     // stride: bytes between keys
+    bool own;
+    __device__ __forceinline__ void enter(const PrefixAttnArgs& a, const I& it, bool values, bool own_keys, int skip) {
+        own = own_keys;
+        const int64_t ss = own ? (values ? a.ov_ss : a.ok_ss) : (values ? a.pv_ss : a.pk_ss);
+        const int64_t hs = own ? (values ? a.ov_hs : a.ok_hs) : (values ? a.pv_hs : a.pk_hs);
+        const int64_t bs = own ? (values ? a.ov_bs : a.ok_bs) : 0;
+        stride = (int)(ss * 2);
+        left = (own ? it.o1 - it.o0 : it.p1 - it.c0) - skip;
+        at = static_cast<const char*>(own ? (values ? a.ov : a.ok) : (values ? a.pv : a.pk)) +
+             (it.b0 * bs + it.hk * hs + (int64_t)((own ? it.o0 : it.c0) + skip) * ss) * 2;
     }
-    // ---- its keys: prefix [p0, p1), own [o0, o1) ----
-    const int c0 = L.k_begin + chunk * L.chunk;
-    const int c1 = c0 + L.chunk < L.k_end ? c0 + L.chunk : L.k_end;
-    const int p1 = c1 < a.prefix ? c1 : a.prefix;
-    const int o0 = c0 > a.prefix ? c0 - a.prefix : 0;
-    const int o1 = c1 - a.prefix < vis_top ? c1 - a.prefix : vis_top;
-    auto segment = [&](bool own) {
-        Segment g;
-        g.n = own ? (o1 > o0 ? o1 - o0 : 0) : (p1 > c0 ? p1 - c0 : 0);
-        const int from = own ? o0 : c0;
-        g.ks = (int)((own ? a.ok_ss : a.pk_ss) * 2);
-        g.vs = (int)((own ? a.ov_ss : a.pv_ss) * 2);
-        const char* k = static_cast<const char*>(own ? a.ok : a.pk);
-        const char* v = static_cast<const char*>(own ? a.ov : a.pv);
-        g.k = k + ((own ? b0 * a.ok_bs : 0) + hk * (own ? a.ok_hs : a.pk_hs)) * 2 + (int64_t)from * g.ks;
-        g.v = v + ((own ? b0 * a.ov_bs : 0) + hk * (own ? a.ov_hs : a.pv_hs)) * 2 + (int64_t)from * g.vs;
-        return g;
-    };
-    const int np = p1 > c0 ? (p1 - c0 + KT - 1) / KT : 0;
-    const int no = o1 > o0 ? (o1 - o0 + KT - 1) / KT : 0;
-    const int stages = np + no;
-    const int first = BYWAVE ? wave : 0, step = BYWAVE ? 4 : 1;
-
-    // A tile's keys or values through a descriptor that ends with the segment's last key: keys behind it read as zeros whatever lies
-    // there.  The lane's offset within a tile changes with the segment's stride only.
-    struct Cursor { Walker<KT> w; Segment g; };
-    auto start = [&](Cursor& c, int t) {
-        c.w.go(t, np);
-        c.g = segment(c.w.own);
-    };
-    auto advance = [&](Cursor& c, int by) {
-        const bool was = c.w.own;
-        c.w.go(c.w.tile + by, np);
-        if (c.w.own != was) c.g = segment(true);
-    };
-    auto tile_of = [&](const Cursor& c, bool values, const char*& base, int& bytes) {
-        const int left = c.g.n - c.w.at, valid = left < KT ? left : KT, stride = values ? c.g.vs : c.g.ks;
-        base = (values ? c.g.v : c.g.k) + (int64_t)c.w.at * stride;
-        bytes = (valid - 1) * stride + ROWB;
-    };
-    const int w4 = BYWAVE ? 0 : wave;
-    auto bring = [&](const Cursor& c, bool values, char* to) {
-        const char* base;
-        int bytes;
-        tile_of(c, values, base, bytes);
-        const u4 d = buffer(base, bytes);
-        const int stride = values ? c.g.vs : c.g.ks;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int pc = i + w4 * PIECES, key = pc * RPP + lane / SLOTS, t = (lane % SLOTS) ^ swz<DIM>(key);
-            dma16(d, to + pc * 1024, key * stride + t * 16);
+    __device__ __forceinline__ void start(const PrefixAttnArgs& a, const I& it, bool values, int tile) {
+        const bool o = tile >= it.np;
+        enter(a, it, values, o, (o ? tile - it.np : tile) * KT);
+    }
+    __device__ __forceinline__ u4 tile() const { return buffer(at, ((left < KT ? left : KT) - 1) * stride + DIM * 2); }
+    // `by` tiles on; true where that entered the own keys
+    __device__ __forceinline__ bool step(const PrefixAttnArgs& a, const I& it, bool values, int by) {
+        at += (int64_t)by * KT * stride;
+        left -= by * KT;
+        if (__builtin_expect(left <= 0 && !own, 0)) {
+            const int np = (it.p1 - it.c0 + KT - 1) / KT * KT, over = (it.p1 - it.c0 - left) - np;   // keys walked behind the prefix's last tile
+            enter(a, it, values, true, over);
+            return true;
         }
-    };
-    s8 kreg[2][BYWAVE ? DS : 1];                                  // by wave: the K operand, this tile's and the next one's
-    auto load_k = [&](const Cursor& c, int buf) {
-        const char* base;
-        int bytes;
-        tile_of(c, false, base, bytes);
-        const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, bytes, 0x00020000);
-#pragma unroll
-        for (int s = 0; s < (BYWAVE ? DS : 0); ++s)
-            kreg[buf][s] = __builtin_bit_cast(s8, (u4)__builtin_amdgcn_raw_buffer_load_b128(d, l31 * c.g.ks + 32 * s + 16 * hi, 0, 0));
-    };
-    Cursor ck, cv;                                                // the next tile of K and of V to ask for
-    start(ck, first);
-    cv = ck;
-    if (first < stages) {
-        if constexpr (BYWAVE) {
-            load_k(ck, 0);
-            bring(cv, true, lds);
-        } else {
-            bring(ck, false, lds);
-            bring(cv, true, lds + 3 * TILE);
-            advance(ck, 1);
-            if (stages > 1) bring(ck, false, lds + TILE);
-            advance(ck, 1);
-        }
-        advance(cv, step);
+        return false;
     }
+};
 
-    // ---- Q as the B operand: lane (row l31, dims 16 s + 8 hi ..) ----
-    s8 q[DS];
-    {
-        const short* p = static_cast<const short*>(a.q) + row_b * a.q_bs + row_i * a.q_ss + row_h * a.q_hs + 8 * hi;
-#pragma unroll
-        for (int s = 0; s < DS; ++s) q[s] = *reinterpret_cast<const s8*>(p + 16 * s);
-    }
-
+// A wave's 32 rows against 32 keys at a time.  A row's maximum is moved only when a score passes it by 2^8: until then its p stay
+// below 256, which changes no relative rounding and saves the exchange between the lanes and the rescaling of o.
+template <class T, int DIM>
+struct Rows32 {
+    static constexpr int ROWB = DIM * 2, DS = DIM / 16, DB = DIM / 32, FRAGS = 2 * DB, AHEAD = 4;
+    s8 q[DS], p[2], vf[AHEAD];
     f32x16 o[DB];
-    float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    const float scale2 = a.scale * kLog2e;
-    const int kswz = swz<DIM>(l31), krow = l31 * ROWB;            // K: key l31 of a 32-key unit
-    // V, transposed reads: group G = lane / 16, lane L of it points at key 4 (G / 2) + L / 4, dims 16 (G % 2) + 4 (L % 4) .. + 3; the
-    // group's lane i receives keys 4 (G / 2) .. + 3 of dim 16 (G % 2) + i
-    const int vkey = 4 * hi + ((lane & 15) >> 2);
-    const int vrow = vkey * ROWB + (lane & 1) * 8, vsl = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    const int vs0 = vsl ^ swz<DIM>(vkey), vs1 = vsl ^ swz<DIM>(vkey + 8);
+    float m, l, limit, base;              // limit: a raw score above it moves m;  base: -m, or 0 while nothing is seen
+    float scale2;
+    int krow[DS], vat[DB], vat8[DB];      // LDS offsets of the lane's fragments within a 32-key unit
 
-    // the K fragments of a unit are asked for before the softmax of the one before it begins
-    s8 kf[BYWAVE ? 1 : DS];
-    auto keys_ahead = [&](const char* kt) {
+    __device__ __forceinline__ Rows32(float scale, int lane) {
+        const int l31 = lane & 31, hi = lane >> 5;
+        m = -INFINITY;
+        l = 0.f;
+        limit = -INFINITY;
+        base = 0.f;
+        scale2 = scale * kLog2e;
 #pragma unroll
-        for (int s = 0; s < (BYWAVE ? 0 : DS); ++s) kf[s] = *reinterpret_cast<const s8*>(kt + krow + (((2 * s + hi) ^ kswz) << 4));
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+        // K: key l31, dims 16 s + 8 hi ..
+#pragma unroll
+        for (int s = 0; s < DS; ++s) krow[s] = l31 * ROWB + (((2 * s + hi) ^ swz<DIM>(l31)) << 4);
+        // V, transposed reads: group G = lane / 16, lane L of it points at key 4 (G / 2) + L / 4, dims 16 (G % 2) + 4 (L % 4) .. + 3; the
+        // group's lane i receives keys 4 (G / 2) .. + 3 of dim 16 (G % 2) + i
+        const int key = 4 * hi + ((lane & 15) >> 2), slot = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), byte = key * ROWB + (lane & 1) * 8;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            vat[d] = byte + (((slot + 4 * d) ^ swz<DIM>(key)) << 4);
+            vat8[d] = byte + 8 * ROWB + (((slot + 4 * d) ^ swz<DIM>(key + 8)) << 4);
+        }
+    }
+    __device__ __forceinline__ void load_q(const short* at) {
+#pragma unroll
+        for (int s = 0; s < DS; ++s) q[s] = *reinterpret_cast<const s8*>(at + 16 * s);
+    }
+    __device__ __forceinline__ void q_is_there() {
+#pragma unroll
+        for (int s = 0; s < DS; ++s) asm volatile("" : "+v"(q[s]));
+    }
+    // the fragments of a unit's keys, asked for before the softmax of the unit before it begins
+    __device__ __forceinline__ void keys(const char* kt, s8 (&kf)[DS]) const {
+#pragma unroll
+        for (int s = 0; s < DS; ++s) kf[s] = *reinterpret_cast<const s8*>(kt + krow[s]);
         __builtin_amdgcn_sched_barrier(0);
-    };
-    auto scores = [&](int buf, f32x16& sc) {
+    }
+    __device__ __forceinline__ void scores(const s8 (&kf)[DS], f32x16& sc) const {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-        for (int s = 0; s < DS; ++s) {
-            if constexpr (BYWAVE) sc = Mma<T>::mul(kreg[buf][s], q[s], sc);
-            else sc = Mma<T>::mul(kf[s], q[s], sc);
-        }
-    };
-    // masks of the unit whose first key is `k0` of the segment's, and the running maximum brought above the scores less 2^8
-    auto settle = [&](const Walker<KT>& w, int unit, f32x16& sc) {
-        const int k0 = w.at + 32 * unit, n = w.own ? o1 - o0 : p1 - c0;
-        if (k0 + 32 > n || (w.own && o0 + k0 + 32 > vis_low)) {   // keys behind the chunk's end, own keys a row does not see
-            const int lim = w.own && vis - o0 < n ? vis - o0 : n;
+        for (int s = 0; s < DS; ++s) sc = Mma<T>::mul(kf[s], q[s], sc);
+    }
+    // keys from `lim` on (of the unit's 32) are hidden from the lane's row
+    __device__ __forceinline__ void mask(f32x16& sc, int lim, int lane) const {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (k0 + mfma32_row(i, lane) >= lim) sc[i] = -INFINITY;
-        }
-        float top = sc[0];
+        for (int i = 0; i < 16; ++i)
+            if (mfma32_row(i, lane) >= lim) sc[i] = -INFINITY;
+    }
+    __device__ __forceinline__ void settle(const f32x16& sc) {
+        float top = fmaxf(sc[0], sc[1]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
-        top *= scale2;
-        if (__any(top > m + 8.f)) {
-            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+        for (int i = 2; i < 16; ++i) top = fmaxf(top, sc[i]);
+        if (__builtin_expect(__any(top > limit), 0)) {
+            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * scale2);
             const float k = mn == -INFINITY ? 0.f : exp2f(m - mn);
             l *= k;
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= k;
             m = mn;
+            limit = mn == -INFINITY ? -INFINITY : (mn + 8.f) / scale2;
+            base = mn == -INFINITY ? 0.f : -mn;
         }
-    };
+    }
     // P^T as the B operand of the unit's two 16-key products, its sum into l
-    s8 p[2];
-    auto weights = [&](const f32x16& sc) {
-        const float base = m == -INFINITY ? 0.f : m;              // nothing seen yet: every p is 2^-inf = 0
+    __device__ __forceinline__ void weights(const f32x16& sc) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * kb + i], scale2, -base));
+            for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * kb + i], scale2, base));
             l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
             struct { unsigned u[4]; } w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) w.u[i] = Mma<T>::pack(e[2 * i], e[2 * i + 1]);
             p[kb] = __builtin_bit_cast(s8, w);
         }
-    };
+    }
     // O^T += V^T P^T over 32 keys.  AHEAD fragments are on their way from LDS at any time, the first ones asked for before the softmax
     // ends (as the compiler orders it alone, each product waits for its own read)
-    constexpr int FRAGS = 2 * DB, AHEAD = 4;
-    s8 vf[AHEAD];
-    auto v_frag = [&](const char* vt, int i) {
-        const char* at = vt + (i / DB) * 16 * ROWB + vrow;
-        const int db = i % DB;
-        const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + ((vs0 ^ (4 * db)) << 4)));
-        const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + 8 * ROWB + ((vs1 ^ (4 * db)) << 4)));
+    __device__ __forceinline__ s8 v_frag(const char* vt, int i) const {
+        const char* at = vt + (i / DB) * 16 * ROWB;
+        const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + vat[i % DB]));
+        const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(at + vat8[i % DB]));
         return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    auto values_ahead = [&](const char* vt) {
+    }
+    __device__ __forceinline__ void values_ahead(const char* vt) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) vf[i] = v_frag(vt, i);
         __builtin_amdgcn_sched_barrier(0);
-    };
-    auto values = [&](const char* vt) {
+    }
+    __device__ __forceinline__ void values(const char* vt) {
 #pragma unroll
         for (int i = 0; i < FRAGS; ++i) {
             o[i % DB] = Mma<T>::mul(vf[i % AHEAD], p[i / DB], o[i % DB]);
             if (i + AHEAD < FRAGS) vf[i % AHEAD] = v_frag(vt, i + AHEAD);
             __builtin_amdgcn_sched_barrier(0);
         }
-    };
-
-    Walker<KT> now;                                               // the tile that is worked on
-    now.go(first, np);
-    if constexpr (BYWAVE) {
-        auto one = [&](int buf) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // the other tile's reads are done
-            const bool more = now.tile + step < stages;
-            if (more) {
-                load_k(cv, buf ^ 1);
-                bring(cv, true, lds + (buf ^ 1) * TILE);
-                advance(cv, step);
-            }
-            f32x16 sc;
-            scores(buf, sc);
-            settle(now, 0, sc);
-            weights(sc);
-            if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES + DS) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            values_ahead(lds + buf * TILE);
-            values(lds + buf * TILE);
-            now.go(now.tile + step, np);
-        };
-        while (now.tile < stages) {
-            one(0);
-            if (now.tile < stages) one(1);
-        }
-    } else if (stages > 0) {
-        f32x16 sc, nx;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        // Q is there too: said to the compiler, which would otherwise wait for it (and for every request) in each turn of the loop
-#pragma unroll
-        for (int i = 0; i < DS; ++i) asm volatile("" : "+v"(q[i]));
-        __syncthreads();
-        if (busy) {
-            keys_ahead(lds);
-            scores(0, sc);
-        }
-        char *kt = lds, *kn = lds + TILE, *k2 = lds + 2 * TILE;   // K of this tile and the next two, V of this one and the next
-        char *vt = lds + 3 * TILE, *vn = lds + 4 * TILE;
-        for (int s = 0; s < stages; ++s) {
-            // K of s + 1 and V of s are in LDS, and every wave has left K and V of s - 1
-            if (s > 0) {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();
-            }
-            if (s + 2 < stages) {
-                bring(ck, false, k2);
-                advance(ck, 1);
-            }
-            if (s + 1 < stages) {
-                bring(cv, true, vn);
-                advance(cv, 1);
-            }
-            if (busy) {
-                keys_ahead(kt + 32 * ROWB);
-                settle(now, 0, sc);
-                scores(0, nx);
-                weights(sc);
-                values_ahead(vt);
-                values(vt);
-                keys_ahead(kn);
-                settle(now, 1, nx);
-                scores(0, sc);                                    // (the last tile: what lies there, not used)
-                weights(nx);
-                values_ahead(vt + 32 * ROWB);
-                values(vt + 32 * ROWB);
-            }
-            now.go(s + 1, np);
-            char* was = kt;
-            kt = kn;
-            kn = k2;
-            k2 = was;
-            was = vt;
-            vt = vn;
-            vn = was;
-        }
     }
-    l += __shfl_xor(l, 32, 64);
-
-    if constexpr (BYWAVE) {                                       // the waves join in a fixed order: 2 into 0 and 3 into 1, then 1 into 0
-        float* jo = reinterpret_cast<float*>(lds_all);            // [2][32 rows][DIM + 4], then [2][m | l][32]
-        float* jm = jo + 2 * 32 * (DIM + 4);
+    // results: lane (row l31) holds dims 32 d + 8 i + 4 hi + e
+    template <class I>
+    __device__ __forceinline__ void store(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, const I& it, int slots, int hi) const {
+        if (!it.row_ok) return;
+        const bool some = l > 0.f || l != l;                      // a NaN sum is a result, an empty row is not
+        const float inv = some ? 1.f / l : 0.f;
+        const float lse2 = some ? m + log2f(l) : -INFINITY;
+        const int64_t row = ((int64_t)it.row_b * a.queries + it.row_i) * a.heads + it.row_h;
+        if (slots == 1) {
+            T* out = static_cast<T*>(a.out) + row * DIM + 4 * hi;
 #pragma unroll
-        for (int half = 2; half > 0; half >>= 1) {
-            __syncthreads();                                      // the LDS is free
-            if (wave >= half && wave < 2 * half) {
-                float* to = jo + ((wave - half) * 32 + l31) * (DIM + 4) + 4 * hi;
+            for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
+                for (int i = 0; i < 4; ++i) {
+                    float v[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<f32x4*>(to + 32 * d + 8 * i) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-                if (hi == 0) {
-                    jm[(wave - half) * 64 + l31] = m;
-                    jm[(wave - half) * 64 + 32 + l31] = l;
+                    for (int e = 0; e < 4; ++e) v[e] = some ? o[d][4 * i + e] * inv : 0.f;
+                    store_vec<T, 4>(out + 32 * d + 8 * i, v);
                 }
+            if (a.lse && hi == 0) a.lse[((int64_t)it.row_b * a.heads + it.row_h) * a.queries + it.row_i] = lse2 * kLn2;
+        } else {
+            const int64_t rows = (int64_t)a.batch * a.queries * a.heads, at = (int64_t)(L.slot0 + it.chunk) * rows + row;
+            float* out = a.work + at * DIM + 4 * hi;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = some ? o[d][4 * i + e] * inv : 0.f;
+                    *reinterpret_cast<f32x4*>(out + 32 * d + 8 * i) = v;
+                }
+            if (hi == 0) (a.work + (int64_t)slots * rows * DIM)[at] = lse2;
+        }
+    }
+};
+
+// Many rows: wave w owns 32 of a block's 128; K and V come in 64-key tiles through LDS (LDS-DMA, a ring of three tiles of K and of two
+// of V).  A tile is two units of 32 keys; the scores of the next unit are multiplied while the softmax of this one runs, so the
+// matrix units work under the exponentials.  What bounds it is the waves' instruction issue (a wave issues one instruction in about
+// eight cycles, two waves share a SIMD), so the loop is unrolled over the rings' six states: LDS addresses are constants.
+template <class T, int DIM>
+__device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int slots, int block, int blocks, char* lds) {
+    constexpr int KT = 64, ROWB = DIM * 2, TILE = KT * ROWB;
+    constexpr int SLOTS = DIM / 8, RPP = 64 / SLOTS, PIECES = KT / RPP / 4;      // 16-byte slots of a key row; key rows of a 1-KiB piece; a wave's pieces
+    using I = Item<128, KT>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const I it(a, L, block, blocks, wave * 32, l31);
+    const bool busy = it.row0 < it.n_rows;                        // this wave has rows (it brings keys in any case)
+
+    // the lane's offsets within a tile of K and of V; they change where the walk enters the own keys
+    int key[PIECES], slot[PIECES], ko[PIECES], vo[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        key[i] = (wave * PIECES + i) * RPP + lane / SLOTS;
+        slot[i] = ((lane % SLOTS) ^ swz<DIM>(key[i])) * 16;
+    }
+    auto offsets = [&](int (&to)[PIECES], int stride) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) to[i] = key[i] * stride + slot[i];
+    };
+    Walk<I, DIM, KT> wk, wv;
+    wk.start(a, it, false, 0);
+    wv.start(a, it, true, 0);
+    offsets(ko, wk.stride);
+    offsets(vo, wv.stride);
+    const unsigned mine = lds_at(lds) + wave * PIECES * 1024;     // the wave's first piece of tile slot 0
+    auto bring_k = [&](auto at) {
+        const u4 d = wk.tile();
+        dma16<decltype(at)::value * TILE>(d, mine, ko[0]);
+        dma16<decltype(at)::value * TILE + 1024>(d, mine, ko[1]);
+        if constexpr (PIECES == 4) {
+            dma16<decltype(at)::value * TILE + 2048>(d, mine, ko[2]);
+            dma16<decltype(at)::value * TILE + 3072>(d, mine, ko[3]);
+        }
+        if (wk.step(a, it, false, 1)) offsets(ko, wk.stride);
+    };
+    auto bring_v = [&](auto at) {
+        const u4 d = wv.tile();
+        dma16<(3 + decltype(at)::value) * TILE>(d, mine, vo[0]);
+        dma16<(3 + decltype(at)::value) * TILE + 1024>(d, mine, vo[1]);
+        if constexpr (PIECES == 4) {
+            dma16<(3 + decltype(at)::value) * TILE + 2048>(d, mine, vo[2]);
+            dma16<(3 + decltype(at)::value) * TILE + 3072>(d, mine, vo[3]);
+        }
+        if (wv.step(a, it, true, 1)) offsets(vo, wv.stride);
+    };
+    static_assert(PIECES == 4 || PIECES == 2, "");
+    constexpr std::integral_constant<int, 0> C0{};
+    constexpr std::integral_constant<int, 1> C1{};
+    constexpr std::integral_constant<int, 2> C2{};
+
+    Rows32<T, DIM> w(a.scale, lane);
+    const int tiles = it.tiles;
+    if (tiles > 0) {
+        bring_k(C0);
+        bring_v(C0);
+        if (tiles > 1) bring_k(C1);
+    }
+    w.load_q(static_cast<const short*>(a.q) + it.row_b * a.q_bs + it.row_i * a.q_ss + it.row_h * a.q_hs + 8 * hi);
+    if (tiles > 0) {
+        // the tile that is worked on: keys from its first one to the segment's end, and those that every row of the wave sees
+        bool own = it.np == 0;
+        int left = own ? it.o1 - it.o0 : it.p1 - it.c0, clear = own ? (it.vis_low - it.o0 < left ? it.vis_low - it.o0 : left) : left;
+        int seen = own ? it.vis - it.o0 : left;                   // the lane's row sees these
+        auto hide = [&](f32x16& sc, int unit) {
+            if (__builtin_expect(clear < 32 * unit + 32, 0)) w.mask(sc, (seen < left ? seen : left) - 32 * unit, lane);
+        };
+        auto next_tile = [&]() {
+            left -= KT;
+            clear -= KT;
+            seen -= KT;
+            if (__builtin_expect(left <= 0 && !own, 0)) {
+                own = true;
+                left = it.o1 - it.o0;
+                clear = it.vis_low - it.o0 < left ? it.vis_low - it.o0 : left;
+                seen = it.vis - it.o0;
             }
-            __syncthreads();
-            if (wave < half) {
-                const float mo = jm[wave * 64 + l31], lo = jm[wave * 64 + 32 + l31], mt = fmaxf(m, mo), base = mt == -INFINITY ? 0.f : mt;
-                const float ka = exp2f(m - base), kb = exp2f(mo - base);
-                const float* from = jo + (wave * 32 + l31) * (DIM + 4) + 4 * hi;
+        };
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        w.q_is_there();       // said to the compiler, which would otherwise wait for Q (and for every request) in each turn of the loop
+        __syncthreads();
+        f32x16 sc, nx;
+        s8 kf[DIM / 16];
+        if (busy) {
+            w.keys(lds, kf);
+            w.scores(kf, sc);
+        }
+        int s = 0;
+        auto tile = [&](auto ks, auto vs) {
+            constexpr int KS = decltype(ks)::value, VS = decltype(vs)::value;
+            // K of s + 1 and V of s are in LDS, and every wave has left K and V of s - 1
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (__builtin_expect(s + 2 < tiles, 1)) bring_k(std::integral_constant<int, (KS + 2) % 3>{});
+            if (__builtin_expect(s + 1 < tiles, 1)) bring_v(std::integral_constant<int, (VS + 1) % 2>{});
+            if (__builtin_expect(busy, 1)) {
+                const char *kt = lds + KS * TILE, *kn = lds + (KS + 1) % 3 * TILE, *vt = lds + (3 + VS) * TILE;
+                w.keys(kt + 32 * ROWB, kf);
+                hide(sc, 0);
+                w.settle(sc);
+                w.scores(kf, nx);
+                w.weights(sc);
+                w.values_ahead(vt);
+                w.values(vt);
+                w.keys(kn, kf);
+                hide(nx, 1);
+                w.settle(nx);
+                w.scores(kf, sc);                                 // (behind the last tile: what lies there, not used)
+                w.weights(nx);
+                w.values_ahead(vt + 32 * ROWB);
+                w.values(vt + 32 * ROWB);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // this wave's reads are done when it meets the others
+            next_tile();
+            return ++s < tiles;
+        };
+        while (true) {
+            if (!tile(C0, C0)) break;
+            if (!tile(C1, C1)) break;
+            if (!tile(C2, C0)) break;
+            if (!tile(C0, C1)) break;
+            if (!tile(C1, C0)) break;
+            if (!tile(C2, C1)) break;
+        }
+    }
+    w.l += __shfl_xor(w.l, 32, 64);
+    w.store(a, L, it, slots, hi);
+}
+
+// Few rows (at most 32): a wave takes every fourth 32-key tile, its K straight into registers, its V through its own two LDS tiles; no
+// barrier until the four waves join at the end.  Bound by the keys' bytes.
+template <class T, int DIM>
+__device__ __forceinline__ void attend_wave(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int slots, int block, int blocks, char* lds_all) {
+    constexpr int KT = 32, ROWB = DIM * 2, TILE = KT * ROWB, DS = DIM / 16, DB = DIM / 32;
+    constexpr int SLOTS = DIM / 8, RPP = 64 / SLOTS, PIECES = KT / RPP;
+    using I = Item<32, KT>;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const I it(a, L, block, blocks, 0, l31);
+    char* lds = lds_all + wave * 2 * TILE;
+    const unsigned mine = lds_at(lds);
+
+    Walk<I, DIM, KT> wk, wv;                                      // the next tile to ask for
+    auto bring_v = [&](auto buf) {
+        const u4 d = wv.tile();
+        auto piece = [&](auto i) {
+            constexpr int P = decltype(i)::value;
+            if constexpr (P < PIECES) {
+                const int key = P * RPP + lane / SLOTS;
+                dma16<decltype(buf)::value * TILE + P * 1024>(d, mine, key * wv.stride + (((lane % SLOTS) ^ swz<DIM>(key)) << 4));
+            }
+        };
+        piece(std::integral_constant<int, 0>{});
+        piece(std::integral_constant<int, 1>{});
+        piece(std::integral_constant<int, 2>{});
+        piece(std::integral_constant<int, 3>{});
+        piece(std::integral_constant<int, 4>{});
+        piece(std::integral_constant<int, 5>{});
+        piece(std::integral_constant<int, 6>{});
+        piece(std::integral_constant<int, 7>{});
+        wv.step(a, it, true, 4);
+    };
+    static_assert(PIECES <= 8, "");
+    s8 kreg[2][DS];
+    auto load_k = [&](int buf) {
+        const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(wk.at), 0, ((wk.left < KT ? wk.left : KT) - 1) * wk.stride + ROWB, 0x00020000);
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
+        for (int s = 0; s < DS; ++s)
+            kreg[buf][s] = __builtin_bit_cast(s8, (u4)__builtin_amdgcn_raw_buffer_load_b128(d, l31 * wk.stride + 32 * s + 16 * hi, 0, 0));
+        wk.step(a, it, false, 4);
+    };
+    constexpr std::integral_constant<int, 0> C0{};
+    constexpr std::integral_constant<int, 1> C1{};
+    Rows32<T, DIM> w(a.scale, lane);
+    int s = wave;
+    if (s < it.tiles) {
+        wk.start(a, it, false, s);
+        wv.start(a, it, true, s);
+        load_k(0);
+        bring_v(C0);
+    }
+    w.load_q(static_cast<const short*>(a.q) + it.row_b * a.q_bs + it.row_i * a.q_ss + it.row_h * a.q_hs + 8 * hi);
+    auto one = [&](auto buf, auto other) {
+        constexpr int B = decltype(buf)::value;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the other tile's reads are done
+        const bool more = s + 4 < it.tiles;
+        if (more) {
+            load_k(B ^ 1);
+            bring_v(other);
+        }
+        f32x16 sc;
+        w.scores(kreg[B], sc);
+        const bool own = s >= it.np;
+        const int at = (own ? s - it.np : s) * KT, n = (own ? it.o1 - it.o0 : it.p1 - it.c0) - at;
+        if (n < KT || (own && it.o0 + at + KT > it.vis_low)) {
+            const int seen = own ? it.vis - it.o0 - at : n;
+            w.mask(sc, seen < n ? seen : n, lane);
+        }
+        w.settle(sc);
+        w.weights(sc);
+        // this tile's values have landed once only the next tile's requests are out: its pieces of V and its fragments of K
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES + DS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        w.values_ahead(lds + B * TILE);
+        w.values(lds + B * TILE);
+        s += 4;
+    };
+    while (s < it.tiles) {
+        one(C0, C1);
+        if (s < it.tiles) one(C1, C0);
+    }
+    w.l += __shfl_xor(w.l, 32, 64);
+
+    // the waves join in a fixed order: 2 into 0 and 3 into 1, then 1 into 0
+    float* jo = reinterpret_cast<float*>(lds_all);                // [2][32 rows][DIM + 4], then [2][m | l][32]
+    float* jm = jo + 2 * 32 * (DIM + 4);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 v = *reinterpret_cast<const f32x4*>(from + 32 * d + 8 * i);
+    for (int half = 2; half > 0; half >>= 1) {
+        __syncthreads();                                          // the LDS is free
+        if (wave >= half && wave < 2 * half) {
+            float* to = jo + ((wave - half) * 32 + l31) * (DIM + 4) + 4 * hi;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[d][4 * i + e] = ka * o[d][4 * i + e] + kb * v[e];
-                    }
-                l = ka * l + kb * lo;
-                m = mt;
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4*>(to + 32 * d + 8 * i) = f32x4{w.o[d][4 * i], w.o[d][4 * i + 1], w.o[d][4 * i + 2], w.o[d][4 * i + 3]};
+            if (hi == 0) {
+                jm[(wave - half) * 64 + l31] = w.m;
+                jm[(wave - half) * 64 + 32 + l31] = w.l;
             }
         }
-        if (wave != 0) return;
+        __syncthreads();
+        if (wave < half) {
+            const float mo = jm[wave * 64 + l31], lo = jm[wave * 64 + 32 + l31], mt = fmaxf(w.m, mo), base = mt == -INFINITY ? 0.f : mt;
+            const float ka = exp2f(w.m - base), kb = exp2f(mo - base);
+            const float* from = jo + (wave * 32 + l31) * (DIM + 4) + 4 * hi;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(from + 32 * d + 8 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w.o[d][4 * i + e] = ka * w.o[d][4 * i + e] + kb * v[e];
+                }
+            w.l = ka * w.l + kb * lo;
+            w.m = mt;
+        }
     }
-    // ---- results: lane (row l31) holds dims 32 d + 8 i + 4 hi + e ----
-    if (!row_ok) return;
-    const bool some = l > 0.f || l != l;                          // a NaN sum is a result, an empty row is not
-    const float inv = some ? 1.f / l : 0.f;
-    const float lse2 = some ? m + log2f(l) : -INFINITY;
-    const int64_t row = ((int64_t)row_b * a.queries + row_i) * a.heads + row_h;
-    if (slots == 1) {
-        T* out = static_cast<T*>(a.out) + row * DIM + 4 * hi;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = some ? o[d][4 * i + e] * inv : 0.f;
-                store_vec<T, 4>(out + 32 * d + 8 * i, v);
-            }
-        if (a.lse && hi == 0) a.lse[((int64_t)row_b * a.heads + row_h) * a.queries + row_i] = lse2 * kLn2;
-    } else {
-        const int64_t rows = (int64_t)a.batch * a.queries * a.heads, at = (int64_t)(L.slot0 + chunk) * rows + row;
-        float* out = a.work + at * DIM + 4 * hi;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = some ? o[d][4 * i + e] * inv : 0.f;
-                *reinterpret_cast<f32x4*>(out + 32 * d + 8 * i) = v;
-            }
-        if (hi == 0) (a.work + (int64_t)slots * rows * DIM)[at] = lse2;
-    }
+    if (wave == 0) w.store(a, L, it, slots, hi);
 }
 
 // The first `n0` blocks work on launch A, the others on B: the packed prefix and the own keys run beside each other.
@@ -473,14 +573,18 @@ __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const PrefixAt
                                                                   int slots) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int block = blockIdx.x;
-    if constexpr (WAVE_A == WAVE_B) {
+    if constexpr (WAVE_A && WAVE_B) {
         const bool second = block >= n0;
         const PrefixAttnLaunch L = second ? B : A;
-        attend<T, DIM, WAVE_A>(a, L, slots, second ? block - n0 : block, second ? (int)gridDim.x - n0 : n0, lds);
+        attend_wave<T, DIM>(a, L, slots, second ? block - n0 : block, second ? (int)gridDim.x - n0 : n0, lds);
+    } else if constexpr (!WAVE_A && !WAVE_B) {
+        const bool second = block >= n0;
+        const PrefixAttnLaunch L = second ? B : A;
+        attend_rows<T, DIM>(a, L, slots, second ? block - n0 : block, second ? (int)gridDim.x - n0 : n0, lds);
     } else if (block < n0) {
-        attend<T, DIM, WAVE_A>(a, A, slots, block, n0, lds);
+        attend_rows<T, DIM>(a, A, slots, block, n0, lds);
     } else {
-        attend<T, DIM, WAVE_B>(a, B, slots, block - n0, (int)gridDim.x - n0, lds);
+        attend_wave<T, DIM>(a, B, slots, block - n0, (int)gridDim.x - n0, lds);
     }
 }
 
