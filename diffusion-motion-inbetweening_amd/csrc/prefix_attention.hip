@@ -175,7 +175,8 @@ struct Rows32 {
     float scale2;
     int krow[DS], vat[DB], vat8[DB];      // LDS offsets of the lane's fragments within a 32-key unit
 
-    __device__ __forceinline__ Rows32(float scale, int lane) {
+    // `keys_at`: where the ring of K lies in LDS (in the offsets, so that every slot is within reach of an instruction's constant)
+    __device__ __forceinline__ Rows32(float scale, int lane, int keys_at) {
         const int l31 = lane & 31, hi = lane >> 5;
         m = -INFINITY;
         l = 0.f;
@@ -188,7 +189,7 @@ struct Rows32 {
             for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
         // K: key l31, dims 16 s + 8 hi ..
 #pragma unroll
-        for (int s = 0; s < DS; ++s) krow[s] = l31 * ROWB + (((2 * s + hi) ^ swz<DIM>(l31)) << 4);
+        for (int s = 0; s < DS; ++s) krow[s] = keys_at + l31 * ROWB + (((2 * s + hi) ^ swz<DIM>(l31)) << 4);
         // V, transposed reads: group G = lane / 16, lane L of it points at key 4 (G / 2) + L / 4, dims 16 (G % 2) + 4 (L % 4) .. + 3; the
         // group's lane i receives keys 4 (G / 2) .. + 3 of dim 16 (G % 2) + i
         const int key = 4 * hi + ((lane & 15) >> 2), slot = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), byte = key * ROWB + (lane & 1) * 8;
@@ -344,21 +345,21 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
     const unsigned mine = lds_at(lds) + wave * PIECES * 1024;     // the wave's first piece of tile slot 0
     auto bring_k = [&](auto at) {
         const u4 d = wk.tile();
-        dma16<decltype(at)::value * TILE>(d, mine, ko[0]);
-        dma16<decltype(at)::value * TILE + 1024>(d, mine, ko[1]);
+        dma16<(2 + decltype(at)::value) * TILE>(d, mine, ko[0]);
+        dma16<(2 + decltype(at)::value) * TILE + 1024>(d, mine, ko[1]);
         if constexpr (PIECES == 4) {
-            dma16<decltype(at)::value * TILE + 2048>(d, mine, ko[2]);
-            dma16<decltype(at)::value * TILE + 3072>(d, mine, ko[3]);
+            dma16<(2 + decltype(at)::value) * TILE + 2048>(d, mine, ko[2]);
+            dma16<(2 + decltype(at)::value) * TILE + 3 * 1024>(d, mine, ko[3]);
         }
         if (wk.step(a, it, false, 1)) offsets(ko, wk.stride);
     };
     auto bring_v = [&](auto at) {
         const u4 d = wv.tile();
-        dma16<(3 + decltype(at)::value) * TILE>(d, mine, vo[0]);
-        dma16<(3 + decltype(at)::value) * TILE + 1024>(d, mine, vo[1]);
+        dma16<decltype(at)::value * TILE>(d, mine, vo[0]);
+        dma16<decltype(at)::value * TILE + 1024>(d, mine, vo[1]);
         if constexpr (PIECES == 4) {
-            dma16<(3 + decltype(at)::value) * TILE + 2048>(d, mine, vo[2]);
-            dma16<(3 + decltype(at)::value) * TILE + 3072>(d, mine, vo[3]);
+            dma16<decltype(at)::value * TILE + 2048>(d, mine, vo[2]);
+            dma16<decltype(at)::value * TILE + 3 * 1024>(d, mine, vo[3]);
         }
         if (wv.step(a, it, true, 1)) offsets(vo, wv.stride);
     };
@@ -367,7 +368,7 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
     constexpr std::integral_constant<int, 1> C1{};
     constexpr std::integral_constant<int, 2> C2{};
 
-    Rows32<T, DIM> w(a.scale, lane);
+    Rows32<T, DIM> w(a.scale, lane, 2 * TILE);
     const int tiles = it.tiles;
     if (tiles > 0) {
         bring_k(C0);
@@ -412,7 +413,7 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
             if (__builtin_expect(s + 2 < tiles, 1)) bring_k(std::integral_constant<int, (KS + 2) % 3>{});
             if (__builtin_expect(s + 1 < tiles, 1)) bring_v(std::integral_constant<int, (VS + 1) % 2>{});
             if (__builtin_expect(busy, 1)) {
-                const char *kt = lds + KS * TILE, *kn = lds + (KS + 1) % 3 * TILE, *vt = lds + (3 + VS) * TILE;
+                const char *kt = lds + KS * TILE, *kn = lds + (KS + 1) % 3 * TILE, *vt = lds + VS * TILE;
                 w.keys(kt + 32 * ROWB, kf);
                 hide(sc, 0);
                 w.settle(sc);
@@ -489,7 +490,7 @@ __device__ __forceinline__ void attend_wave(const PrefixAttnArgs& a, const Prefi
     };
     constexpr std::integral_constant<int, 0> C0{};
     constexpr std::integral_constant<int, 1> C1{};
-    Rows32<T, DIM> w(a.scale, lane);
+    Rows32<T, DIM> w(a.scale, lane, 0);
     int s = wave;
     if (s < it.tiles) {
         wk.start(a, it, false, s);
