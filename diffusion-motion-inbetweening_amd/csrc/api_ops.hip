@@ -66,14 +66,6 @@ int norm_args(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_grads* g, Gat
             (a.g_b && !d->d_bias) || (a.g_wp && !d->d_post_weight) || (a.g_bp && !d->d_post_bias))
             return fail(CMDI_E_INVALID, "gradient wanted of a parameter that is not there");
     }
-    const int w = 16 / dt_bytes(d->dtype);
-    a.vec = d->dim % w == 0;
-    for (const void* p : rows) a.vec = a.vec && at16(p);
-    const Rows* all[] = {&a.x, &a.y, &a.gr, &a.gh};
-    for (const Rows* r : all) a.vec = a.vec && (!r->p || (r->bs % w == 0 && r->ss % w == 0));
-    a.pvec = a.vec;
-    for (const void* p : params) a.pvec = a.pvec && at16(p);
-    for (const NormParam* p : {&a.gate, &a.scale, &a.shift}) a.pvec = a.pvec && p->bs % w == 0;
     return CMDI_OK;
 }
 
@@ -158,7 +150,6 @@ int cmdi_gated_norm_fwd(const cmdi_gated_norm_desc* d, void* d_r, void* d_h, cmd
     if (!d_h) return fail(CMDI_E_INVALID, "null h");
     if (!at_elem(d_r, a.dtype) || !at_elem(d_h, a.dtype)) return fail(CMDI_E_INVALID, "an output is not aligned to its element");
     a.r = d_r; a.h = d_h;
-    if (!at16(d_r) || !at16(d_h)) a.vec = a.pvec = 0;
     gated_norm_plan(a, false);
     if (a.groups * a.chunks > kMaxBlocks) return fail(CMDI_E_INVALID, "too many samples");
     HIPCHK(launch_gated_norm_fwd(a, static_cast<hipStream_t>(stream)));
@@ -198,8 +189,7 @@ int cmdi_quant_rows_i8(const void* d_x, int32_t dtype, int64_t rows, int32_t col
     if (rows == 0) return CMDI_OK;
     if (!d_x || !d_q || !d_scale) return fail(CMDI_E_INVALID, "null tensor");
     if (!at16(d_q) || !at_elem(d_x, dtype) || !at_elem(d_scale, CMDI_DT_F32)) return fail(CMDI_E_INVALID, "q must be 16-byte aligned, x and scale to their elements");
-    const int w = 16 / dt_bytes(dtype);
-    QuantRowsArgs a{d_x, rows, ld, cols, dtype, cols % w == 0 && ld % w == 0 && at16(d_x), static_cast<int8_t*>(d_q), kp, d_scale};
+    QuantRowsArgs a{d_x, rows, ld, cols, dtype, static_cast<int8_t*>(d_q), kp, d_scale};
     HIPCHK(launch_quant_rows_i8(a, static_cast<hipStream_t>(stream)));
     return CMDI_OK;
 }

@@ -12,7 +12,8 @@
 //   A = sum dh,  N = sum dh n,  P = sum dr ny,  Q = sum dr:
 //   ds = w N + b A,  dt = A,  dg = wp P + bp Q,  dw = sum_b (1 + s) N,  db = sum_b (1 + s) A,  dwp = sum_b g P,  dbp = sum_b g Q,
 // because s, t, g are constant along a sample.  So the pass over the rows adds four numbers a column in registers, writes them
-// once per block, and two small kernels join them in a fixed order: no atomics, the same bits every run.
+// once per block, and two small kernels join them in a fixed order: no atomics, the same bits every run.  Where samples are many and
+// short, a team of lanes takes whole samples instead: it writes their gradients itself and carries only the sums over all samples.
 //
 // Bound by memory: forward reads x, y and writes r, h; backward reads x, y, dr', dh and writes dx, dy (r is computed again from
 // x and y, unrounded, which costs no more reads than r itself would).  A row stays in the registers of its team of lanes, so the
@@ -27,61 +28,49 @@
 namespace cmdi {
 namespace {
 
-// A team of TEAM lanes holds one row: element (c * TEAM + lane) * W + i, c < NV.  TEAM = 64: the row's sums never leave the wave;
-// wider teams are whole blocks and join their waves through LDS, one barrier a sum (two slots in turn).
+// A team of TEAM lanes holds a row: element (c * TEAM + lane) * W + i, c < NV.  TEAM = 64: the row's sums never leave the wave;
+// wider teams are whole blocks and join their waves through LDS, one barrier for all sums of a step (two slots in turn).
 template <int TEAM>
 struct TeamSum {
-    float* lds;      // [2][2][TEAM / 64]
+    static constexpr int NW = TEAM / 64, MOST = 4;
+    float* lds;      // [2][MOST][NW]
     int slot = 0;
     __device__ __forceinline__ explicit TeamSum(float* l) : lds(l) {}
-    __device__ __forceinline__ void two(float& a, float& b) {
-        a = wave_total(a);
-        b = wave_total(b);
+    template <int N>
+    __device__ __forceinline__ void all(float (&v)[N]) {
+        static_assert(N <= MOST, "");
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = wave_total(v[k]);
         if constexpr (TEAM > 64) {
-            constexpr int NW = TEAM / 64;
-            float* at = lds + slot * 2 * NW;
+            float* at = lds + slot * MOST * NW;
             slot ^= 1;
             if ((threadIdx.x & 63) == 0) {
-                at[threadIdx.x >> 6] = a;
-                at[NW + (threadIdx.x >> 6)] = b;
+#pragma unroll
+                for (int k = 0; k < N; ++k) at[k * NW + (threadIdx.x >> 6)] = v[k];
             }
             __syncthreads();
-            a = 0.f;
-            b = 0.f;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) { a += at[i]; b += at[NW + i]; }
-        }
-    }
-    __device__ __forceinline__ float one(float a) {
-        a = wave_total(a);
-        if constexpr (TEAM > 64) {
-            constexpr int NW = TEAM / 64;
-            float* at = lds + slot * 2 * NW;
-            slot ^= 1;
-            if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = a;
-            __syncthreads();
-            a = 0.f;
+            for (int k = 0; k < N; ++k) {
+                v[k] = 0.f;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) a += at[i];
+                for (int i = 0; i < NW; ++i) v[k] += at[k * NW + i];
+            }
         }
-        return a;
     }
 };
 
 template <int W, int NV>
 struct Row { float v[NV][W]; };
 
+#define FOR_ROW(c, i) _Pragma("unroll") for (int c = 0; c < NV; ++c) _Pragma("unroll") for (int i = 0; i < W; ++i)
+
+// columns behind `dim` read as 0
 template <class T, int W, int TEAM, int NV>
 __device__ __forceinline__ void load_row(Row<W, NV>& r, const T* p, int lane, int dim) {
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
         const int e = (c * TEAM + lane) * W;
-        if (e < dim) {
-            load_vec<T, W>(p + e, r.v[c]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) r.v[c][i] = 0.f;
-        }
+        load_part<T, W>(p + e, r.v[c], dim - e);
     }
 }
 template <class T, int W, int TEAM, int NV>
@@ -89,65 +78,43 @@ __device__ __forceinline__ void store_row(T* p, const Row<W, NV>& r, int lane, i
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
         const int e = (c * TEAM + lane) * W;
-        if (e < dim) store_vec<T, W>(p + e, r.v[c]);
+        store_part<T, W>(p + e, r.v[c], dim - e);
     }
 }
-// a parameter row, or `fill` where there is none (columns behind `dim` hold 0)
-template <class P, int W, int TEAM, int NV>
-__device__ __forceinline__ void load_param_as(Row<W, NV>& r, const P* p, int lane, int dim, bool vec) {
-#pragma unroll
-    for (int c = 0; c < NV; ++c) {
-        const int e = (c * TEAM + lane) * W;
-        if (vec && e < dim) {
-            load_vec<P, W>(p + e, r.v[c]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) r.v[c][i] = e + i < dim ? Elem<P>::up(p[e + i]) : 0.f;
-        }
-    }
-}
+// a parameter row, or `fill` where there is none (columns behind `dim` hold 0); the entries allow 32 bits or the rows' own type
 template <class T, int W, int TEAM, int NV>
 __device__ __forceinline__ void load_param(Row<W, NV>& r, const void* p, int64_t off, float fill, const GatedNormArgs& a, int lane) {
     if (!p) {
-#pragma unroll
-        for (int c = 0; c < NV; ++c)
-#pragma unroll
-            for (int i = 0; i < W; ++i) r.v[c][i] = (c * TEAM + lane) * W + i < a.dim ? fill : 0.f;
+        FOR_ROW(c, i) r.v[c][i] = (c * TEAM + lane) * W + i < a.dim ? fill : 0.f;
     } else if (a.param_dtype == CMDI_DT_F32) {
-        load_param_as<float, W, TEAM, NV>(r, static_cast<const float*>(p) + off, lane, a.dim, a.pvec);
-    } else {   // the entries allow 32 bits or the rows' own type
-        load_param_as<T, W, TEAM, NV>(r, static_cast<const T*>(p) + off, lane, a.dim, a.pvec);
+        load_row<float, W, TEAM, NV>(r, static_cast<const float*>(p) + off, lane, a.dim);
+    } else {
+        load_row<T, W, TEAM, NV>(r, static_cast<const T*>(p) + off, lane, a.dim);
     }
+}
+template <class T, int W, int TEAM, int NV>
+__device__ __forceinline__ void store_param(void* p, int64_t off, const Row<W, NV>& r, const GatedNormArgs& a, int lane) {
+    if (a.param_dtype == CMDI_DT_F32) store_row<float, W, TEAM, NV>(static_cast<float*>(p) + off, r, lane, a.dim);
+    else store_row<T, W, TEAM, NV>(static_cast<T*>(p) + off, r, lane, a.dim);
 }
 
 // v <- N(v), returns k = 1 / sqrt(mean + eps).  Columns behind `dim` stay 0.
 template <int W, int TEAM, int NV>
 __device__ __forceinline__ float normalise(Row<W, NV>& r, int kind, const GatedNormArgs& a, float inv_dim, int lane, TeamSum<TEAM>& sum) {
     if (kind == CMDI_NORM_NONE) return 1.f;
+    float v[1];
     if (kind == CMDI_NORM_LAYER) {
-        float s = 0.f;
-#pragma unroll
-        for (int c = 0; c < NV; ++c)
-#pragma unroll
-            for (int i = 0; i < W; ++i) s += r.v[c][i];
-        const float mean = sum.one(s) * inv_dim;
-#pragma unroll
-        for (int c = 0; c < NV; ++c)
-            if ((c * TEAM + lane) * W < a.dim) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) r.v[c][i] -= mean;
-            }
+        v[0] = 0.f;
+        FOR_ROW(c, i) v[0] += r.v[c][i];
+        sum.all(v);
+        const float mean = v[0] * inv_dim;
+        FOR_ROW(c, i) r.v[c][i] = (c * TEAM + lane) * W + i < a.dim ? r.v[c][i] - mean : 0.f;
     }
-    float q = 0.f;
-#pragma unroll
-    for (int c = 0; c < NV; ++c)
-#pragma unroll
-        for (int i = 0; i < W; ++i) q += r.v[c][i] * r.v[c][i];
-    const float k = 1.f / sqrtf(sum.one(q) * inv_dim + a.eps);
-#pragma unroll
-    for (int c = 0; c < NV; ++c)
-#pragma unroll
-        for (int i = 0; i < W; ++i) r.v[c][i] *= k;
+    v[0] = 0.f;
+    FOR_ROW(c, i) v[0] += r.v[c][i] * r.v[c][i];
+    sum.all(v);
+    const float k = 1.f / sqrtf(v[0] * inv_dim + a.eps);
+    FOR_ROW(c, i) r.v[c][i] *= k;
     return k;
 }
 
@@ -156,21 +123,30 @@ __device__ __forceinline__ int64_t row_at(const Rows& t, unsigned row, unsigned 
     const unsigned b = row / seq, s = row - b * seq;
     return (int64_t)b * t.bs + (int64_t)s * t.ss;
 }
+template <class T, int W, int TEAM, int NV>
+__device__ __forceinline__ void load_at(Row<W, NV>& r, const Rows& t, int64_t row, const GatedNormArgs& a, int lane) {
+    load_row<T, W, TEAM, NV>(r, static_cast<const T*>(t.p) + row_at(t, (unsigned)row, a.seq), lane, a.dim);
+}
 
-#define FOR_ROW(c, i) _Pragma("unroll") for (int c = 0; c < NV; ++c) _Pragma("unroll") for (int i = 0; i < W; ++i)
+// the rows of block `blockIdx.x`: a chunk of a group
+__device__ __forceinline__ void chunk_rows(const GatedNormArgs& a, int64_t& group, int64_t& chunk, int64_t& first, int64_t& end) {
+    group = blockIdx.x / (unsigned)a.chunks;
+    chunk = blockIdx.x % (unsigned)a.chunks;
+    first = group * a.rows_per_group + chunk * a.rows_per_chunk;
+    end = first + a.rows_per_chunk;
+    const int64_t total = (int64_t)a.batch * a.seq, stop = (group + 1) * a.rows_per_group;
+    if (end > stop) end = stop;
+    if (end > total) end = total;
+}
 
 template <class T, int W, int TEAM, int NV>
-__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void gated_norm_fwd_kernel(const GatedNormArgs a) {
-    constexpr int BLOCK = TEAM < 256 ? 256 : TEAM, TPB = BLOCK / TEAM;
-    __shared__ float lds[4 * (TEAM / 64)];
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void gated_norm_fwd_kernel(const GatedNormArgs a) {
+    constexpr int BLOCK = TEAM == 64 ? 256 : TEAM, TPB = BLOCK / TEAM;
+    __shared__ float lds[2 * TeamSum<TEAM>::MOST * (TEAM / 64)];
     TeamSum<TEAM> sum(lds);
     const int lane = threadIdx.x % TEAM, team = TPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
-    const int64_t group = blockIdx.x / (unsigned)a.chunks, chunk = blockIdx.x % (unsigned)a.chunks;
-    const int64_t total = (int64_t)a.batch * a.seq;
-    const int64_t first = group * a.rows_per_group + chunk * a.rows_per_chunk;
-    int64_t end = group * a.rows_per_group + (chunk + 1) * a.rows_per_chunk;
-    if (end > (group + 1) * a.rows_per_group) end = (group + 1) * a.rows_per_group;
-    if (end > total) end = total;
+    int64_t group, chunk, first, end;
+    chunk_rows(a, group, chunk, first, end);
     const float inv_dim = 1.f / (float)a.dim;
 
     Row<W, NV> g, wp, bp, w, t;
@@ -186,13 +162,11 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void gated_norm_fwd_kernel
     load_param<T, W, TEAM, NV>(g, a.shift.p, group * a.shift.bs, 0.f, a, lane);
     FOR_ROW(c, i) t.v[c][i] += g.v[c][i];
 
-    for (int64_t row0 = first; row0 < end; row0 += TPB) {
-        const int64_t row = row0 + team;
-        if (row >= end) break;                     // a whole wave (TEAM = 64) or never (TPB = 1)
+    for (int64_t row = first + team; row < end; row += TPB) {     // (TPB > 1: a team is a wave, nothing in here waits for another)
         Row<W, NV> x, y;
-        load_row<T, W, TEAM, NV>(x, static_cast<const T*>(a.x.p) + row_at(a.x, (unsigned)row, a.seq), lane, a.dim);
+        load_at<T, W, TEAM, NV>(x, a.x, row, a, lane);
         if (a.y.p) {
-            load_row<T, W, TEAM, NV>(y, static_cast<const T*>(a.y.p) + row_at(a.y, (unsigned)row, a.seq), lane, a.dim);
+            load_at<T, W, TEAM, NV>(y, a.y, row, a, lane);
             normalise<W, TEAM, NV>(y, a.post, a, inv_dim, lane, sum);
             FOR_ROW(c, i) x.v[c][i] = a.alpha * x.v[c][i] + (y.v[c][i] * wp.v[c][i] + bp.v[c][i]);
         } else {
@@ -205,128 +179,149 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void gated_norm_fwd_kernel
     }
 }
 
+// Column sums of the rows seen so far.
+template <int W, int NV>
+struct Sums {
+    Row<W, NV> A, N, P, Q;
+    __device__ __forceinline__ void clear() {
+        FOR_ROW(c, i) { A.v[c][i] = 0.f; N.v[c][i] = 0.f; P.v[c][i] = 0.f; Q.v[c][i] = 0.f; }
+    }
+};
+
+// One row backward: gx, gy written, its column sums added.  wp, bp: N_post's weight and bias times the gate; w: weight (1 + s).
 template <class T, int W, int TEAM, int NV>
-__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void gated_norm_vjp_kernel(const GatedNormArgs a) {
-    constexpr int BLOCK = TEAM < 256 ? 256 : TEAM, TPB = BLOCK / TEAM;
-    __shared__ float lds[4 * (TEAM / 64)];
+__device__ __forceinline__ void vjp_row(const GatedNormArgs& a, int64_t row, const Row<W, NV>& wp, const Row<W, NV>& bp, const Row<W, NV>& w, float inv_dim,
+                                        int lane, TeamSum<TEAM>& sum, Sums<W, NV>& s) {
+    Row<W, NV> x, y, d;
+    float ky = 1.f, m[2];
+    load_at<T, W, TEAM, NV>(x, a.x, row, a, lane);
+    if (a.gh.p) {
+        load_at<T, W, TEAM, NV>(d, a.gh, row, a, lane);
+    } else {
+        FOR_ROW(c, i) d.v[c][i] = 0.f;
+    }
+    if (a.y.p) {
+        load_at<T, W, TEAM, NV>(y, a.y, row, a, lane);
+        ky = normalise<W, TEAM, NV>(y, a.post, a, inv_dim, lane, sum);
+        FOR_ROW(c, i) x.v[c][i] = a.alpha * x.v[c][i] + (y.v[c][i] * wp.v[c][i] + bp.v[c][i]);
+    } else {
+        FOR_ROW(c, i) { y.v[c][i] = 0.f; x.v[c][i] *= a.alpha; }
+    }
+    const float kr = normalise<W, TEAM, NV>(x, a.pre, a, inv_dim, lane, sum);     // x = n
+    m[0] = m[1] = 0.f;
+    FOR_ROW(c, i) {
+        s.A.v[c][i] += d.v[c][i];
+        s.N.v[c][i] += d.v[c][i] * x.v[c][i];
+        d.v[c][i] *= w.v[c][i];                                                   // dn
+        m[0] += d.v[c][i];
+        m[1] += d.v[c][i] * x.v[c][i];
+    }
+    sum.all(m);
+    float m1 = a.pre == CMDI_NORM_LAYER ? m[0] * inv_dim : 0.f, m2 = m[1] * inv_dim;
+    FOR_ROW(c, i) d.v[c][i] = kr * (d.v[c][i] - x.v[c][i] * m2 - m1);
+    if (a.gr.p) {
+        load_at<T, W, TEAM, NV>(x, a.gr, row, a, lane);
+        FOR_ROW(c, i) d.v[c][i] += x.v[c][i];                                     // dr
+    }
+    if (a.gx) {
+        FOR_ROW(c, i) x.v[c][i] = a.alpha * d.v[c][i];
+        store_row<T, W, TEAM, NV>(static_cast<T*>(a.gx) + row * a.dim, x, lane, a.dim);
+    }
+    if (!a.y.p) return;
+    m[0] = m[1] = 0.f;
+    FOR_ROW(c, i) {
+        // columns behind `dim` hold -kr m1 in d; their weights are 0 and their sums never written
+        s.P.v[c][i] += d.v[c][i] * y.v[c][i];
+        s.Q.v[c][i] += d.v[c][i];
+        d.v[c][i] *= wp.v[c][i];
+        m[0] += d.v[c][i];
+        m[1] += d.v[c][i] * y.v[c][i];
+    }
+    if (!a.gy) return;
+    if (a.post != CMDI_NORM_NONE) {
+        sum.all(m);
+        m1 = a.post == CMDI_NORM_LAYER ? m[0] * inv_dim : 0.f;
+        m2 = m[1] * inv_dim;
+        FOR_ROW(c, i) d.v[c][i] = ky * (d.v[c][i] - y.v[c][i] * m2 - m1);
+    }
+    store_row<T, W, TEAM, NV>(static_cast<T*>(a.gy) + row * a.dim, d, lane, a.dim);
+}
+
+// SPAN: a team takes a.rows_per_chunk whole samples one after the other; otherwise a block a chunk of one group's rows.
+template <class T, int W, int TEAM, int NV, bool SPAN>
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void gated_norm_vjp_kernel(const GatedNormArgs a) {
+    constexpr int BLOCK = TEAM == 64 ? 256 : TEAM, TPB = BLOCK / TEAM;
+    __shared__ float lds[2 * TeamSum<TEAM>::MOST * (TEAM / 64)];
     __shared__ float joined[TPB > 1 ? TEAM * NV * W : 1];
     TeamSum<TEAM> sum(lds);
     const int lane = threadIdx.x % TEAM, team = TPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
-    const int64_t group = blockIdx.x / (unsigned)a.chunks, chunk = blockIdx.x % (unsigned)a.chunks;
-    const int64_t total = (int64_t)a.batch * a.seq;
-    const int64_t first = group * a.rows_per_group + chunk * a.rows_per_chunk;
-    int64_t end = group * a.rows_per_group + (chunk + 1) * a.rows_per_chunk;
-    if (end > (group + 1) * a.rows_per_group) end = (group + 1) * a.rows_per_group;
-    if (end > total) end = total;
     const float inv_dim = 1.f / (float)a.dim;
-
-    Row<W, NV> g, wp, bp, w;     // gate, N_post's weight and bias, w (1 + s)
-    load_param<T, W, TEAM, NV>(w, a.w, 0, 1.f, a, lane);
-    load_param<T, W, TEAM, NV>(g, a.scale.p, group * a.scale.bs, 0.f, a, lane);
-    FOR_ROW(c, i) w.v[c][i] *= 1.f + g.v[c][i];
-    load_param<T, W, TEAM, NV>(g, a.gate.p, group * a.gate.bs, 1.f, a, lane);
-    load_param<T, W, TEAM, NV>(wp, a.wp, 0, 1.f, a, lane);
-    load_param<T, W, TEAM, NV>(bp, a.bp, 0, 0.f, a, lane);
-
-    Row<W, NV> sA, sN, sP, sQ;
-    FOR_ROW(c, i) { sA.v[c][i] = 0.f; sN.v[c][i] = 0.f; sP.v[c][i] = 0.f; sQ.v[c][i] = 0.f; }
-
-    for (int64_t row0 = first; row0 < end; row0 += TPB) {
-        const int64_t row = row0 + team;
-        if (row >= end) break;
-        Row<W, NV> x, y, d;
-        float ky = 1.f;
-        load_row<T, W, TEAM, NV>(x, static_cast<const T*>(a.x.p) + row_at(a.x, (unsigned)row, a.seq), lane, a.dim);
-        if (a.gh.p) {
-            load_row<T, W, TEAM, NV>(d, static_cast<const T*>(a.gh.p) + row_at(a.gh, (unsigned)row, a.seq), lane, a.dim);
-        } else {
-            FOR_ROW(c, i) d.v[c][i] = 0.f;
-        }
-        if (a.y.p) {
-            load_row<T, W, TEAM, NV>(y, static_cast<const T*>(a.y.p) + row_at(a.y, (unsigned)row, a.seq), lane, a.dim);
-            ky = normalise<W, TEAM, NV>(y, a.post, a, inv_dim, lane, sum);
-            FOR_ROW(c, i) x.v[c][i] = a.alpha * x.v[c][i] + (y.v[c][i] * wp.v[c][i] + bp.v[c][i]) * g.v[c][i];
-        } else {
-            FOR_ROW(c, i) { y.v[c][i] = 0.f; x.v[c][i] *= a.alpha; }
-        }
-        const float kr = normalise<W, TEAM, NV>(x, a.pre, a, inv_dim, lane, sum);     // x = n
-        float m1 = 0.f, m2 = 0.f;
-        FOR_ROW(c, i) {
-            sA.v[c][i] += d.v[c][i];
-            sN.v[c][i] += d.v[c][i] * x.v[c][i];
-            d.v[c][i] *= w.v[c][i];                                                   // dn
-            m1 += d.v[c][i];
-            m2 += d.v[c][i] * x.v[c][i];
-        }
-        sum.two(m1, m2);
-        m1 = a.pre == CMDI_NORM_LAYER ? m1 * inv_dim : 0.f;
-        m2 *= inv_dim;
-        FOR_ROW(c, i) d.v[c][i] = kr * (d.v[c][i] - x.v[c][i] * m2 - m1);
-        if (a.gr.p) {
-            load_row<T, W, TEAM, NV>(x, static_cast<const T*>(a.gr.p) + row_at(a.gr, (unsigned)row, a.seq), lane, a.dim);
-            FOR_ROW(c, i) d.v[c][i] += x.v[c][i];                                     // dr
-        }
-        if (a.gx) {
-            FOR_ROW(c, i) x.v[c][i] = a.alpha * d.v[c][i];
-            store_row<T, W, TEAM, NV>(static_cast<T*>(a.gx) + row * a.dim, x, lane, a.dim);
-        }
-        if (a.y.p) {
-            m1 = 0.f;
-            m2 = 0.f;
-            FOR_ROW(c, i) {
-                // columns behind `dim` (only the last chunk has them) hold -kr m1 in d; their weights are 0
-                sP.v[c][i] += d.v[c][i] * y.v[c][i];
-                sQ.v[c][i] += d.v[c][i];
-                d.v[c][i] *= g.v[c][i] * wp.v[c][i];
-                m1 += d.v[c][i];
-                m2 += d.v[c][i] * y.v[c][i];
+    Row<W, NV> wp, bp, w;
+    auto params = [&](int64_t sample) {
+        Row<W, NV> g;
+        load_param<T, W, TEAM, NV>(w, a.w, 0, 1.f, a, lane);
+        load_param<T, W, TEAM, NV>(g, a.scale.p, sample * a.scale.bs, 0.f, a, lane);
+        FOR_ROW(c, i) w.v[c][i] *= 1.f + g.v[c][i];
+        load_param<T, W, TEAM, NV>(g, a.gate.p, sample * a.gate.bs, 1.f, a, lane);
+        load_param<T, W, TEAM, NV>(wp, a.wp, 0, 1.f, a, lane);
+        load_param<T, W, TEAM, NV>(bp, a.bp, 0, 0.f, a, lane);
+        FOR_ROW(c, i) { wp.v[c][i] *= g.v[c][i]; bp.v[c][i] *= g.v[c][i]; }
+    };
+    Sums<W, NV> s;
+    s.clear();
+    if constexpr (SPAN) {
+        Sums<W, NV> own;
+        const int64_t s0 = ((int64_t)blockIdx.x * TPB + team) * a.rows_per_chunk;
+        const int64_t s1 = s0 + a.rows_per_chunk < a.batch ? s0 + a.rows_per_chunk : a.batch;
+        for (int64_t b = s0; b < s1; ++b) {
+            params(b);
+            own.clear();
+            for (int i = 0; i < a.seq; ++i) vjp_row<T, W, TEAM, NV>(a, b * a.seq + i, wp, bp, w, inv_dim, lane, sum, own);
+            // ds = w N + b A, dt = A, dg = wp P + bp Q; the other parameters' sums take (1 + s) or g along
+            Row<W, NV> u, v;
+            load_param<T, W, TEAM, NV>(u, a.scale.p, b * a.scale.bs, 0.f, a, lane);
+            FOR_ROW(c, i) { s.A.v[c][i] += (1.f + u.v[c][i]) * own.A.v[c][i]; s.N.v[c][i] += (1.f + u.v[c][i]) * own.N.v[c][i]; }
+            load_param<T, W, TEAM, NV>(u, a.gate.p, b * a.gate.bs, 1.f, a, lane);
+            FOR_ROW(c, i) { s.P.v[c][i] += u.v[c][i] * own.P.v[c][i]; s.Q.v[c][i] += u.v[c][i] * own.Q.v[c][i]; }
+            if (a.g_shift) store_param<T, W, TEAM, NV>(a.g_shift, b * a.dim, own.A, a, lane);
+            if (a.g_scale) {
+                load_param<T, W, TEAM, NV>(u, a.w, 0, 1.f, a, lane);
+                load_param<T, W, TEAM, NV>(v, a.b, 0, 0.f, a, lane);
+                FOR_ROW(c, i) u.v[c][i] = u.v[c][i] * own.N.v[c][i] + v.v[c][i] * own.A.v[c][i];
+                store_param<T, W, TEAM, NV>(a.g_scale, b * a.dim, u, a, lane);
             }
-            if (a.gy) {
-                if (a.post != CMDI_NORM_NONE) {
-                    sum.two(m1, m2);
-                    m1 = a.post == CMDI_NORM_LAYER ? m1 * inv_dim : 0.f;
-                    m2 *= inv_dim;
-                    FOR_ROW(c, i) d.v[c][i] = ky * (d.v[c][i] - y.v[c][i] * m2 - m1);
-                }
-                store_row<T, W, TEAM, NV>(static_cast<T*>(a.gy) + row * a.dim, d, lane, a.dim);
+            if (a.g_gate) {
+                load_param<T, W, TEAM, NV>(u, a.wp, 0, 1.f, a, lane);
+                load_param<T, W, TEAM, NV>(v, a.bp, 0, 0.f, a, lane);
+                FOR_ROW(c, i) u.v[c][i] = u.v[c][i] * own.P.v[c][i] + v.v[c][i] * own.Q.v[c][i];
+                store_param<T, W, TEAM, NV>(a.g_gate, b * a.dim, u, a, lane);
             }
         }
+    } else {
+        int64_t group, chunk, first, end;
+        chunk_rows(a, group, chunk, first, end);
+        params(group);
+        for (int64_t row = first + team; row < end; row += TPB) vjp_row<T, W, TEAM, NV>(a, row, wp, bp, w, inv_dim, lane, sum, s);
     }
     // the block's column sums: teams add in order, one sum after another, then one write
-    float* out = a.work + (group * a.chunks + chunk) * (int64_t)__builtin_popcount(a.slots) * a.dim;
+    float* out = a.work + (int64_t)blockIdx.x * __builtin_popcount(a.slots) * a.dim;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if (!(a.slots >> k & 1)) continue;
-        Row<W, NV>& s = k == 0 ? sA : k == 1 ? sN : k == 2 ? sP : sQ;
+        Row<W, NV>& r = k == 0 ? s.A : k == 1 ? s.N : k == 2 ? s.P : s.Q;
         if constexpr (TPB > 1) {
             for (int tm = 0; tm < TPB; ++tm) {
                 __syncthreads();
                 if (team == tm) {
                     FOR_ROW(c, i) {
                         float& at = joined[(c * W + i) * TEAM + lane];
-                        s.v[c][i] += tm ? at : 0.f;
-                        at = s.v[c][i];
+                        r.v[c][i] += tm ? at : 0.f;
+                        at = r.v[c][i];
                     }
                 }
             }
-            if (team == TPB - 1) {
-#pragma unroll
-                for (int c = 0; c < NV; ++c) {
-                    const int e = (c * TEAM + lane) * W;
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-                        if (e + i < a.dim) out[e + i] = s.v[c][i];
-                }
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < NV; ++c) {
-                const int e = (c * TEAM + lane) * W;
-#pragma unroll
-                for (int i = 0; i < W; ++i)
-                    if (e + i < a.dim) out[e + i] = s.v[c][i];
-            }
         }
+        if (team == TPB - 1) store_row<float, W, TEAM, NV>(out, r, lane, a.dim);
         out += a.dim;
     }
 }
@@ -406,8 +401,8 @@ __global__ __launch_bounds__(JOIN_COLS * JOIN_SLICES) void gated_norm_join_all_k
                 v[k] = 0.f;
                 if (a.slots >> k & 1) { v[k] = *p; p += a.dim; }
             }
-            const float s1 = 1.f + param_at(a.scale.p, gi * a.scale.bs + col, 0.f, pd);
-            const float gg = param_at(a.gate.p, gi * a.gate.bs + col, 1.f, pd);
+            const float s1 = a.span ? 1.f : 1.f + param_at(a.scale.p, gi * a.scale.bs + col, 0.f, pd);
+            const float gg = a.span ? 1.f : param_at(a.gate.p, gi * a.gate.bs + col, 1.f, pd);   // (span: taken along already)
 #pragma unroll
             for (int k = 0; k < 4; ++k) { tot[k] += v[k]; tot[4 + k] += (k < 2 ? s1 : gg) * v[k]; }
         }
@@ -434,25 +429,34 @@ __global__ __launch_bounds__(JOIN_COLS * JOIN_SLICES) void gated_norm_join_all_k
 bool per_sample(const GatedNormArgs& a) {
     return (a.gate.p && a.gate.bs) || (a.scale.p && a.scale.bs) || (a.shift.p && a.shift.bs);
 }
-int teams_per_block(int dim) { return dim <= 1024 ? 4 : 1; }
+int teams_per_block(int dim, bool vjp) { return dim <= (vjp ? 512 : 1024) ? 4 : 1; }
 
-// Width of the team by the row's length: 8 or 16 elements a lane (a lane's registers hold the row, the parameters and, backward,
-// four column sums of each of its columns).
-template <class T, int W, class F>
+// Width of the team by the row's length.  Forward 8 or 16 elements a lane; backward, where a lane's registers also hold four column
+// sums of each of its columns, 8 as long as a block can be that wide.
+template <bool VJP, int W, class F>
 hipError_t by_width(int dim, F&& f) {
     if (dim <= 512) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 8 / W>());
-    if (dim <= 1024) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 16 / W>());
+    if constexpr (VJP) {
+        if (dim <= 1024) return f(std::integral_constant<int, 128>(), std::integral_constant<int, 8 / W>());
+    } else {
+        if (dim <= 1024) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 16 / W>());
+    }
     if (dim <= 2048) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 8 / W>());
-    if (dim <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 16 / W>());
-    if (dim <= 8192) return f(std::integral_constant<int, 512>(), std::integral_constant<int, 16 / W>());
+    if constexpr (VJP) {
+        if (dim <= 4096) return f(std::integral_constant<int, 512>(), std::integral_constant<int, 8 / W>());
+        if (dim <= 8192) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 8 / W>());
+    } else {
+        if (dim <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 16 / W>());
+        if (dim <= 8192) return f(std::integral_constant<int, 512>(), std::integral_constant<int, 16 / W>());
+    }
     return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 16 / W>());
 }
 template <class F>
 hipError_t by_type(const GatedNormArgs& a, F&& f) {
     switch (a.dtype) {
-        case CMDI_DT_F32: return a.vec ? f(float(), std::integral_constant<int, 4>()) : f(float(), std::integral_constant<int, 1>());
-        case CMDI_DT_BF16: return a.vec ? f(Bf16(), std::integral_constant<int, 8>()) : f(Bf16(), std::integral_constant<int, 1>());
-        default: return a.vec ? f(_Float16(), std::integral_constant<int, 8>()) : f(_Float16(), std::integral_constant<int, 1>());
+        case CMDI_DT_F32: return f(float());
+        case CMDI_DT_BF16: return f(Bf16());
+        default: return f(_Float16());
     }
 }
 
@@ -460,32 +464,51 @@ hipError_t by_type(const GatedNormArgs& a, F&& f) {
 
 void gated_norm_plan(GatedNormArgs& a, bool vjp) {
     const int64_t total = (int64_t)a.batch * a.seq;
-    const int tpb = teams_per_block(a.dim);
-    // blocks that keep the chip busy; a block's rows share its parameter registers and, backward, its column sums
-    const int64_t want = 2048;
-    if (per_sample(a)) {
-        a.groups = a.batch;
-        a.rows_per_group = a.seq;
-    } else {
-        // no sample of its own anywhere: cut the rows into pieces so that the joins run beside each other
-        a.groups = vjp ? (total + 31) / 32 : 1;
-        if (a.groups > 32) a.groups = 32;
-        if (a.groups < 1) a.groups = 1;
-        a.rows_per_group = (total + a.groups - 1) / a.groups;
-        if (a.rows_per_group < 1) a.rows_per_group = 1;
-        a.groups = (total + a.rows_per_group - 1) / a.rows_per_group;
-        if (a.groups < 1) a.groups = 1;
+    const int tpb = teams_per_block(a.dim, vjp);
+    // blocks that keep the chip busy; a block's rows share its parameter registers and, backward, its column sums (whose partial
+    // results the joins read back: fewer, longer blocks there)
+    const int64_t want = vjp ? 1024 : 2048;
+    const bool own = per_sample(a);
+    a.slots = 0;
+    a.span = vjp && own && a.batch >= 256 && a.seq <= 32 && (!a.gate.p || a.gate.bs) && (!a.scale.p || a.scale.bs) && (!a.shift.p || a.shift.bs);
+    if (a.span) {
+        // many short samples (4096 of one row, width 2048: 959 us with the joins below, see there): teams take whole ones
+        const int64_t teams = want * tpb;
+        a.rows_per_chunk = (a.batch + teams - 1) / teams;
+        a.groups = ((a.batch + a.rows_per_chunk - 1) / a.rows_per_chunk + tpb - 1) / tpb;
+        a.chunks = 1;
+        a.rows_per_group = 0;
+        a.slots = (a.g_b ? 1 : 0) | (a.g_w ? 2 : 0) | (a.g_wp ? 4 : 0) | (a.g_bp ? 8 : 0);
+        return;
     }
-    int64_t chunks = (want + a.groups - 1) / a.groups;
-    const int64_t most = (a.rows_per_group + tpb - 1) / tpb;
+    const int64_t span = own ? a.seq : total, spans = own ? a.batch : 1;
+    int64_t chunks = (want + spans - 1) / spans;
+    const int64_t most = (span + tpb - 1) / tpb;
     if (chunks > most) chunks = most;
     if (chunks < 1) chunks = 1;
-    int64_t rows = (a.rows_per_group + chunks - 1) / chunks;
+    int64_t rows = (span + chunks - 1) / chunks;
     rows = (rows + tpb - 1) / tpb * tpb;
-    a.rows_per_chunk = rows;
-    a.chunks = (a.rows_per_group + rows - 1) / rows;
-    if (a.chunks < 1) a.chunks = 1;
-    a.slots = 0;
+    chunks = (span + rows - 1) / rows;
+    if (chunks < 1) chunks = 1;
+    a.rows_per_chunk = rows < 1 ? 1 : rows;
+    if (own) {
+        a.groups = a.batch;
+        a.chunks = chunks;
+        a.rows_per_group = a.seq;
+    } else if (vjp && chunks > 256) {
+        // no sample of its own anywhere: 32 groups of chunks whose joins run beside each other, then one of the groups
+        a.chunks = (chunks + 31) / 32;
+        a.groups = (chunks + a.chunks - 1) / a.chunks;
+        a.rows_per_group = a.chunks * a.rows_per_chunk;
+    } else if (vjp) {
+        a.chunks = 1;            // few chunks: the last join takes them all
+        a.groups = chunks;
+        a.rows_per_group = a.rows_per_chunk;
+    } else {
+        a.chunks = chunks;
+        a.groups = 1;
+        a.rows_per_group = total;
+    }
     if (a.g_shift || a.g_b || (a.g_scale && a.b)) a.slots |= 1;
     if (a.g_scale || a.g_w) a.slots |= 2;
     if (a.g_gate || a.g_wp) a.slots |= 4;
@@ -497,34 +520,38 @@ int64_t gated_norm_work_floats(const GatedNormArgs& a) {
 }
 
 hipError_t launch_gated_norm_fwd(const GatedNormArgs& a, hipStream_t stream) {
-    return by_type(a, [&](auto t, auto w) {
+    return by_type(a, [&](auto t) {
         using T = decltype(t);
-        constexpr int W = decltype(w)::value;
-        return by_width<T, W>(a.dim, [&](auto team, auto nv) {
+        constexpr int W = Elem<T>::W;
+        return by_width<false, W>(a.dim, [&](auto team, auto nv) {
             constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
-            gated_norm_fwd_kernel<T, W, TEAM, NV><<<dim3((unsigned)(a.groups * a.chunks)), dim3(TEAM < 256 ? 256 : TEAM), 0, stream>>>(a);
+            gated_norm_fwd_kernel<T, W, TEAM, NV><<<dim3((unsigned)(a.groups * a.chunks)), dim3(TEAM == 64 ? 256 : TEAM), 0, stream>>>(a);
             return hipGetLastError();
         });
     });
 }
 
 hipError_t launch_gated_norm_vjp(const GatedNormArgs& a, hipStream_t stream) {
-    hipError_t err = by_type(a, [&](auto t, auto w) {
+    hipError_t err = by_type(a, [&](auto t) {
         using T = decltype(t);
-        constexpr int W = decltype(w)::value;
-        return by_width<T, W>(a.dim, [&](auto team, auto nv) {
+        constexpr int W = Elem<T>::W;
+        return by_width<true, W>(a.dim, [&](auto team, auto nv) {
             constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
-            gated_norm_vjp_kernel<T, W, TEAM, NV><<<dim3((unsigned)(a.groups * a.chunks)), dim3(TEAM < 256 ? 256 : TEAM), 0, stream>>>(a);
+            const dim3 grid((unsigned)(a.groups * a.chunks)), block(TEAM == 64 ? 256 : TEAM);
+            if (a.span) gated_norm_vjp_kernel<T, W, TEAM, NV, true><<<grid, block, 0, stream>>>(a);
+            else gated_norm_vjp_kernel<T, W, TEAM, NV, false><<<grid, block, 0, stream>>>(a);
             return hipGetLastError();
         });
     });
     if (err != hipSuccess || !a.slots) return err;
-    const bool own = (a.g_scale && a.scale.bs) || (a.g_shift && a.shift.bs) || (a.g_gate && a.gate.bs);
+    const bool own = !a.span && ((a.g_scale && a.scale.bs) || (a.g_shift && a.shift.bs) || (a.g_gate && a.gate.bs));
     const bool all = a.g_w || a.g_b || a.g_wp || a.g_bp || (a.g_scale && !a.scale.bs) || (a.g_shift && !a.shift.bs) || (a.g_gate && !a.gate.bs);
     const unsigned cols = (unsigned)((a.dim + JOIN_COLS - 1) / JOIN_COLS);
-    gated_norm_join_kernel<<<dim3(cols * (unsigned)a.groups), dim3(JOIN_COLS * JOIN_SLICES), 0, stream>>>(a, own, all);
-    err = hipGetLastError();
-    if (err != hipSuccess || !all) return err;
+    if (own || a.chunks > 1) {
+        gated_norm_join_kernel<<<dim3(cols * (unsigned)a.groups), dim3(JOIN_COLS * JOIN_SLICES), 0, stream>>>(a, own, all);
+        err = hipGetLastError();
+        if (err != hipSuccess || !all) return err;
+    }
     gated_norm_join_all_kernel<<<dim3(cols), dim3(JOIN_COLS * JOIN_SLICES), 0, stream>>>(a);
     return hipGetLastError();
 }

@@ -25,11 +25,10 @@ struct GatedNormArgs {
     void *gx, *gy;                           // vjp: contiguous outputs, either may be null
     void *g_gate, *g_scale, *g_shift, *g_w, *g_b, *g_wp, *g_bp;
     float* work;                             // vjp: partial column sums
-    int32_t vec;                             // rows and outputs allow 16-byte accesses
-    int32_t pvec;                            // parameters allow them too
     // split of the rows (gated_norm_plan)
     int64_t groups, rows_per_group, chunks, rows_per_chunk;
-    int32_t slots;                           // column sums kept: bit 0 sum dh, 1 sum dh n, 2 sum dr ny, 3 sum dr
+    int32_t span;                            // vjp: teams take whole samples (many short ones); rows_per_chunk = samples a team
+    int32_t slots;                           // column sums kept: bit 0 sum dh, 1 sum dh n, 2 sum dr ny, 3 sum dr (span: times 1 + s, g)
 };
 
 constexpr int kGatedNormMaxDim = 16384;

@@ -21,9 +21,10 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 // ---- quantise ------------------------------------------------------------------------------------------------------------
 // A team of TEAM lanes takes a row; its first NV vectors of a lane stay in registers between the two passes, the rest of a
 // longer row is read again (from the L2).  Bound by memory: 2 or 4 bytes read, 1 written.
-template <class T, int W, int TEAM>
+template <class T, int TEAM>
 __global__ __launch_bounds__(256) void quant_rows_i8_kernel(const QuantRowsArgs a) {
-    constexpr int NV = W == 1 ? 8 : 4, TPB = 256 / TEAM;
+    constexpr int W = Elem<T>::W;
+    constexpr int NV = 4, TPB = 256 / TEAM;
     __shared__ float lds[2][4];
     const int lane = threadIdx.x % TEAM;
     const int team = TPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
@@ -35,12 +36,7 @@ __global__ __launch_bounds__(256) void quant_rows_i8_kernel(const QuantRowsArgs 
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
         const int e = (c * TEAM + lane) * W;
-        if (e < a.cols) {
-            load_vec<T, W>(x + e, v[c]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[c][i] = 0.f;
-        }
+        load_part<T, W>(x + e, v[c], a.cols - e);
     }
 #pragma unroll
     for (int c = 0; c < NV; ++c)
@@ -48,7 +44,7 @@ __global__ __launch_bounds__(256) void quant_rows_i8_kernel(const QuantRowsArgs 
         for (int i = 0; i < W; ++i) { top = fmaxf(top, fabsf(v[c][i])); odd += 0.f * v[c][i]; }
     for (int e = (NV * TEAM + lane) * W; e < a.cols; e += TEAM * W) {
         float u[W];
-        load_vec<T, W>(x + e, u);
+        load_part<T, W>(x + e, u, a.cols - e);
 #pragma unroll
         for (int i = 0; i < W; ++i) { top = fmaxf(top, fabsf(u[i])); odd += 0.f * u[i]; }
     }
@@ -79,9 +75,7 @@ __global__ __launch_bounds__(256) void quant_rows_i8_kernel(const QuantRowsArgs 
     }
     for (int e = (NV * TEAM + lane) * W; e < a.kp; e += TEAM * W) {
         float u[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) u[i] = 0.f;
-        if (e < a.cols) load_vec<T, W>(x + e, u);
+        load_part<T, W>(x + e, u, a.cols - e);
         Out o;
 #pragma unroll
         for (int i = 0; i < W; ++i) o.e[i] = (int8_t)(fine ? (int)rintf(u[i] * inv) : 0);
@@ -110,7 +104,7 @@ __device__ __forceinline__ void finish_at(const GemmI8Args& p, int row, int col,
 // overwritten (requests of step s + 2 go out) and, with the wait in front of it, step s + 1 has landed and its first fragments are
 // read under the last products: the matrix pipe waits for other waves once a step, never for LDS.
 template <class T, int TM, int TN, int WM, int WN, int NST>
-__global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_tile_kernel(const GemmI8Args p, int tiles_m, int tiles_n, int vec) {
+__global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_tile_kernel(const GemmI8Args p, int tiles_m, int tiles_n) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
     constexpr int PIECES = (BM + BN) / 8 / NW;       // 1-KiB pieces (8 rows) a wave brings per step
     static_assert((BM / 8) % NW == 0 && (BN / 8) % NW == 0, "a piece lies in one operand for every wave");
@@ -249,7 +243,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
     __syncthreads();
     int* strip = reinterpret_cast<int*>(lds) + wave * 32 * PITCH;
     if constexpr (!EARLY) scales();
-    const bool whole = vec && col + W <= p.n;
+    const bool whole = col + W <= p.n;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
@@ -348,11 +342,8 @@ hipError_t launch_tile(const GemmI8Args& p, hipStream_t stream) {
             done = 1;
         }
     }
-    constexpr int W = Elem<T>::W;
-    const auto wide = [&](const void* t, int64_t ld) { return (reinterpret_cast<uintptr_t>(t) & 15) == 0 && ld % W == 0; };
-    const int vec = wide(p.c, p.ldc) && (p.epi != 3 || wide(p.resid, p.ldr));
     const int tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-    kernel<<<dim3((unsigned)tm * tn), dim3(64 * WM * WN), LDS, stream>>>(p, tm, tn, vec);
+    kernel<<<dim3((unsigned)tm * tn), dim3(64 * WM * WN), LDS, stream>>>(p, tm, tn);
     return hipGetLastError();
 }
 
@@ -382,17 +373,16 @@ hipError_t launch_typed(const GemmI8Args& p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_quant_rows_i8(const QuantRowsArgs& a, hipStream_t stream) {
-    auto go = [&](auto t, auto w) {
+    auto go = [&](auto t) {
         using T = decltype(t);
-        constexpr int W = decltype(w)::value;
-        if (a.cols <= 2048) quant_rows_i8_kernel<T, W, 64><<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, stream>>>(a);
-        else quant_rows_i8_kernel<T, W, 256><<<dim3((unsigned)a.rows), 256, 0, stream>>>(a);
+        if (a.cols <= 2048) quant_rows_i8_kernel<T, 64><<<dim3((unsigned)((a.rows + 3) / 4)), 256, 0, stream>>>(a);
+        else quant_rows_i8_kernel<T, 256><<<dim3((unsigned)a.rows), 256, 0, stream>>>(a);
         return hipGetLastError();
     };
     switch (a.dtype) {
-        case CMDI_DT_F32: return a.vec ? go(float(), std::integral_constant<int, 4>()) : go(float(), std::integral_constant<int, 1>());
-        case CMDI_DT_BF16: return a.vec ? go(Bf16(), std::integral_constant<int, 8>()) : go(Bf16(), std::integral_constant<int, 1>());
-        default: return a.vec ? go(_Float16(), std::integral_constant<int, 8>()) : go(_Float16(), std::integral_constant<int, 1>());
+        case CMDI_DT_F32: return go(float());
+        case CMDI_DT_BF16: return go(Bf16());
+        default: return go(_Float16());
     }
 }
 

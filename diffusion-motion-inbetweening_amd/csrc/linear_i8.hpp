@@ -11,7 +11,7 @@ constexpr int kI8MaxK = 130048;  // 127 * 127 * K (and 128 * 128 * K) stays belo
 struct QuantRowsArgs {
     const void* x;
     int64_t rows, ld;            // ld: elements between rows
-    int32_t cols, dtype, vec;
+    int32_t cols, dtype;
     int8_t* q;                   // [rows][kp]
     int32_t kp;
     float* scale;                // [rows]

@@ -28,29 +28,41 @@ template <> struct Elem<Bf16> {
     static __device__ __forceinline__ Bf16 down(float x) { return Bf16{__builtin_bit_cast(bf16_bits, (__bf16)x)}; }
 };
 
-// W consecutive elements <-> fp32 registers.  W > 1 needs an address that is a multiple of W elements (16-byte accesses; a
-// 32-bit parameter row beside 16-bit data takes two of them, a 16-bit one beside 32-bit data takes 8 bytes).
+// W consecutive elements <-> fp32 registers, one access of up to 16 bytes at any element's address (the hardware takes vector
+// accesses that straddle their alignment; the compiler is told that an element's alignment is all there is).
 template <class T, int W>
 __device__ __forceinline__ void load_vec(const T* p, float (&v)[W]) {
-    if constexpr (W == 1) {
-        v[0] = Elem<T>::up(*p);
-    } else {
-        struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Pack { T e[W]; };
-        const Pack k = *reinterpret_cast<const Pack*>(p);
+    struct __attribute__((packed, aligned(sizeof(T)))) Pack { T e[W]; };
+    const Pack k = *reinterpret_cast<const Pack*>(p);
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = Elem<T>::up(k.e[i]);
-    }
+    for (int i = 0; i < W; ++i) v[i] = Elem<T>::up(k.e[i]);
 }
 template <class T, int W>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[W]) {
-    if constexpr (W == 1) {
-        *p = Elem<T>::down(v[0]);
-    } else {
-        struct alignas(sizeof(T) * W < 16 ? sizeof(T) * W : 16) Pack { T e[W]; };
-        Pack k;
+    struct __attribute__((packed, aligned(sizeof(T)))) Pack { T e[W]; };
+    Pack k;
 #pragma unroll
-        for (int i = 0; i < W; ++i) k.e[i] = Elem<T>::down(v[i]);
-        *reinterpret_cast<Pack*>(p) = k;
+    for (int i = 0; i < W; ++i) k.e[i] = Elem<T>::down(v[i]);
+    *reinterpret_cast<Pack*>(p) = k;
+}
+// the same of the first `n` of them (the end of a row); the others read as 0
+template <class T, int W>
+__device__ __forceinline__ void load_part(const T* p, float (&v)[W], int n) {
+    if (n >= W) {
+        load_vec<T, W>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = i < n ? Elem<T>::up(p[i]) : 0.f;
+    }
+}
+template <class T, int W>
+__device__ __forceinline__ void store_part(T* p, const float (&v)[W], int n) {
+    if (n >= W) {
+        store_vec<T, W>(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (i < n) p[i] = Elem<T>::down(v[i]);
     }
 }
 
