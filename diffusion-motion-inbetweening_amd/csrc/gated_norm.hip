@@ -62,45 +62,76 @@ struct TeamSum {
 template <int W, int NV>
 struct Row { float v[NV][W]; };
 
+// How a team's lanes lie on a row.  WHOLE: W divides the row, a lane's access is all in or all out (a row's odd end costs every
+// access a branch: 130 us against 112 us for 16 x 2048 rows of 2048 forward).
+template <int W_, int TEAM_, int NV_, bool WHOLE_>
+struct Shape {
+    static constexpr int W = W_, TEAM = TEAM_, NV = NV_;
+    static constexpr bool WHOLE = WHOLE_;
+    static constexpr int BLOCK = TEAM == 64 ? 256 : TEAM, TPB = BLOCK / TEAM;
+    using R = Row<W, NV>;
+};
+#define SHAPE                                                      \
+    constexpr int W = S::W, TEAM = S::TEAM, NV = S::NV;            \
+    using R = typename S::R;                                       \
+    (void)W, (void)TEAM, (void)NV
+
 #define FOR_ROW(c, i) _Pragma("unroll") for (int c = 0; c < NV; ++c) _Pragma("unroll") for (int i = 0; i < W; ++i)
 
 // columns behind `dim` read as 0
-template <class T, int W, int TEAM, int NV>
-__device__ __forceinline__ void load_row(Row<W, NV>& r, const T* p, int lane, int dim) {
+template <class S, class T>
+__device__ __forceinline__ void load_row(typename S::R& r, const T* p, int lane, int dim) {
+    SHAPE;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
         const int e = (c * TEAM + lane) * W;
-        load_part<T, W>(p + e, r.v[c], dim - e);
+        if constexpr (S::WHOLE) {
+            if (e < dim) {
+                load_vec<T, W>(p + e, r.v[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i) r.v[c][i] = 0.f;
+            }
+        } else {
+            load_part<T, W>(p + e, r.v[c], dim - e);
+        }
     }
 }
-template <class T, int W, int TEAM, int NV>
-__device__ __forceinline__ void store_row(T* p, const Row<W, NV>& r, int lane, int dim) {
+template <class S, class T>
+__device__ __forceinline__ void store_row(T* p, const typename S::R& r, int lane, int dim) {
+    SHAPE;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
         const int e = (c * TEAM + lane) * W;
-        store_part<T, W>(p + e, r.v[c], dim - e);
+        if constexpr (S::WHOLE) {
+            if (e < dim) store_vec<T, W>(p + e, r.v[c]);
+        } else {
+            store_part<T, W>(p + e, r.v[c], dim - e);
+        }
     }
 }
 // a parameter row, or `fill` where there is none (columns behind `dim` hold 0); the entries allow 32 bits or the rows' own type
-template <class T, int W, int TEAM, int NV>
-__device__ __forceinline__ void load_param(Row<W, NV>& r, const void* p, int64_t off, float fill, const GatedNormArgs& a, int lane) {
+template <class S, class T>
+__device__ __forceinline__ void load_param(typename S::R& r, const void* p, int64_t off, float fill, const GatedNormArgs& a, int lane) {
+    SHAPE;
     if (!p) {
         FOR_ROW(c, i) r.v[c][i] = (c * TEAM + lane) * W + i < a.dim ? fill : 0.f;
     } else if (a.param_dtype == CMDI_DT_F32) {
-        load_row<float, W, TEAM, NV>(r, static_cast<const float*>(p) + off, lane, a.dim);
+        load_row<S, float>(r, static_cast<const float*>(p) + off, lane, a.dim);
     } else {
-        load_row<T, W, TEAM, NV>(r, static_cast<const T*>(p) + off, lane, a.dim);
+        load_row<S, T>(r, static_cast<const T*>(p) + off, lane, a.dim);
     }
 }
-template <class T, int W, int TEAM, int NV>
-__device__ __forceinline__ void store_param(void* p, int64_t off, const Row<W, NV>& r, const GatedNormArgs& a, int lane) {
-    if (a.param_dtype == CMDI_DT_F32) store_row<float, W, TEAM, NV>(static_cast<float*>(p) + off, r, lane, a.dim);
-    else store_row<T, W, TEAM, NV>(static_cast<T*>(p) + off, r, lane, a.dim);
+template <class S, class T>
+__device__ __forceinline__ void store_param(void* p, int64_t off, const typename S::R& r, const GatedNormArgs& a, int lane) {
+    if (a.param_dtype == CMDI_DT_F32) store_row<S, float>(static_cast<float*>(p) + off, r, lane, a.dim);
+    else store_row<S, T>(static_cast<T*>(p) + off, r, lane, a.dim);
 }
 
 // v <- N(v), returns k = 1 / sqrt(mean + eps).  Columns behind `dim` stay 0.
-template <int W, int TEAM, int NV>
-__device__ __forceinline__ float normalise(Row<W, NV>& r, int kind, const GatedNormArgs& a, float inv_dim, int lane, TeamSum<TEAM>& sum) {
+template <class S>
+__device__ __forceinline__ float normalise(typename S::R& r, int kind, const GatedNormArgs& a, float inv_dim, int lane, TeamSum<S::TEAM>& sum) {
+    SHAPE;
     if (kind == CMDI_NORM_NONE) return 1.f;
     float v[1];
     if (kind == CMDI_NORM_LAYER) {
@@ -123,9 +154,9 @@ __device__ __forceinline__ int64_t row_at(const Rows& t, unsigned row, unsigned 
     const unsigned b = row / seq, s = row - b * seq;
     return (int64_t)b * t.bs + (int64_t)s * t.ss;
 }
-template <class T, int W, int TEAM, int NV>
-__device__ __forceinline__ void load_at(Row<W, NV>& r, const Rows& t, int64_t row, const GatedNormArgs& a, int lane) {
-    load_row<T, W, TEAM, NV>(r, static_cast<const T*>(t.p) + row_at(t, (unsigned)row, a.seq), lane, a.dim);
+template <class S, class T>
+__device__ __forceinline__ void load_at(typename S::R& r, const Rows& t, int64_t row, const GatedNormArgs& a, int lane) {
+    load_row<S, T>(r, static_cast<const T*>(t.p) + row_at(t, (unsigned)row, a.seq), lane, a.dim);
 }
 
 // the rows of block `blockIdx.x`: a chunk of a group
@@ -139,9 +170,10 @@ __device__ __forceinline__ void chunk_rows(const GatedNormArgs& a, int64_t& grou
     if (end > total) end = total;
 }
 
-template <class T, int W, int TEAM, int NV>
-__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void gated_norm_fwd_kernel(const GatedNormArgs a) {
-    constexpr int BLOCK = TEAM == 64 ? 256 : TEAM, TPB = BLOCK / TEAM;
+template <class T, class S>
+__global__ __launch_bounds__(S::BLOCK) void gated_norm_fwd_kernel(const GatedNormArgs a) {
+    SHAPE;
+    constexpr int TPB = S::TPB;
     __shared__ float lds[2 * TeamSum<TEAM>::MOST * (TEAM / 64)];
     TeamSum<TEAM> sum(lds);
     const int lane = threadIdx.x % TEAM, team = TPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
@@ -149,33 +181,33 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void gated_norm_fwd_kernel
     chunk_rows(a, group, chunk, first, end);
     const float inv_dim = 1.f / (float)a.dim;
 
-    Row<W, NV> g, wp, bp, w, t;
+    R g, wp, bp, w, t;
     // h = n w (1 + s) + (b (1 + s) + t); r = alpha x + ny (wp g) + bp g
-    load_param<T, W, TEAM, NV>(g, a.gate.p, group * a.gate.bs, 1.f, a, lane);
-    load_param<T, W, TEAM, NV>(wp, a.wp, 0, 1.f, a, lane);
-    load_param<T, W, TEAM, NV>(bp, a.bp, 0, 0.f, a, lane);
-    load_param<T, W, TEAM, NV>(w, a.w, 0, 1.f, a, lane);
-    load_param<T, W, TEAM, NV>(t, a.b, 0, 0.f, a, lane);
+    load_param<S, T>(g, a.gate.p, group * a.gate.bs, 1.f, a, lane);
+    load_param<S, T>(wp, a.wp, 0, 1.f, a, lane);
+    load_param<S, T>(bp, a.bp, 0, 0.f, a, lane);
+    load_param<S, T>(w, a.w, 0, 1.f, a, lane);
+    load_param<S, T>(t, a.b, 0, 0.f, a, lane);
     FOR_ROW(c, i) { wp.v[c][i] *= g.v[c][i]; bp.v[c][i] *= g.v[c][i]; }
-    load_param<T, W, TEAM, NV>(g, a.scale.p, group * a.scale.bs, 0.f, a, lane);
+    load_param<S, T>(g, a.scale.p, group * a.scale.bs, 0.f, a, lane);
     FOR_ROW(c, i) { w.v[c][i] *= 1.f + g.v[c][i]; t.v[c][i] *= 1.f + g.v[c][i]; }
-    load_param<T, W, TEAM, NV>(g, a.shift.p, group * a.shift.bs, 0.f, a, lane);
+    load_param<S, T>(g, a.shift.p, group * a.shift.bs, 0.f, a, lane);
     FOR_ROW(c, i) t.v[c][i] += g.v[c][i];
 
     for (int64_t row = first + team; row < end; row += TPB) {     // (TPB > 1: a team is a wave, nothing in here waits for another)
-        Row<W, NV> x, y;
-        load_at<T, W, TEAM, NV>(x, a.x, row, a, lane);
+        R x, y;
+        load_at<S, T>(x, a.x, row, a, lane);
         if (a.y.p) {
-            load_at<T, W, TEAM, NV>(y, a.y, row, a, lane);
-            normalise<W, TEAM, NV>(y, a.post, a, inv_dim, lane, sum);
+            load_at<S, T>(y, a.y, row, a, lane);
+            normalise<S>(y, a.post, a, inv_dim, lane, sum);
             FOR_ROW(c, i) x.v[c][i] = a.alpha * x.v[c][i] + (y.v[c][i] * wp.v[c][i] + bp.v[c][i]);
         } else {
             FOR_ROW(c, i) x.v[c][i] *= a.alpha;
         }
-        if (a.r) store_row<T, W, TEAM, NV>(static_cast<T*>(a.r) + row * a.dim, x, lane, a.dim);
-        normalise<W, TEAM, NV>(x, a.pre, a, inv_dim, lane, sum);
+        if (a.r) store_row<S, T>(static_cast<T*>(a.r) + row * a.dim, x, lane, a.dim);
+        normalise<S>(x, a.pre, a, inv_dim, lane, sum);
         FOR_ROW(c, i) x.v[c][i] = x.v[c][i] * w.v[c][i] + t.v[c][i];
-        store_row<T, W, TEAM, NV>(static_cast<T*>(a.h) + row * a.dim, x, lane, a.dim);
+        store_row<S, T>(static_cast<T*>(a.h) + row * a.dim, x, lane, a.dim);
     }
 }
 
@@ -189,25 +221,26 @@ struct Sums {
 };
 
 // One row backward: gx, gy written, its column sums added.  wp, bp: N_post's weight and bias times the gate; w: weight (1 + s).
-template <class T, int W, int TEAM, int NV>
-__device__ __forceinline__ void vjp_row(const GatedNormArgs& a, int64_t row, const Row<W, NV>& wp, const Row<W, NV>& bp, const Row<W, NV>& w, float inv_dim,
-                                        int lane, TeamSum<TEAM>& sum, Sums<W, NV>& s) {
-    Row<W, NV> x, y, d;
+template <class S, class T>
+__device__ __forceinline__ void vjp_row(const GatedNormArgs& a, int64_t row, const typename S::R& wp, const typename S::R& bp, const typename S::R& w, float inv_dim,
+                                        int lane, TeamSum<S::TEAM>& sum, Sums<S::W, S::NV>& s) {
+    SHAPE;
+    R x, y, d;
     float ky = 1.f, m[2];
-    load_at<T, W, TEAM, NV>(x, a.x, row, a, lane);
+    load_at<S, T>(x, a.x, row, a, lane);
     if (a.gh.p) {
-        load_at<T, W, TEAM, NV>(d, a.gh, row, a, lane);
+        load_at<S, T>(d, a.gh, row, a, lane);
     } else {
         FOR_ROW(c, i) d.v[c][i] = 0.f;
     }
     if (a.y.p) {
-        load_at<T, W, TEAM, NV>(y, a.y, row, a, lane);
-        ky = normalise<W, TEAM, NV>(y, a.post, a, inv_dim, lane, sum);
+        load_at<S, T>(y, a.y, row, a, lane);
+        ky = normalise<S>(y, a.post, a, inv_dim, lane, sum);
         FOR_ROW(c, i) x.v[c][i] = a.alpha * x.v[c][i] + (y.v[c][i] * wp.v[c][i] + bp.v[c][i]);
     } else {
         FOR_ROW(c, i) { y.v[c][i] = 0.f; x.v[c][i] *= a.alpha; }
     }
-    const float kr = normalise<W, TEAM, NV>(x, a.pre, a, inv_dim, lane, sum);     // x = n
+    const float kr = normalise<S>(x, a.pre, a, inv_dim, lane, sum);     // x = n
     m[0] = m[1] = 0.f;
     FOR_ROW(c, i) {
         s.A.v[c][i] += d.v[c][i];
@@ -220,12 +253,12 @@ __device__ __forceinline__ void vjp_row(const GatedNormArgs& a, int64_t row, con
     float m1 = a.pre == CMDI_NORM_LAYER ? m[0] * inv_dim : 0.f, m2 = m[1] * inv_dim;
     FOR_ROW(c, i) d.v[c][i] = kr * (d.v[c][i] - x.v[c][i] * m2 - m1);
     if (a.gr.p) {
-        load_at<T, W, TEAM, NV>(x, a.gr, row, a, lane);
+        load_at<S, T>(x, a.gr, row, a, lane);
         FOR_ROW(c, i) d.v[c][i] += x.v[c][i];                                     // dr
     }
     if (a.gx) {
         FOR_ROW(c, i) x.v[c][i] = a.alpha * d.v[c][i];
-        store_row<T, W, TEAM, NV>(static_cast<T*>(a.gx) + row * a.dim, x, lane, a.dim);
+        store_row<S, T>(static_cast<T*>(a.gx) + row * a.dim, x, lane, a.dim);
     }
     if (!a.y.p) return;
     m[0] = m[1] = 0.f;
@@ -244,27 +277,28 @@ __device__ __forceinline__ void vjp_row(const GatedNormArgs& a, int64_t row, con
         m2 = m[1] * inv_dim;
         FOR_ROW(c, i) d.v[c][i] = ky * (d.v[c][i] - y.v[c][i] * m2 - m1);
     }
-    store_row<T, W, TEAM, NV>(static_cast<T*>(a.gy) + row * a.dim, d, lane, a.dim);
+    store_row<S, T>(static_cast<T*>(a.gy) + row * a.dim, d, lane, a.dim);
 }
 
 // SPAN: a team takes a.rows_per_chunk whole samples one after the other; otherwise a block a chunk of one group's rows.
-template <class T, int W, int TEAM, int NV, bool SPAN>
-__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void gated_norm_vjp_kernel(const GatedNormArgs a) {
-    constexpr int BLOCK = TEAM == 64 ? 256 : TEAM, TPB = BLOCK / TEAM;
+template <class T, class S, bool SPAN>
+__global__ __launch_bounds__(S::BLOCK) void gated_norm_vjp_kernel(const GatedNormArgs a) {
+    SHAPE;
+    constexpr int TPB = S::TPB;
     __shared__ float lds[2 * TeamSum<TEAM>::MOST * (TEAM / 64)];
     __shared__ float joined[TPB > 1 ? TEAM * NV * W : 1];
     TeamSum<TEAM> sum(lds);
     const int lane = threadIdx.x % TEAM, team = TPB == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
     const float inv_dim = 1.f / (float)a.dim;
-    Row<W, NV> wp, bp, w;
+    R wp, bp, w;
     auto params = [&](int64_t sample) {
-        Row<W, NV> g;
-        load_param<T, W, TEAM, NV>(w, a.w, 0, 1.f, a, lane);
-        load_param<T, W, TEAM, NV>(g, a.scale.p, sample * a.scale.bs, 0.f, a, lane);
+        R g;
+        load_param<S, T>(w, a.w, 0, 1.f, a, lane);
+        load_param<S, T>(g, a.scale.p, sample * a.scale.bs, 0.f, a, lane);
         FOR_ROW(c, i) w.v[c][i] *= 1.f + g.v[c][i];
-        load_param<T, W, TEAM, NV>(g, a.gate.p, sample * a.gate.bs, 1.f, a, lane);
-        load_param<T, W, TEAM, NV>(wp, a.wp, 0, 1.f, a, lane);
-        load_param<T, W, TEAM, NV>(bp, a.bp, 0, 0.f, a, lane);
+        load_param<S, T>(g, a.gate.p, sample * a.gate.bs, 1.f, a, lane);
+        load_param<S, T>(wp, a.wp, 0, 1.f, a, lane);
+        load_param<S, T>(bp, a.bp, 0, 0.f, a, lane);
         FOR_ROW(c, i) { wp.v[c][i] *= g.v[c][i]; bp.v[c][i] *= g.v[c][i]; }
     };
     Sums<W, NV> s;
@@ -276,39 +310,39 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void gated_norm_vjp_kernel
         for (int64_t b = s0; b < s1; ++b) {
             params(b);
             own.clear();
-            for (int i = 0; i < a.seq; ++i) vjp_row<T, W, TEAM, NV>(a, b * a.seq + i, wp, bp, w, inv_dim, lane, sum, own);
+            for (int i = 0; i < a.seq; ++i) vjp_row<S, T>(a, b * a.seq + i, wp, bp, w, inv_dim, lane, sum, own);
             // ds = w N + b A, dt = A, dg = wp P + bp Q; the other parameters' sums take (1 + s) or g along
-            Row<W, NV> u, v;
-            load_param<T, W, TEAM, NV>(u, a.scale.p, b * a.scale.bs, 0.f, a, lane);
+            R u, v;
+            load_param<S, T>(u, a.scale.p, b * a.scale.bs, 0.f, a, lane);
             FOR_ROW(c, i) { s.A.v[c][i] += (1.f + u.v[c][i]) * own.A.v[c][i]; s.N.v[c][i] += (1.f + u.v[c][i]) * own.N.v[c][i]; }
-            load_param<T, W, TEAM, NV>(u, a.gate.p, b * a.gate.bs, 1.f, a, lane);
+            load_param<S, T>(u, a.gate.p, b * a.gate.bs, 1.f, a, lane);
             FOR_ROW(c, i) { s.P.v[c][i] += u.v[c][i] * own.P.v[c][i]; s.Q.v[c][i] += u.v[c][i] * own.Q.v[c][i]; }
-            if (a.g_shift) store_param<T, W, TEAM, NV>(a.g_shift, b * a.dim, own.A, a, lane);
+            if (a.g_shift) store_param<S, T>(a.g_shift, b * a.dim, own.A, a, lane);
             if (a.g_scale) {
-                load_param<T, W, TEAM, NV>(u, a.w, 0, 1.f, a, lane);
-                load_param<T, W, TEAM, NV>(v, a.b, 0, 0.f, a, lane);
+                load_param<S, T>(u, a.w, 0, 1.f, a, lane);
+                load_param<S, T>(v, a.b, 0, 0.f, a, lane);
                 FOR_ROW(c, i) u.v[c][i] = u.v[c][i] * own.N.v[c][i] + v.v[c][i] * own.A.v[c][i];
-                store_param<T, W, TEAM, NV>(a.g_scale, b * a.dim, u, a, lane);
+                store_param<S, T>(a.g_scale, b * a.dim, u, a, lane);
             }
             if (a.g_gate) {
-                load_param<T, W, TEAM, NV>(u, a.wp, 0, 1.f, a, lane);
-                load_param<T, W, TEAM, NV>(v, a.bp, 0, 0.f, a, lane);
+                load_param<S, T>(u, a.wp, 0, 1.f, a, lane);
+                load_param<S, T>(v, a.bp, 0, 0.f, a, lane);
                 FOR_ROW(c, i) u.v[c][i] = u.v[c][i] * own.P.v[c][i] + v.v[c][i] * own.Q.v[c][i];
-                store_param<T, W, TEAM, NV>(a.g_gate, b * a.dim, u, a, lane);
+                store_param<S, T>(a.g_gate, b * a.dim, u, a, lane);
             }
         }
     } else {
         int64_t group, chunk, first, end;
         chunk_rows(a, group, chunk, first, end);
         params(group);
-        for (int64_t row = first + team; row < end; row += TPB) vjp_row<T, W, TEAM, NV>(a, row, wp, bp, w, inv_dim, lane, sum, s);
+        for (int64_t row = first + team; row < end; row += TPB) vjp_row<S, T>(a, row, wp, bp, w, inv_dim, lane, sum, s);
     }
     // the block's column sums: teams add in order, one sum after another, then one write
     float* out = a.work + (int64_t)blockIdx.x * __builtin_popcount(a.slots) * a.dim;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if (!(a.slots >> k & 1)) continue;
-        Row<W, NV>& r = k == 0 ? s.A : k == 1 ? s.N : k == 2 ? s.P : s.Q;
+        typename S::R& r = k == 0 ? s.A : k == 1 ? s.N : k == 2 ? s.P : s.Q;
         if constexpr (TPB > 1) {
             for (int tm = 0; tm < TPB; ++tm) {
                 __syncthreads();
@@ -321,7 +355,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void gated_norm_vjp_kernel
                 }
             }
         }
-        if (team == TPB - 1) store_row<float, W, TEAM, NV>(out, r, lane, a.dim);
+        if (team == TPB - 1) store_row<S, float>(out, r, lane, a.dim);
         out += a.dim;
     }
 }
@@ -429,27 +463,25 @@ __global__ __launch_bounds__(JOIN_COLS * JOIN_SLICES) void gated_norm_join_all_k
 bool per_sample(const GatedNormArgs& a) {
     return (a.gate.p && a.gate.bs) || (a.scale.p && a.scale.bs) || (a.shift.p && a.shift.bs);
 }
-int teams_per_block(int dim, bool vjp) { return dim <= (vjp ? 512 : 1024) ? 4 : 1; }
+int teams_per_block(int dim) { return dim <= 512 ? 4 : 1; }
+int block_threads(int dim) { return dim <= 512 ? 256 : dim <= 1024 ? 128 : dim <= 2048 ? 256 : dim <= 4096 ? 512 : 1024; }
 
-// Width of the team by the row's length.  Forward 8 or 16 elements a lane; backward, where a lane's registers also hold four column
-// sums of each of its columns, 8 as long as a block can be that wide.
-template <bool VJP, int W, class F>
-hipError_t by_width(int dim, F&& f) {
-    if (dim <= 512) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 8 / W>());
-    if constexpr (VJP) {
-        if (dim <= 1024) return f(std::integral_constant<int, 128>(), std::integral_constant<int, 8 / W>());
-    } else {
-        if (dim <= 1024) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 16 / W>());
-    }
-    if (dim <= 2048) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 8 / W>());
-    if constexpr (VJP) {
-        if (dim <= 4096) return f(std::integral_constant<int, 512>(), std::integral_constant<int, 8 / W>());
-        if (dim <= 8192) return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 8 / W>());
-    } else {
-        if (dim <= 4096) return f(std::integral_constant<int, 256>(), std::integral_constant<int, 16 / W>());
-        if (dim <= 8192) return f(std::integral_constant<int, 512>(), std::integral_constant<int, 16 / W>());
-    }
-    return f(std::integral_constant<int, 1024>(), std::integral_constant<int, 16 / W>());
+// Width of the team by the row's length: 8 elements a lane as long as a block can be that wide (backward a lane's registers also
+// hold four column sums of each of its columns).
+template <class T, class F>
+hipError_t by_shape(int dim, F&& f) {
+    constexpr int W = Elem<T>::W;
+    auto go = [&](auto team, auto nv) {
+        constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
+        return dim % W == 0 ? f(Shape<W, TEAM, NV, true>()) : f(Shape<W, TEAM, NV, false>());
+    };
+    using std::integral_constant;
+    if (dim <= 512) return go(integral_constant<int, 64>(), integral_constant<int, 8 / W>());
+    if (dim <= 1024) return go(integral_constant<int, 128>(), integral_constant<int, 8 / W>());
+    if (dim <= 2048) return go(integral_constant<int, 256>(), integral_constant<int, 8 / W>());
+    if (dim <= 4096) return go(integral_constant<int, 512>(), integral_constant<int, 8 / W>());
+    if (dim <= 8192) return go(integral_constant<int, 1024>(), integral_constant<int, 8 / W>());
+    return go(integral_constant<int, 1024>(), integral_constant<int, 16 / W>());
 }
 template <class F>
 hipError_t by_type(const GatedNormArgs& a, F&& f) {
@@ -464,10 +496,10 @@ hipError_t by_type(const GatedNormArgs& a, F&& f) {
 
 void gated_norm_plan(GatedNormArgs& a, bool vjp) {
     const int64_t total = (int64_t)a.batch * a.seq;
-    const int tpb = teams_per_block(a.dim, vjp);
+    const int tpb = teams_per_block(a.dim);
     // blocks that keep the chip busy; a block's rows share its parameter registers and, backward, its column sums (whose partial
     // results the joins read back: fewer, longer blocks there)
-    const int64_t want = vjp ? 1024 : 2048;
+    const int64_t want = (vjp ? 262144 : 524288) / block_threads(a.dim);
     const bool own = per_sample(a);
     a.slots = 0;
     a.span = vjp && own && a.batch >= 256 && a.seq <= 32 && (!a.gate.p || a.gate.bs) && (!a.scale.p || a.scale.bs) && (!a.shift.p || a.shift.bs);
@@ -522,10 +554,9 @@ int64_t gated_norm_work_floats(const GatedNormArgs& a) {
 hipError_t launch_gated_norm_fwd(const GatedNormArgs& a, hipStream_t stream) {
     return by_type(a, [&](auto t) {
         using T = decltype(t);
-        constexpr int W = Elem<T>::W;
-        return by_width<false, W>(a.dim, [&](auto team, auto nv) {
-            constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
-            gated_norm_fwd_kernel<T, W, TEAM, NV><<<dim3((unsigned)(a.groups * a.chunks)), dim3(TEAM == 64 ? 256 : TEAM), 0, stream>>>(a);
+        return by_shape<T>(a.dim, [&](auto shape) {
+            using S = decltype(shape);
+            gated_norm_fwd_kernel<T, S><<<dim3((unsigned)(a.groups * a.chunks)), dim3(S::BLOCK), 0, stream>>>(a);
             return hipGetLastError();
         });
     });
@@ -534,12 +565,11 @@ hipError_t launch_gated_norm_fwd(const GatedNormArgs& a, hipStream_t stream) {
 hipError_t launch_gated_norm_vjp(const GatedNormArgs& a, hipStream_t stream) {
     hipError_t err = by_type(a, [&](auto t) {
         using T = decltype(t);
-        constexpr int W = Elem<T>::W;
-        return by_width<true, W>(a.dim, [&](auto team, auto nv) {
-            constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
-            const dim3 grid((unsigned)(a.groups * a.chunks)), block(TEAM == 64 ? 256 : TEAM);
-            if (a.span) gated_norm_vjp_kernel<T, W, TEAM, NV, true><<<grid, block, 0, stream>>>(a);
-            else gated_norm_vjp_kernel<T, W, TEAM, NV, false><<<grid, block, 0, stream>>>(a);
+        return by_shape<T>(a.dim, [&](auto shape) {
+            using S = decltype(shape);
+            const dim3 grid((unsigned)(a.groups * a.chunks)), block(S::BLOCK);
+            if (a.span) gated_norm_vjp_kernel<T, S, true><<<grid, block, 0, stream>>>(a);
+            else gated_norm_vjp_kernel<T, S, false><<<grid, block, 0, stream>>>(a);
             return hipGetLastError();
         });
     });
