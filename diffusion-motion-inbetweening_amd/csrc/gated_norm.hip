@@ -79,8 +79,10 @@ struct Shape {
 #define FOR_ROW(c, i) _Pragma("unroll") for (int c = 0; c < NV; ++c) _Pragma("unroll") for (int i = 0; i < W; ++i)
 
 // columns behind `dim` read as 0
+// `over`: the W - 1 elements behind the row may be read (they are the tensor's own): one access then also at an odd end, whose
+// separate elements would cost the row a second trip to memory
 template <class S, class T>
-__device__ __forceinline__ void load_row(typename S::R& r, const T* p, int lane, int dim) {
+__device__ __forceinline__ void load_row(typename S::R& r, const T* p, int lane, int dim, bool over = false) {
     SHAPE;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
@@ -91,6 +93,12 @@ __device__ __forceinline__ void load_row(typename S::R& r, const T* p, int lane,
             } else {
 #pragma unroll
                 for (int i = 0; i < W; ++i) r.v[c][i] = 0.f;
+            }
+        } else if (over) {
+            load_part<T, W>(p + e, r.v[c], e < dim ? W : 0);
+            if (e + W > dim) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) r.v[c][i] = e + i < dim ? r.v[c][i] : 0.f;
             }
         } else {
             load_part<T, W>(p + e, r.v[c], dim - e);
@@ -156,7 +164,8 @@ __device__ __forceinline__ int64_t row_at(const Rows& t, unsigned row, unsigned 
 }
 template <class S, class T>
 __device__ __forceinline__ void load_at(typename S::R& r, const Rows& t, int64_t row, const GatedNormArgs& a, int lane) {
-    load_row<S, T>(r, static_cast<const T*>(t.p) + row_at(t, (unsigned)row, a.seq), lane, a.dim);
+    const int64_t at = row_at(t, (unsigned)row, a.seq), last = (int64_t)(a.batch - 1) * t.bs + (int64_t)(a.seq - 1) * t.ss;
+    load_row<S, T>(r, static_cast<const T*>(t.p) + at, lane, a.dim, at + S::W - 1 <= last);
 }
 
 // the rows of block `blockIdx.x`: a chunk of a group
