@@ -672,10 +672,14 @@ PrefixAttnPlan prefix_attention_plan(const PrefixAttnArgs& a, int cus) {
         l.tiles = (int)((rows + bm - 1) / bm);
         const int64_t items = (int64_t)(packed ? 1 : a.batch) * a.kv_heads * l.tiles;
         const int keys = k_end - k_begin, unit = 128;
-        // fill the chip (two blocks a CU) with chunks of at least 256 keys (512 for 128 rows, whose partial results are the
-        // largest); at most 32 of them, so that a wave of the join holds all weights
-        int64_t n = (2 * cus + items - 1) / items;
-        n = std::min<int64_t>(n, std::max(1, keys / (l.by_wave ? 256 : 512)));
+        // Chunks: every one more is a partial result of each row to write and join.  Measured (us, bf16, 32 heads over 8, dim 128):
+        //   64 x 1 token behind 8192 + 512 keys, prefix in 16 / 8 chunks: 43.5 / 37.3;   256 x 1: 8 / 4 chunks: 122 / 109
+        //   8 x 64 tokens behind 8192, 2 / 4 chunks (a block / two a CU): 93 / 85;   32 x 197 tokens, 4 heads, 1000 keys, 1 / 2: 28 / 37
+        //   1 x 100 tokens behind 8192, 8 / 16 chunks: 29.5 / 23.7;   16 x 1 token, own 4096 by wave, 16 / 8 chunks: 46.3 / 42.4
+        // so one block a CU with chunks of 512 keys or more (1024 where the own keys' items run beside them), two where they still have
+        // 2048; by wave, whose blocks hold little, two a CU.  At most 32, so that a wave of the join holds all weights.
+        auto fill = [&](int64_t per_cu, int least) { return std::min<int64_t>((per_cu * cus + items - 1) / items, std::max(1, keys / least)); };
+        int64_t n = l.by_wave ? fill(2, 512) : std::max(fill(1, packed ? 1024 : 512), fill(2, 2048));
         n = std::min<int64_t>(n, 32);
         l.chunk = (int)std::max<int64_t>(unit, ((keys + n - 1) / n + unit - 1) / unit * unit);   // no keys at all: one empty chunk
         l.chunks = std::max(1, (keys + l.chunk - 1) / l.chunk);
@@ -683,7 +687,9 @@ PrefixAttnPlan prefix_attention_plan(const PrefixAttnArgs& a, int cus) {
         plan.slots += l.chunks;
         plan.l[plan.n++] = l;
     };
-    if (a.batch > 1 && a.prefix >= 256 && rows_own < 64) {
+    // Packing pays where the prefix would be read often enough (us, 8 heads, 16 tokens behind 300 keys, 32 samples: packed 18.0, each
+    // for itself 12.4; one token behind 600, 32 samples: 16.5 both) and a sample alone does not fill half a tile of rows
+    if (a.batch > 1 && a.prefix >= 256 && (int64_t)a.batch * a.prefix >= 16384 && rows_own < 64) {
         add(true, 0, a.prefix);
         if (a.own_max > 0) add(false, a.prefix, a.prefix + a.own_max);
         else plan.l[1] = plan.l[0];
