@@ -36,12 +36,16 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 template <class T> struct Mma;
 template <> struct Mma<Bf16> {
+    static constexpr unsigned short TOP = 0x7f80;     // exponent of an infinity or a NaN
+    static __device__ __forceinline__ float up(short v) { return __uint_as_float((unsigned)(unsigned short)v << 16); }
     static __device__ __forceinline__ f32x16 mul(s8 a, s8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ unsigned pack(float x, float y) { return __builtin_bit_cast(unsigned, b2{(__bf16)x, (__bf16)y}); }
 };
 template <> struct Mma<_Float16> {
+    static constexpr unsigned short TOP = 0x7c00;
+    static __device__ __forceinline__ float up(short v) { return (float)__builtin_bit_cast(_Float16, v); }
     static __device__ __forceinline__ f32x16 mul(s8 a, s8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
@@ -80,44 +84,39 @@ constexpr int lds_bytes() {
     return BYWAVE ? 4 * 2 * 32 * DIM * 2 : 5 * 64 * DIM * 2;
 }
 
-// Which rows and which keys an item has.
+// A lane's row: sample, query, head.
+struct Row {
+    bool ok;                              // it exists (else it repeats the last one)
+    int b, i, h;
+};
+
+// Which rows and which keys an item has; the same in all lanes of a wave.
 template <int BM, int KT>
 struct Item {
-    int chunk, n_rows, row0, hk, b0;      // row0: the wave's first row
-    bool row_ok;                          // this lane's row exists (else it repeats the last one)
-    int row_b, row_i, row_h, vis;         // the lane's sample, query, head; own keys it sees
-    int vis_low;                          // own keys that the wave's first row sees
+    int chunk, n_rows, row0, hk, b0;      // row0: the wave's first row;  b0: the sample (packed: 0, it comes from the row)
+    int len;                              // own keys of the sample
+    int vis_low, vis_first;               // own keys that the wave's first row sees, and the block's
     int c0, p1, o0, o1;                   // prefix keys [c0, p1), own keys [o0, o1)
     int np, tiles;                        // tiles of KT keys: prefix ones, all
 
-    __device__ __forceinline__ Item(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int block, int blocks, int first_row, int l31) {
+    __device__ __forceinline__ Item(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int block, int blocks, int first_row) {
         const int grp = a.heads / a.kv_heads;
         const int id = xcd_remap(block, blocks);
         const int tile = id % L.tiles, rest = id / L.tiles;
         const int bh = rest / L.chunks;
         chunk = rest % L.chunks;
         hk = bh % a.kv_heads;
-        b0 = bh / a.kv_heads;                                     // packed: 0, the sample comes from the row
+        b0 = bh / a.kv_heads;
         n_rows = (L.packed ? a.batch : 1) * a.queries * grp;
         row0 = tile * BM + first_row;
-        row_ok = row0 + l31 < n_rows;
-        const int r = row_ok ? row0 + l31 : n_rows - 1;
-        const int rq = r / grp;
-        row_h = hk * grp + r - rq * grp;
-        row_b = L.packed ? rq / a.queries : b0;
-        row_i = L.packed ? rq - row_b * a.queries : rq;
-        vis = vis_low = 0;
+        len = vis_low = vis_first = 0;
         int vis_top = 0;                                          // own keys that the block's last row sees
         if (L.k_end > a.prefix) {                                 // (never for packed rows)
-            int len = a.own_len ? a.own_len[b0] : a.own_max;
+            len = a.own_len ? a.own_len[b0] : a.own_max;
             len = len < 0 ? 0 : len > a.own_max ? a.own_max : len;
-            auto sees = [&](int i) {
-                const int v = a.causal ? len - a.queries + i + 1 : len;
-                return v < 0 ? 0 : v > len ? len : v;
-            };
-            vis = sees(row_i);
-            vis_top = sees(((tile + 1) * BM < n_rows ? (tile + 1) * BM - 1 : n_rows - 1) / grp);
-            vis_low = sees(row0 / grp);
+            vis_top = sees(a, ((tile + 1) * BM < n_rows ? (tile + 1) * BM - 1 : n_rows - 1) / grp);
+            vis_low = sees(a, row0 / grp);
+            vis_first = sees(a, tile * BM / grp);
         }
         c0 = L.k_begin + chunk * L.chunk;
         const int c1 = c0 + L.chunk < L.k_end ? c0 + L.chunk : L.k_end;
@@ -126,6 +125,24 @@ struct Item {
         o1 = c1 - a.prefix < vis_top ? c1 - a.prefix : vis_top;
         np = p1 > c0 ? (p1 - c0 + KT - 1) / KT : 0;
         tiles = np + (o1 > o0 ? (o1 - o0 + KT - 1) / KT : 0);
+    }
+    // own keys that query i sees
+    __device__ __forceinline__ int sees(const PrefixAttnArgs& a, int i) const {
+        const int v = a.causal ? len - a.queries + i + 1 : len;
+        return v < 0 ? 0 : v > len ? len : v;
+    }
+    // worked out anew at each use: kept over the loop it would cost registers that the loop has not got
+    __device__ __forceinline__ Row row(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int l31) const {
+        asm volatile("" : "+v"(l31));
+        const int grp = a.heads / a.kv_heads;
+        Row to;
+        to.ok = row0 + l31 < n_rows;
+        const int r = to.ok ? row0 + l31 : n_rows - 1;
+        const int rq = r / grp;
+        to.h = hk * grp + r - rq * grp;
+        to.b = L.packed ? rq / a.queries : b0;
+        to.i = L.packed ? rq - to.b * a.queries : rq;
+        return to;
     }
 };
 
@@ -163,6 +180,32 @@ struct Walk {
         return false;
     }
 };
+
+// Does any of a tile's `N` KiB in LDS hold an infinity or a NaN (the same answer in all lanes), and zeros for those of the lane's parts
+// (`from`, then every 1 KiB).
+typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+template <class T, int N>
+__device__ __forceinline__ bool any_odd(const char* at, int lane) {
+    us8 top = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        top = __builtin_elementwise_max(top, (us8)(*reinterpret_cast<const us8*>(at + i * 1024 + lane * 16) & (unsigned short)0x7fff));
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) odd |= top[e] >= Mma<T>::TOP;
+    return __any(odd);
+}
+template <class T>
+__device__ __forceinline__ void clear_odd(char* from, int n) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        us8 v = *reinterpret_cast<us8*>(from + i * 1024);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if ((v[e] & 0x7fff) >= Mma<T>::TOP) v[e] = 0;
+        *reinterpret_cast<us8*>(from + i * 1024) = v;
+    }
+}
 
 // A wave's 32 rows against 32 keys at a time.  A row's maximum is moved only when a score passes it by 2^8: until then its p stay
 // below 256, which changes no relative rounding and saves the exchange between the lanes and the rescaling of o.
@@ -275,14 +318,30 @@ struct Rows32 {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+    // Where rows see different keys, a value that is infinite or not a number must reach the rows that see its key and no others (0 times
+    // it is not 0): it is added to their o as it is, which no weight above zero would change, and a zero takes its place in LDS.
+    // `lim`: keys of the tile that the lane's row sees.
+    __device__ __forceinline__ void odd_values(const char* vt, int keys, int lim, int hi) {
+#pragma unroll 1
+        for (int key = 0; key < keys; ++key) {
+            const char* row = vt + key * ROWB + 8 * hi;
+            asm volatile("" : "+v"(row));                         // (no address of this path is kept in registers outside it)
+#pragma unroll
+            for (int i = 0; i < DIM / 8; ++i) {
+                const s4 v = *reinterpret_cast<const s4*>(row + ((i ^ swz<DIM>(key)) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if ((v[e] & Mma<T>::TOP) == Mma<T>::TOP && key < lim) o[i / 4][4 * (i % 4) + e] += Mma<T>::up(v[e]);
+            }
+        }
+    }
     // results: lane (row l31) holds dims 32 d + 8 i + 4 hi + e
-    template <class I>
-    __device__ __forceinline__ void store(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, const I& it, int slots, int hi) const {
-        if (!it.row_ok) return;
+    __device__ __forceinline__ void store(const PrefixAttnArgs& a, const PrefixAttnLaunch& L, int chunk, const Row& r, int slots, int hi) const {
+        if (!r.ok) return;
         const bool some = l > 0.f || l != l;                      // a NaN sum is a result, an empty row is not
         const float inv = some ? 1.f / l : 0.f;
         const float lse2 = some ? m + log2f(l) : -INFINITY;
-        const int64_t row = ((int64_t)it.row_b * a.queries + it.row_i) * a.heads + it.row_h;
+        const int64_t row = ((int64_t)r.b * a.queries + r.i) * a.heads + r.h;
         if (slots == 1) {
             T* out = static_cast<T*>(a.out) + row * DIM + 4 * hi;
 #pragma unroll
@@ -294,9 +353,9 @@ struct Rows32 {
                     for (int e = 0; e < 4; ++e) v[e] = some ? o[d][4 * i + e] * inv : 0.f;
                     store_vec<T, 4>(out + 32 * d + 8 * i, v);
                 }
-            if (a.lse && hi == 0) a.lse[((int64_t)it.row_b * a.heads + it.row_h) * a.queries + it.row_i] = lse2 * kLn2;
+            if (a.lse && hi == 0) a.lse[((int64_t)r.b * a.heads + r.h) * a.queries + r.i] = lse2 * kLn2;
         } else {
-            const int64_t rows = (int64_t)a.batch * a.queries * a.heads, at = (int64_t)(L.slot0 + it.chunk) * rows + row;
+            const int64_t rows = (int64_t)a.batch * a.queries * a.heads, at = (int64_t)(L.slot0 + chunk) * rows + row;
             float* out = a.work + at * DIM + 4 * hi;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
@@ -323,19 +382,19 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
     using I = Item<128, KT>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const I it(a, L, block, blocks, wave * 32, l31);
+    const I it(a, L, block, blocks, wave * 32);
     const bool busy = it.row0 < it.n_rows;                        // this wave has rows (it brings keys in any case)
 
     // the lane's offsets within a tile of K and of V; they change where the walk enters the own keys
-    int key[PIECES], slot[PIECES], ko[PIECES], vo[PIECES];
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-        key[i] = (wave * PIECES + i) * RPP + lane / SLOTS;
-        slot[i] = ((lane % SLOTS) ^ swz<DIM>(key[i])) * 16;
-    }
+    int ko[PIECES], vo[PIECES];
     auto offsets = [&](int (&to)[PIECES], int stride) {
+        int at = lane;
+        asm volatile("" : "+v"(at));                              // (nothing of it is kept in registers)
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) to[i] = key[i] * stride + slot[i];
+        for (int i = 0; i < PIECES; ++i) {
+            const int key = (wave * PIECES + i) * RPP + at / SLOTS;
+            to[i] = key * stride + ((at % SLOTS) ^ swz<DIM>(key)) * 16;
+        }
     };
     Walk<I, DIM, KT> wk, wv;
     wk.start(a, it, false, 0);
@@ -343,7 +402,7 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
     offsets(ko, wk.stride);
     offsets(vo, wv.stride);
     const unsigned mine = lds_at(lds) + wave * PIECES * 1024;     // the wave's first piece of tile slot 0
-    auto bring_k = [&](auto at) {
+    auto bring_k = [&](auto at, unsigned mine) {
         const u4 d = wk.tile();
         dma16<(2 + decltype(at)::value) * TILE>(d, mine, ko[0]);
         dma16<(2 + decltype(at)::value) * TILE + 1024>(d, mine, ko[1]);
@@ -353,7 +412,7 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
         }
         if (wk.step(a, it, false, 1)) offsets(ko, wk.stride);
     };
-    auto bring_v = [&](auto at) {
+    auto bring_v = [&](auto at, unsigned mine) {
         const u4 d = wv.tile();
         dma16<decltype(at)::value * TILE>(d, mine, vo[0]);
         dma16<decltype(at)::value * TILE + 1024>(d, mine, vo[1]);
@@ -371,28 +430,25 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
     Rows32<T, DIM> w(a.scale, lane, 2 * TILE);
     const int tiles = it.tiles;
     if (tiles > 0) {
-        bring_k(C0);
-        bring_v(C0);
-        if (tiles > 1) bring_k(C1);
+        bring_k(C0, mine);
+        bring_v(C0, mine);
+        if (tiles > 1) bring_k(C1, mine);
     }
-    w.load_q(static_cast<const short*>(a.q) + it.row_b * a.q_bs + it.row_i * a.q_ss + it.row_h * a.q_hs + 8 * hi);
+    {
+        const Row r = it.row(a, L, l31);
+        w.load_q(static_cast<const short*>(a.q) + r.b * a.q_bs + r.i * a.q_ss + r.h * a.q_hs + 8 * hi);
+    }
     if (tiles > 0) {
-        // the tile that is worked on: keys from its first one to the segment's end, and those that every row of the wave sees
+        // The tiles up to `plain` hide keys behind a segment's end only, the same for all rows; those behind it (the last ones of causal
+        // own keys) hide keys from some of the block's rows.
+        const int plain = it.vis_first >= it.o1 ? tiles : it.np + (it.vis_first > it.o0 ? (it.vis_first - it.o0) / KT : 0);
         bool own = it.np == 0;
-        int left = own ? it.o1 - it.o0 : it.p1 - it.c0, clear = own ? (it.vis_low - it.o0 < left ? it.vis_low - it.o0 : left) : left;
-        int seen = own ? it.vis - it.o0 : left;                   // the lane's row sees these
-        auto hide = [&](f32x16& sc, int unit) {
-            if (__builtin_expect(clear < 32 * unit + 32, 0)) w.mask(sc, (seen < left ? seen : left) - 32 * unit, lane);
-        };
+        int left = own ? it.o1 - it.o0 : it.p1 - it.c0;           // keys from the tile's first one to the segment's end
         auto next_tile = [&]() {
             left -= KT;
-            clear -= KT;
-            seen -= KT;
             if (__builtin_expect(left <= 0 && !own, 0)) {
                 own = true;
                 left = it.o1 - it.o0;
-                clear = it.vis_low - it.o0 < left ? it.vis_low - it.o0 : left;
-                seen = it.vis - it.o0;
             }
         };
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -405,24 +461,26 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
             w.scores(kf, sc);
         }
         int s = 0;
-        auto tile = [&](auto ks, auto vs) {
-            constexpr int KS = decltype(ks)::value, VS = decltype(vs)::value;
-            // K of s + 1 and V of s are in LDS, and every wave has left K and V of s - 1
+        auto meet = [&]() {   // K of s + 1 and V of s are in LDS, and every wave has left K and V of s - 1
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
-            if (__builtin_expect(s + 2 < tiles, 1)) bring_k(std::integral_constant<int, (KS + 2) % 3>{});
-            if (__builtin_expect(s + 1 < tiles, 1)) bring_v(std::integral_constant<int, (VS + 1) % 2>{});
+        };
+        auto tile = [&](auto ks, auto vs) {
+            constexpr int KS = decltype(ks)::value, VS = decltype(vs)::value;
+            meet();
+            if (__builtin_expect(s + 2 < tiles, 1)) bring_k(std::integral_constant<int, (KS + 2) % 3>{}, mine);
+            if (__builtin_expect(s + 1 < tiles, 1)) bring_v(std::integral_constant<int, (VS + 1) % 2>{}, mine);
             if (__builtin_expect(busy, 1)) {
                 const char *kt = lds + KS * TILE, *kn = lds + (KS + 1) % 3 * TILE, *vt = lds + VS * TILE;
                 w.keys(kt + 32 * ROWB, kf);
-                hide(sc, 0);
+                if (__builtin_expect(left < 32, 0)) w.mask(sc, left, lane);
                 w.settle(sc);
                 w.scores(kf, nx);
                 w.weights(sc);
                 w.values_ahead(vt);
                 w.values(vt);
                 w.keys(kn, kf);
-                hide(nx, 1);
+                if (__builtin_expect(left < 64, 0)) w.mask(nx, left - 32, lane);
                 w.settle(nx);
                 w.scores(kf, sc);                                 // (behind the last tile: what lies there, not used)
                 w.weights(nx);
@@ -431,9 +489,9 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // this wave's reads are done when it meets the others
             next_tile();
-            return ++s < tiles;
+            return ++s < plain;
         };
-        while (true) {
+        while (s < plain) {
             if (!tile(C0, C0)) break;
             if (!tile(C1, C1)) break;
             if (!tile(C2, C0)) break;
@@ -441,9 +499,37 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
             if (!tile(C1, C0)) break;
             if (!tile(C2, C1)) break;
         }
+        // the rest, tile by tile
+        const int seen = it.sees(a, it.row(a, L, l31).i);
+        for (; s < tiles; ++s) {
+            const int ks = s % 3, vs = s & 1;
+            meet();
+            if (s + 2 < tiles) bring_k(C0, mine + (ks == 0 ? 2 : ks - 1) * TILE);
+            if (s + 1 < tiles) bring_v(C0, mine + (vs ^ 1) * TILE);
+            const int at = it.o0 + (s - it.np) * KT, lim = (seen < it.o1 ? seen : it.o1) - at;     // (only own keys are hidden from some rows)
+            char* vt = lds + vs * TILE;
+            if (__builtin_expect(any_odd<T, TILE / 1024>(vt, lane), 0)) {         // all waves say the same
+                w.odd_values(vt, KT, lim, hi);
+                __syncthreads();
+                clear_odd<T>(vt + wave * PIECES * 1024 + lane * 16, PIECES);
+                __syncthreads();
+            }
+            if (busy) {
+                for (int unit = 0; unit < 2; ++unit) {
+                    w.mask(sc, lim - 32 * unit, lane);
+                    w.settle(sc);
+                    w.weights(sc);
+                    w.values_ahead(vt + unit * 32 * ROWB);
+                    w.values(vt + unit * 32 * ROWB);
+                    w.keys(unit == 0 ? lds + ks * TILE + 32 * ROWB : lds + (ks == 2 ? 0 : ks + 1) * TILE, kf);
+                    w.scores(kf, sc);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
     }
     w.l += __shfl_xor(w.l, 32, 64);
-    w.store(a, L, it, slots, hi);
+    w.store(a, L, it.chunk, it.row(a, L, l31), slots, hi);
 }
 
 // Few rows (at most 32): a wave takes every fourth 32-key tile, its K straight into registers, its V through its own two LDS tiles; no
@@ -455,12 +541,12 @@ __device__ __forceinline__ void attend_wave(const PrefixAttnArgs& a, const Prefi
     using I = Item<32, KT>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hi = lane >> 5;
-    const I it(a, L, block, blocks, 0, l31);
+    const I it(a, L, block, blocks, 0);
     char* lds = lds_all + wave * 2 * TILE;
     const unsigned mine = lds_at(lds);
 
     Walk<I, DIM, KT> wk, wv;                                      // the next tile to ask for
-    auto bring_v = [&](auto buf) {
+    auto bring_v = [&](auto buf, unsigned mine) {
         const u4 d = wv.tile();
         auto piece = [&](auto i) {
             constexpr int P = decltype(i)::value;
@@ -496,37 +582,72 @@ __device__ __forceinline__ void attend_wave(const PrefixAttnArgs& a, const Prefi
         wk.start(a, it, false, s);
         wv.start(a, it, true, s);
         load_k(0);
-        bring_v(C0);
+        bring_v(C0, mine);
     }
-    w.load_q(static_cast<const short*>(a.q) + it.row_b * a.q_bs + it.row_i * a.q_ss + it.row_h * a.q_hs + 8 * hi);
+    {
+        const Row r = it.row(a, L, l31);
+        w.load_q(static_cast<const short*>(a.q) + r.b * a.q_bs + r.i * a.q_ss + r.h * a.q_hs + 8 * hi);
+    }
+    // the tiles up to `plain` hide keys behind a segment's end only; those behind it (own keys in causal order) hide keys from some rows
+    const int plain = it.vis_low >= it.o1 ? it.tiles : it.np + (it.vis_low > it.o0 ? (it.vis_low - it.o0) / KT : 0);
+    f32x16 sc;
+    auto landed = [&](bool more) {                                // this tile's values: all but the next one's pieces of V and fragments of K
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES + DS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
     auto one = [&](auto buf, auto other) {
         constexpr int B = decltype(buf)::value;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // the other tile's reads are done
         const bool more = s + 4 < it.tiles;
         if (more) {
             load_k(B ^ 1);
-            bring_v(other);
+            bring_v(other, mine);
         }
-        f32x16 sc;
         w.scores(kreg[B], sc);
-        const bool own = s >= it.np;
-        const int at = (own ? s - it.np : s) * KT, n = (own ? it.o1 - it.o0 : it.p1 - it.c0) - at;
-        if (n < KT || (own && it.o0 + at + KT > it.vis_low)) {
-            const int seen = own ? it.vis - it.o0 - at : n;
-            w.mask(sc, seen < n ? seen : n, lane);
-        }
+        const int n = s >= it.np ? it.o1 - it.o0 - (s - it.np) * KT : it.p1 - it.c0 - s * KT;
+        if (n < KT) w.mask(sc, n, lane);
         w.settle(sc);
         w.weights(sc);
-        // this tile's values have landed once only the next tile's requests are out: its pieces of V and its fragments of K
-        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES + DS) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        landed(more);
         w.values_ahead(lds + B * TILE);
         w.values(lds + B * TILE);
         s += 4;
     };
-    while (s < it.tiles) {
+    int cur = 0;
+    while (s < plain) {
         one(C0, C1);
-        if (s < it.tiles) one(C1, C0);
+        cur = 1;
+        if (s >= plain) break;
+        one(C1, C0);
+        cur = 0;
+    }
+    if (s < it.tiles) {
+        const int seen = it.sees(a, it.row(a, L, l31).i);
+        if (cur)
+#pragma unroll
+            for (int i = 0; i < DS; ++i) kreg[0][i] = kreg[1][i];
+#pragma unroll 1
+        for (; s < it.tiles; s += 4, cur ^= 1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const bool more = s + 4 < it.tiles;
+            w.scores(kreg[0], sc);
+            if (more) {
+                load_k(0);
+                bring_v(C0, mine + (cur ^ 1) * TILE);
+            }
+            const int lim = (seen < it.o1 ? seen : it.o1) - it.o0 - (s - it.np) * KT;
+            char* vt = lds + cur * TILE;
+            w.mask(sc, lim, lane);
+            w.settle(sc);
+            w.weights(sc);
+            landed(more);
+            if (__builtin_expect(any_odd<T, TILE / 1024>(vt, lane), 0)) {
+                w.odd_values(vt, KT, lim, hi);
+                clear_odd<T>(vt + lane * 16, TILE / 1024);
+            }
+            w.values_ahead(vt);
+            w.values(vt);
+        }
     }
     w.l += __shfl_xor(w.l, 32, 64);
 
@@ -565,7 +686,7 @@ __device__ __forceinline__ void attend_wave(const PrefixAttnArgs& a, const Prefi
             w.m = mt;
         }
     }
-    if (wave == 0) w.store(a, L, it, slots, hi);
+    if (wave == 0) w.store(a, L, it.chunk, it.row(a, L, l31), slots, hi);
 }
 
 // The first `n0` blocks work on launch A, the others on B: the packed prefix and the own keys run beside each other.

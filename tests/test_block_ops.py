@@ -152,6 +152,10 @@ NORM_CASES = [
     (2, 3, 16384, "bf16", "bf16", "layer", "layer", "shared", True, True),
     (1, 2, 16383, "bf16", "f32", "rms", "layer", "sample", True, True),
     (700, 2, 40, "bf16", "bf16", "none", "rms", "sample", True, True),
+    (300, 3, 1000, "f16", "f32", "layer", "layer", "sample", False, True),
+    (256, 1, 1025, "f32", "f32", "rms", "rms", "sample", False, True),
+    (3000, 1, 33, "bf16", "f32", "rms", "layer", "sample", False, False),
+    (5, 700, 77, "f32", "f32", "layer", "rms", "shared", False, True),
 ]
 
 
@@ -477,6 +481,53 @@ def test_shared_prefix_attention_never_reads_behind_a_length(n, p):
     # lengths beyond the room and below zero count as the room and zero
     assert torch.equal(ops().shared_prefix_attention(q, pk, pv, ok[:1].expand(3, -1, -1, -1), ov[:1].expand(3, -1, -1, -1),
                                                      torch.tensor([100, 1000, -5], dtype=torch.int32, device="cuda"))[:1], want[:1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,grp,p", [(5, 2, 40), (40, 4, 70), (150, 1, 300), (3, 1, 9000)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_shared_prefix_attention_hidden_values_reach_no_row(n, grp, p, dtype):
+    """Causal order: an infinity or a NaN among the newest tokens changes the queries that see it and no others."""
+    q, pk, pv, ok, ov, _ = attention_case(2, n, 2 * grp, 2, 64, p, n + 20, dtype, seed=6)
+    want = ops().shared_prefix_attention(q, pk, pv, ok, ov)
+    for at, bad in ((n + 19, math.nan), (20 + n // 2, math.inf), (21, -math.inf)):
+        k2, v2 = ok.clone(), ov.clone()
+        v2[1, at, 1, 3] = bad
+        k2[1, at, 0, :] = math.nan                                   # hidden keys do no harm either
+        got = ops().shared_prefix_attention(q, pk, pv, k2, v2)
+        first = at - 20                                              # the first query that sees token `at`
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1, :first], want[1, :first]), at
+        assert torch.isnan(got[1, first:, :grp]).all()               # a key that is no number
+        head1 = got[1, first:, grp:].float()
+        assert (torch.isnan(head1[..., 3]) if bad != bad else torch.isinf(head1[..., 3]) | torch.isnan(head1[..., 3])).all()
+        rest = [d for d in range(64) if d != 3]
+        close = (head1[..., rest] - want[1, first:, grp:].float()[..., rest]).abs().max().item() if first < n else 0.0
+        assert close <= 2 * half_step(q.dtype) * float(v2[1, :, 1, rest].float().abs().nan_to_num(0, 0, 0).max().clamp_min(pv.float().abs().max()))
+
+
+@pytest.mark.gpu
+def test_shared_prefix_attention_and_norm_offsets_beyond_32_bits():
+    # tokens 2^22 elements apart: the last of 1200 starts beyond 2^32 bytes and 2^32 elements
+    g = torch.Generator().manual_seed(8)
+    step, p = 1 << 22, 1200
+    room = torch.empty((p - 1) * step + 256, dtype=torch.bfloat16, device="cuda")
+    wide = room.as_strided((p, 2, 64), (step, 64, 1))
+    near = torch.randn(p, 2, 64, generator=g).bfloat16().cuda()
+    wide.copy_(near)
+    q = torch.randn(3, 2, 4, 64, generator=g).bfloat16().cuda()
+    assert torch.equal(ops().shared_prefix_attention(q, wide, wide), ops().shared_prefix_attention(q, near, near))
+    own = room.as_strided((1, p, 2, 64), (0, step, 64, 1))
+    q = torch.randn(1, 70, 4, 64, generator=g).bfloat16().cuda()
+    assert torch.equal(ops().shared_prefix_attention(q, None, None, own, own), ops().shared_prefix_attention(q, None, None, near[None], near[None]))
+    del room, wide, own
+    step = 1 << 27
+    room = torch.empty(39 * step + 96, dtype=torch.bfloat16, device="cuda")
+    x, near = room.as_strided((4, 10, 96), (10 * step, step, 1)), torch.randn(4, 10, 96, generator=g).bfloat16().cuda()
+    x.copy_(near)
+    for a, b in zip(ops().gated_norm_fwd(x, x), ops().gated_norm_fwd(near, near)):
+        assert torch.equal(a, b)
+    for a, b in zip(ops().gated_norm_vjp(x, x, x, x).values(), ops().gated_norm_vjp(near, near, near, near).values()):
+        assert a is None and b is None or torch.equal(a, b)
 
 
 @pytest.mark.gpu
