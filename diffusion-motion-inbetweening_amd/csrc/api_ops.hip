@@ -139,6 +139,20 @@ int gemm_i8_checked(const void* d_a, const float* d_a_scale, const void* d_w, co
     return CMDI_OK;
 }
 
+int quant_checked(const void* d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld, void* d_q, int32_t kp, float* d_scale, cmdi_stream stream,
+                  bool go) {
+    if (!dt_known(dtype)) return fail(CMDI_E_INVALID, "dtype must be CMDI_DT_F32, CMDI_DT_BF16 or CMDI_DT_F16");
+    if (rows < 0 || rows > kMaxBlocks || cols < 1 || ld < 0) return fail(CMDI_E_INVALID, "rows must lie in [0, 2^22], cols be positive, ld not negative");
+    if (kp < cols || kp % kI8KAlign != 0 || kp > kI8MaxK) return fail(CMDI_E_INVALID, "kp must be a multiple of 128 from cols to 130048");
+    if (rows == 0) return CMDI_OK;
+    if (!d_x || !d_q || !d_scale) return fail(CMDI_E_INVALID, "null tensor");
+    if (!at16(d_q) || !at_elem(d_x, dtype) || !at_elem(d_scale, CMDI_DT_F32)) return fail(CMDI_E_INVALID, "q must be 16-byte aligned, x and scale to their elements");
+    if (!go) return CMDI_OK;
+    QuantRowsArgs a{d_x, rows, ld, cols, dtype, static_cast<int8_t*>(d_q), kp, d_scale};
+    HIPCHK(launch_quant_rows_i8(a, static_cast<hipStream_t>(stream)));
+    return CMDI_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -183,15 +197,7 @@ int cmdi_gated_norm_vjp(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_gra
 
 int cmdi_quant_rows_i8(const void* d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld, void* d_q, int32_t kp, float* d_scale,
                        cmdi_stream stream) {
-    if (!dt_known(dtype)) return fail(CMDI_E_INVALID, "dtype must be CMDI_DT_F32, CMDI_DT_BF16 or CMDI_DT_F16");
-    if (rows < 0 || rows > kMaxBlocks || cols < 1 || ld < 0) return fail(CMDI_E_INVALID, "rows must lie in [0, 2^22], cols be positive, ld not negative");
-    if (kp < cols || kp % kI8KAlign != 0 || kp > kI8MaxK) return fail(CMDI_E_INVALID, "kp must be a multiple of 128 from cols to 130048");
-    if (rows == 0) return CMDI_OK;
-    if (!d_x || !d_q || !d_scale) return fail(CMDI_E_INVALID, "null tensor");
-    if (!at16(d_q) || !at_elem(d_x, dtype) || !at_elem(d_scale, CMDI_DT_F32)) return fail(CMDI_E_INVALID, "q must be 16-byte aligned, x and scale to their elements");
-    QuantRowsArgs a{d_x, rows, ld, cols, dtype, static_cast<int8_t*>(d_q), kp, d_scale};
-    HIPCHK(launch_quant_rows_i8(a, static_cast<hipStream_t>(stream)));
-    return CMDI_OK;
+    return quant_checked(d_x, dtype, rows, cols, ld, d_q, kp, d_scale, stream, true);
 }
 
 int cmdi_gemm_i8(const void* d_a, const float* d_a_scale, const void* d_w, const float* d_w_scale, const float* d_bias, const void* d_resid,
@@ -209,10 +215,18 @@ int cmdi_linear_i8(const void* d_x, int32_t dtype, int32_t m, int32_t cols, int6
         return fail(CMDI_E_INVALID, "workspace must be 16-byte aligned and hold m * (kp + 4) bytes");
     int8_t* q = static_cast<int8_t*>(d_work);
     float* scale = reinterpret_cast<float*>(q + (int64_t)m * kp);
-    // the product's own checks first (m = 0: they need no tensors), so that a refused call has launched nothing
-    const int rc = gemm_i8_checked(q, scale, d_w, d_w_scale, d_bias, d_resid, d_c, m, n, kp, kp, ldw, ldc, ldr, dtype, epi, nullptr, false);
-    if (rc != CMDI_OK || m == 0) return rc;
-    if (int e = cmdi_quant_rows_i8(d_x, dtype, m, cols, ldx, q, kp, scale, stream)) return e;
+    // the checks of both halves first (m = 0: they need no tensors), so that a refused call has launched nothing
+    if (int rc = gemm_i8_checked(q, scale, d_w, d_w_scale, d_bias, d_resid, d_c, m, n, kp, kp, ldw, ldc, ldr, dtype, epi, nullptr, false)) return rc;
+    if (int rc = quant_checked(d_x, dtype, m, cols, ldx, q, kp, scale, nullptr, false)) return rc;
+    if (m == 0) return CMDI_OK;
+    if (linear_i8_fused(m, n, kp, dtype)) {
+        const QuantRowsArgs x{d_x, m, ldx, cols, dtype, nullptr, kp, nullptr};
+        const GemmI8Args p{nullptr, static_cast<const int8_t*>(d_w), nullptr, d_w_scale, d_bias, epi == 3 ? d_resid : nullptr, d_c,
+                           m, n, kp, kp, ldw, ldc, ldr, dtype, epi};
+        HIPCHK(launch_linear_i8_fused(x, p, static_cast<hipStream_t>(stream)));
+        return CMDI_OK;
+    }
+    if (int rc = quant_checked(d_x, dtype, m, cols, ldx, q, kp, scale, stream, true)) return rc;
     return gemm_i8_checked(q, scale, d_w, d_w_scale, d_bias, d_resid, d_c, m, n, kp, kp, ldw, ldc, ldr, dtype, epi, stream, true);
 }
 

@@ -329,6 +329,140 @@ __global__ __launch_bounds__(256) void gemm_i8_rows_kernel(const GemmI8Args p) {
     }
 }
 
+// Few rows with their quantising: every block rounds all the activations for itself, into its LDS, while its weights are on their way
+// (8 x 8192 x 4096: 11.6 us, 2.9 TB/s of weights); the bits are those of quant_rows_i8_kernel and gemm_i8_rows_kernel.  2^lanes lanes share an activation row; a lane's vectors stay
+// packed between the two passes.
+__device__ __forceinline__ float plus_apart(float x, float y) {     // never one instruction with the product that x is
+#pragma clang fp contract(off)
+    return x + y;
+}
+template <class T> struct Packed;
+template <> struct Packed<float> {
+    typedef unsigned U;
+    typedef U V __attribute__((ext_vector_type(4)));
+    static constexpr unsigned ABS = 0x7fffffffu, INF = 0x7f800000u;
+    static __device__ __forceinline__ float up(unsigned v) { return __uint_as_float(v); }
+};
+template <> struct Packed<Bf16> {
+    typedef unsigned short U;
+    typedef U V __attribute__((ext_vector_type(8)));
+    static constexpr unsigned short ABS = 0x7fff, INF = 0x7f80;
+    static __device__ __forceinline__ float up(unsigned short v) { return __uint_as_float((unsigned)v << 16); }
+};
+template <> struct Packed<_Float16> {
+    typedef unsigned short U;
+    typedef U V __attribute__((ext_vector_type(8)));
+    static constexpr unsigned short ABS = 0x7fff, INF = 0x7c00;
+    static __device__ __forceinline__ float up(unsigned short v) { return (float)__builtin_bit_cast(_Float16, v); }
+};
+
+template <class T>
+__global__ __launch_bounds__(256, 2) void linear_i8_rows_kernel(const QuantRowsArgs x, const GemmI8Args p, int lanes) {
+    typedef Packed<T> P;
+    typedef typename P::V V;
+    constexpr int W = Elem<T>::W, NV = kI8FusedBytes / 256 / 16, U = 16;
+    extern __shared__ __attribute__((aligned(16))) char rows8[];       // [m][kp + 16]
+    __shared__ i32x4 part[4][64];
+    __shared__ unsigned high[4];
+    __shared__ float sas[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l15 = lane & 15, kg = lane >> 4;
+    const int kp = p.k, ldq = kp + 16, steps = kp / 64;
+
+    // the activations first: a wait for them must not be one for the weights
+    const int team = 1 << lanes, at = threadIdx.x & (team - 1), row = threadIdx.x >> lanes;
+    const T* xr = static_cast<const T*>(x.x) + (int64_t)(row < p.m ? row : p.m - 1) * x.ld;
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw { V v; };
+    V v[NV];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int e = (c * team + at) * W;
+        v[c] = V(0);
+        if (e + W <= x.cols) v[c] = reinterpret_cast<const Raw*>(xr + e)->v;
+    }
+    const int whole = x.cols / W, rest = x.cols - whole * W;           // a part of a vector at the row's end
+    V end = V(0);
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+        if (i < rest) end[i] = reinterpret_cast<const typename P::U*>(xr)[whole * W + i];
+    const int n0 = blockIdx.x * 16;
+    const int wr = n0 + l15 < p.n ? n0 + l15 : p.n - 1, ar = l15 < p.m ? l15 : p.m - 1;
+    const int8_t* w = p.w + (int64_t)wr * p.ldw + kg * 16;
+    i32x4 fw[U];
+    auto weights = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) fw[u] = *reinterpret_cast<const i32x4*>(w + (int64_t)(s0 + u < steps ? s0 + u : steps - 1) * 64);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    weights(wave * U);
+
+    if (rest > 0 && (whole & (team - 1)) == at) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+            if (c == whole >> lanes) v[c] = end;
+    }
+    // absolute values order as their bits do, infinities and NaN on top
+    V tops = V(0);
+#pragma unroll
+    for (int c = 0; c < NV; ++c) tops = __builtin_elementwise_max(tops, (V)(v[c] & P::ABS));
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) top = top > tops[i] ? top : tops[i];
+    for (int d = team < 64 ? team / 2 : 32; d > 0; d >>= 1) {
+        const unsigned other = __shfl_xor(top, d, 64);
+        top = top > other ? top : other;
+    }
+    if (team > 64) {
+        if (lane == 0) high[wave] = top;
+        __syncthreads();
+        const int first = threadIdx.x >> lanes << (lanes - 6);
+        for (int i = 0; i < team / 64; ++i) top = top > high[first + i] ? top : high[first + i];
+    }
+    const bool fine = top < P::INF;
+    const float most = fine ? P::up(top) : 0.f;
+    const bool some = most >= 1e-35f;
+    const float inv = some ? 127.f / most : 0.f;
+    if (at == 0 && row < p.m) sas[row] = fine ? (some ? most / 127.f : 0.f) : __builtin_nanf("");
+    if (row < p.m) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int e = (c * team + at) * W;
+            if (e < kp) {
+                unsigned o[W / 4];
+#pragma unroll
+                for (int i = 0; i < W; i += 4) {
+                    unsigned b[4];
+                    // 1.5 * 2^23 more: rounded to a whole number, halves to even, its lowest byte in front
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(plus_apart(P::up(v[c][i + k]) * inv, 12582912.f));
+                    o[i / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), 0x05040100u);
+                }
+                __builtin_memcpy(__builtin_assume_aligned(rows8 + row * ldq + e, W), o, W);
+            }
+        }
+    }
+    __syncthreads();
+    i32x4 acc{0, 0, 0, 0};
+    const char* a = rows8 + ar * ldq + kg * 16;
+    for (int s0 = wave * U; s0 < steps;) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (s0 + u < steps) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u], *reinterpret_cast<const i32x4*>(a + (s0 + u) * 64), acc, 0, 0, 0);
+        s0 += 4 * U;
+        if (s0 < steps) weights(s0);
+    }
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0 || l15 >= p.m) return;
+    const i32x4 s = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    const float sa = sas[l15];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int col = n0 + 4 * kg + r;
+        if (col < p.n) finish_at<T>(p, l15, col, s[r], sa, p.w_scale[col], p.bias ? p.bias[col] : 0.f);
+    }
+}
+
 template <class T, int TM, int TN, int WM, int WN, int NST>
 hipError_t launch_tile(const GemmI8Args& p, hipStream_t stream) {
     constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN, LDS = NST * (BM + BN) * 128;
@@ -370,6 +504,9 @@ hipError_t launch_typed(const GemmI8Args& p, hipStream_t stream) {
     return launch_tile<T, 1, 1, 2, 2, 4>(p, stream);
 }
 
+// bits of the row's number among the (up to 16) rows
+int fused_row_bits(int m) { return m <= 1 ? 0 : m <= 2 ? 1 : m <= 4 ? 2 : m <= 8 ? 3 : 4; }
+
 }  // namespace
 
 hipError_t launch_quant_rows_i8(const QuantRowsArgs& a, hipStream_t stream) {
@@ -392,6 +529,24 @@ hipError_t launch_gemm_i8(const GemmI8Args& p, hipStream_t stream) {
         case CMDI_DT_BF16: return launch_typed<Bf16>(p, stream);
         default: return launch_typed<_Float16>(p, stream);
     }
+}
+
+bool linear_i8_fused(int m, int n, int kp, int dtype) {
+    // Measured on an MI355X (us, one launch / quantise, then product):
+    //   8 x 8192 x 4096: 11.6 / 13.5    16 x 8192 x 2048: 10.3 / 10.5   1 x 1024 x 32768: 20.7 / 34.5   16 x 512 x 512 fp32: 5.8 / 6.8
+    //   where the weights take more than one round of blocks:  1 x 28672 x 4096: 27.6 / 26.8    8 x 28672 x 4096: 33.7 / 33.2
+    return m <= 16 && (n + 15) / 16 <= 2 * device_cu_count() && (1 << fused_row_bits(m)) * (int64_t)kp * (dtype == CMDI_DT_F32 ? 4 : 2) <= kI8FusedBytes;
+}
+
+hipError_t launch_linear_i8_fused(const QuantRowsArgs& x, const GemmI8Args& p, hipStream_t stream) {
+    const int lanes = 8 - fused_row_bits(p.m), lds = p.m * (p.k + 16);
+    const dim3 grid((unsigned)((p.n + 15) / 16));
+    switch (p.dtype) {
+        case CMDI_DT_F32: linear_i8_rows_kernel<float><<<grid, 256, lds, stream>>>(x, p, lanes); break;
+        case CMDI_DT_BF16: linear_i8_rows_kernel<Bf16><<<grid, 256, lds, stream>>>(x, p, lanes); break;
+        default: linear_i8_rows_kernel<_Float16><<<grid, 256, lds, stream>>>(x, p, lanes); break;
+    }
+    return hipGetLastError();
 }
 
 }  // namespace cmdi

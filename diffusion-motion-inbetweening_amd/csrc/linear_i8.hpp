@@ -29,4 +29,9 @@ struct GemmI8Args {
 };
 hipError_t launch_gemm_i8(const GemmI8Args& a, hipStream_t stream);
 
+// Few rows: quantising and product in one launch (p.a and p.a_scale are not read).
+constexpr int kI8FusedBytes = 65536;   // bytes of the activations, their rows rounded up to a power of two
+bool linear_i8_fused(int m, int n, int kp, int dtype);
+hipError_t launch_linear_i8_fused(const QuantRowsArgs& x, const GemmI8Args& p, hipStream_t stream);
+
 }  // namespace cmdi

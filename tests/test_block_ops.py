@@ -394,6 +394,53 @@ def test_linear_i8(m, n, k, dtype):
     assert torch.equal(got, ops().gemm_i8(q, scale, qw, sw, bias.cuda(), dtype=got.dtype))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,dtype", [
+    (1, 130, 4096, "bf16"), (2, 515, 2048, "f16"), (3, 96, 4090, "f16"), (4, 8200, 1000, "bf16"), (5, 64, 4095, "bf16"), (8, 300, 4096, "bf16"),
+    (8, 48, 2048, "f32"), (9, 100, 2047, "f16"), (16, 200, 1024, "f32"), (16, 77, 2048, "bf16"), (16, 40, 5000, "bf16"), (1, 33, 32768, "f16"),
+    (1, 17, 16001, "f32"), (2, 50, 9000, "bf16"), (7, 20, 1, "f32"), (13, 8300, 130, "f16"),
+])
+def test_linear_i8_few_rows(m, n, k, dtype):
+    """Quantised in the product's own launch where the rows are few and short, before it otherwise: the same bits."""
+    g = torch.Generator().manual_seed(m * n + k)
+    dt = DTYPES[dtype]
+    x = torch.randn(m, k + 3, generator=g).to(dt).cuda()[:, 3:]        # rows at any alignment
+    qw, sw = ops().quantize_rows(torch.randn(n, k, generator=g).cuda())
+    bias, resid = torch.randn(n, generator=g).cuda(), torch.randn(m, n, generator=g).to(dt).cuda()
+    q, scale = ops().quantize_rows(x)
+    for epi, kw in (("bias", {}), ("gelu", {"bias": bias}), ("resid", {"bias": bias, "resid": resid})):
+        assert torch.equal(ops().linear_i8(x, qw, sw, epi=epi, **kw), ops().gemm_i8(q, scale, qw, sw, epi=epi, dtype=dt, **kw)), epi
+    qa, sa = quant_np(x.float().cpu().numpy())
+    want, tol = gemm64(qa, sa, qw.cpu().numpy()[:, :k], sw.cpu().numpy(), None, "bias", None, dt)
+    within(ops().linear_i8(x, qw, sw), want, tol, "linear")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4, 40])
+def test_linear_i8_rows_that_are_no_numbers(m):
+    g = torch.Generator().manual_seed(m)
+    x = torch.randn(m, 700, generator=g).cuda()
+    x[0, 3], x[1, 699], x[2] = math.inf, math.nan, 1e-38
+    qw, sw = ops().quantize_rows(torch.randn(50, 700, generator=g).cuda())
+    one = torch.ones(50, device="cuda")
+    c = ops().linear_i8(x, qw, sw, one)
+    assert torch.isnan(c[:2]).all() and torch.equal(c[2], one) and torch.isfinite(c[3:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,steps", [(m, n, s) for s in (1, 2, 3, 4, 5, 6, 9) for m, n in ((70, 60), (2040, 2050), (4010, 2050), (4001, 4090))])
+def test_gemm_i8_every_tile_and_step_count(m, n, steps):
+    """Each tile (64, 128 in three and in two stages, 256) at every remainder of its ring; the sums against exact fp64 products."""
+    g = torch.Generator(device="cuda").manual_seed(steps)
+    k = 128 * steps
+    a = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device="cuda")
+    w = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8, device="cuda")
+    one = lambda r: torch.ones(r, device="cuda")  # noqa: E731
+    got = ops().gemm_i8(a, one(m), w, one(n))
+    want = a.double() @ w.double().t()                                 # every partial sum is a whole number below 2^53
+    assert torch.equal(got.double(), want.float().double())
+
+
 # ---- shared-prefix attention ----------------------------------------------------------------------------------------------------
 
 def attention64(q, pk, pv, ok, ov, lens, causal, scale=None):
