@@ -244,7 +244,8 @@ int cmdi_prefix_attention(const cmdi_prefix_attention_desc* d, void* d_out, floa
     if (!d_out || !at16(d_out)) return fail(CMDI_E_INVALID, "out must be there and 16-byte aligned");
     if (!at_elem(d_lse, CMDI_DT_F32)) return fail(CMDI_E_INVALID, "lse is not aligned");
     const PrefixAttnPlan plan = prefix_attention_plan(a, device_cu_count());
-    if (prefix_blocks(a, plan) > kMaxBlocks) return fail(CMDI_E_INVALID, "batch * heads * queries too large");
+    // (the join takes four rows a block)
+    if (prefix_blocks(a, plan) > kMaxBlocks || (plan.slots > 1 && (int64_t)a.batch * a.queries * a.heads > 4 * kMaxBlocks)) return fail(CMDI_E_INVALID, "batch * heads * queries too large");
     const int64_t need = prefix_attention_work_floats(a, plan) * (int64_t)sizeof(float);
     if (need > 0 && (!d_work || work_bytes < need)) return fail(CMDI_E_INVALID, "workspace too small (cmdi_prefix_attention_workspace)");
     if (!at16(d_work)) return fail(CMDI_E_INVALID, "workspace must be 16-byte aligned");

@@ -711,7 +711,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attention_kernel(const PrefixAt
 }
 
 // Joins a row's partial results: out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  One wave a row, a lane a partial
-// result's weight (at most 64), then a lane two columns or one.
+// result's weight (at most 64), then a lane two columns or one, eight partial results in flight.
 template <class T, int DIM>
 __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const PrefixAttnArgs a, int slots, int rows) {
     constexpr int W = DIM / 64;
@@ -725,13 +725,17 @@ __global__ __launch_bounds__(256) void prefix_attention_join_kernel(const Prefix
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.f;
     const float* o = a.work + (int64_t)row * DIM + lane * W;
-#pragma unroll 8
-    for (int s = 0; s < slots; ++s) {
-        float v[W];
-        load_vec<float, W>(o + (int64_t)s * rows * DIM, v);
-        const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k), s));
+    for (int s0 = 0; s0 < slots; s0 += 8) {
+        float v[8][W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) acc[i] += ks * v[i];
+        for (int u = 0; u < 8; ++u) load_vec<float, W>(o + (int64_t)(s0 + u < slots ? s0 + u : slots - 1) * rows * DIM, v[u]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (s0 + u < slots) {
+                const float ks = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(k), s0 + u));
+#pragma unroll
+                for (int i = 0; i < W; ++i) acc[i] += ks * v[u][i];
+            }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll

@@ -47,16 +47,29 @@ def _elsewhere(name: str, t: torch.Tensor, device: int):
     _refuse(f"{name} is on {t.device}, the call's tensors on cuda:{device}")
 
 
-def _launch(device: int, entry, *args):
-    """entry(*args, current stream of `device`) with that device current; raises what the entry reports."""
-    stream = torch._C._cuda_getCurrentRawStream(device)
+def _on(device: int, entry, *args) -> int:
+    """entry(*args) with `device` current; raises what the entry reports."""
     if torch._C._cuda_getDevice() == device:
-        rc = entry(*args, stream)
+        rc = entry(*args)
     else:
         with torch.cuda.device(device):
-            rc = entry(*args, stream)
-    if rc:
-        N.check(rc)
+            rc = entry(*args)
+    if rc < 0:
+        N.check(int(rc))
+    return rc
+
+
+def _launch(device: int, entry, *args):
+    """entry(*args, current stream of `device`)."""
+    _on(device, entry, *args, torch._C._cuda_getCurrentRawStream(device))
+
+
+def _no_backward(name: str, *tensors):
+    """A result without a gradient where one is asked for would train nothing, silently."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _refuse(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 # ---- gated norm -------------------------------------------------------------------------------------------------------------
@@ -150,9 +163,7 @@ def _norm_vjp(args, kw, gr, gh, wanted):
     rs, hs = (0, 0) if gr is None else gr.stride()[:2], (0, 0) if gh is None else gh.stride()[:2]
     lib = N.load()
     grads = [N.ptr(gr), N.ptr(gh), *rs, *hs, *(N.ptr(t) for t in out.values())]
-    need = lib.cmdi_gated_norm_vjp_workspace(desc, _NORM_GRADS.pack(*grads, 0, 0))
-    if need < 0:
-        N.check(int(need))
+    need = _on(device, lib.cmdi_gated_norm_vjp_workspace, desc, _NORM_GRADS.pack(*grads, 0, 0))
     work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _launch(device, lib.cmdi_gated_norm_vjp, desc, _NORM_GRADS.pack(*grads, N.ptr(work), need))
     return out
@@ -297,9 +308,10 @@ def gemm_i8(a, a_scale, w, w_scale, bias=None, *, epi="bias", resid=None, dtype=
 
 def linear_i8(x, w, w_scale, bias=None, *, epi="bias", resid=None) -> torch.Tensor:
     """A linear layer in 8-bit integers: rows of x [M, in] are quantised in the call, (w, w_scale) = quantize_rows(weight [out, in])
-    once -> [M, out] of x's type.  epi 'bias', 'gelu' or 'resid' (+ resid [M, out]); the same bits as gemm_i8 behind
+    once -> [M, out] of x's type, without a backward pass.  epi 'bias', 'gelu' or 'resid' (+ resid [M, out]); the same bits as gemm_i8 behind
     quantize_rows."""
     x, dt, device = _float_rows(x)
+    _no_backward("linear_i8", x, w_scale, bias, resid)
     w = _bytes_rows(w, "w", device)
     (m, cols), (n, kp) = x.shape, w.shape
     if kp != (cols + 127) // 128 * 128:
@@ -326,6 +338,8 @@ def _heads(t: torch.Tensor, name: str, shape, dtype, device: int, limit=1 << 62)
         _refuse(f"{name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
     if t.get_device() != device:
         _elsewhere(name, t, device)
+    if not t.numel():
+        return t, 0, (0,) * (len(shape) - 1)
     for again in (False, True):
         st, at = t.stride(), t.data_ptr()
         fine = st[-1] == 1 and at % 16 == 0
@@ -333,7 +347,7 @@ def _heads(t: torch.Tensor, name: str, shape, dtype, device: int, limit=1 << 62)
             st = [0 if n == 1 else s for n, s in zip(shape, st)]
         for s in st[:-1]:
             fine = fine and s % 8 == 0
-        if again or (fine and st[-3] <= limit) or not t.numel():
+        if again or (fine and st[-3] <= limit):
             return t, at, st[:-1]
         t = t.contiguous()
 
@@ -346,8 +360,10 @@ def shared_prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_l
     q [batch, queries, heads, dim]; prefix_k, prefix_v [prefix, kv_heads, dim] (or None); own_k, own_v [batch, own_max, kv_heads,
     dim] (or None); own_len int32 [batch] on the device (None: own_max); bfloat16 or float16, dim 64 or 128, heads a multiple of
     kv_heads.  scale None: 1 / sqrt(dim).  -> out [batch, queries, heads, dim], with return_lse also the log-sums float32 [batch,
-    heads, queries].  A query that sees no key gives 0 and -inf."""
+    heads, queries].  A query that sees no key gives 0 and -inf.  For serving: there is no
+    backward pass."""
     device = _on_device(q, "q")
+    _no_backward("shared_prefix_attention", q, prefix_k, prefix_v, own_k, own_v)
     dtype, shape = q.dtype, q.shape
     if len(shape) != 4 or dtype not in (torch.bfloat16, torch.float16):
         _refuse(f"q must be [batch, queries, heads, dim] bfloat16 or float16, got {list(shape)} {dtype}")
@@ -387,13 +403,7 @@ def shared_prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_l
     out = torch.empty_like(q, memory_format=_CONTIGUOUS)
     lse = torch.empty((b, h, n), dtype=torch.float32, device=q.device) if return_lse else None
     lib = N.load()
-    if torch._C._cuda_getDevice() == device:
-        need = lib.cmdi_prefix_attention_workspace(desc)
-    else:
-        with torch.cuda.device(device):
-            need = lib.cmdi_prefix_attention_workspace(desc)
-    if need < 0:
-        N.check(int(need))
+    need = _on(device, lib.cmdi_prefix_attention_workspace, desc)
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _launch(device, lib.cmdi_prefix_attention, desc, out.data_ptr(), N.ptr(lse), N.ptr(work), need)
     return (out, lse) if return_lse else out

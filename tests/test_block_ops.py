@@ -497,6 +497,10 @@ ATTENTION_CASES = [
     (2, 2, 4, 1, 64, 333, 70), (4, 3, 8, 2, 128, 1000, 17), (40, 1, 4, 2, 64, 700, 0), (33, 1, 10, 2, 128, 513, 9), (1, 1, 8, 1, 128, 5000, 3),
     (3, 20, 4, 4, 64, 100, 20), (2, 30, 4, 2, 128, 300, 64), (1, 65, 2, 2, 128, 65, 65), (2, 197, 2, 1, 64, 196, 197), (1, 150, 4, 2, 128, 0, 300),
     (6, 5, 4, 4, 128, 600, 300), (1, 17, 1, 1, 64, 2000, 500), (2, 9, 16, 2, 128, 257, 90),
+    # the prefix read once for the whole batch: few rows in all, many in all and few of each sample's own, many of both
+    (20, 1, 8, 8, 128, 1000, 33), (70, 1, 4, 2, 64, 700, 40), (9, 10, 8, 2, 128, 2000, 50), (17, 40, 2, 2, 64, 1000, 64), (300, 1, 2, 2, 128, 256, 5),
+    # long prefixes, split and joined: by wave, in tiles, with a ragged end
+    (1, 2, 2, 1, 128, 40000, 300), (2, 300, 2, 2, 128, 3001, 400), (1, 130, 1, 1, 64, 20001, 0),
 ]
 
 
@@ -703,6 +707,56 @@ def test_block_on_side_streams_and_in_graphs():
                 assert eager_g[n] is None or torch.equal(grads[n], eager_g[n]), (turn, n)
 
 
+FIRST_IN_A_GRAPH = """
+import importlib, torch
+ops = importlib.import_module("diffusion-motion-inbetweening_amd.ops")
+torch.manual_seed(0)
+x = torch.randn(2, 9, 256).half().cuda()
+q, k = torch.randn(2, 70, 4, 128).half().cuda(), torch.randn(2, 400, 2, 128).half().cuda()
+a, w = (torch.randint(-128, 128, (4096, 128), dtype=torch.int8).cuda() for _ in range(2))
+one = torch.ones(4096).cuda()
+
+def calls():
+    q8, s8 = ops.quantize_rows(x[0])
+    return [*ops.gated_norm_fwd(x, x), *(t for t in ops.gated_norm_vjp(x, x, x, x).values() if t is not None), ops.linear_i8(x[0], q8, s8),
+            ops.gemm_i8(a, one, w, one), ops.gemm_i8(a[:2048], one[:2048], w[:2048], one[:2048]), ops.shared_prefix_attention(q, k[0], k[0], k, k),
+            ops.shared_prefix_attention(q[:, :1], k[0], k[0], k, k)]
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls()
+for turn in range(3):
+    x.mul_(0.5)
+    graph.replay()
+    for g, e in zip(got, calls()):
+        assert torch.equal(g, e), turn
+print("all replays agree")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_inside_a_graph():
+    """Nothing has to run eagerly before a capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    run = subprocess.run([sys.executable, "-c", FIRST_IN_A_GRAPH], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=100)
+    assert run.returncode == 0 and "all replays agree" in run.stdout, run.stdout + run.stderr
+
+
+@pytest.mark.gpu
+def test_gated_norm_vjp_without_gradients_and_without_rows():
+    x, w = torch.randn(2, 3, 40, device="cuda"), torch.randn(40, device="cuda")
+    out = ops().gated_norm_vjp(None, None, x, x, gate=w, weight=w)
+    assert sorted(n for n in out if out[n] is not None) == ["gate", "weight", "x", "y"] and not any(t.any() for t in out.values() if t is not None)
+    out = ops().gated_norm_vjp(x[:, :0], x[:, :0], x[:, :0], x[:, :0], gate=w, weight=w)
+    assert out["x"].shape == (2, 0, 40) and not out["gate"].any() and not out["weight"].any()
+    r, h = ops().gated_norm(x[:0], x[:0], weight=w.requires_grad_())
+    (r.sum() + h.sum()).backward()
+    assert r.shape == h.shape == (0, 3, 40) and not w.grad.any()
+
+
 @pytest.mark.gpu
 def test_gated_norm_with_gradients_is_refused_under_capture():
     x = torch.randn(1, 4, 64, device="cuda", requires_grad=True)
@@ -757,6 +811,8 @@ def test_block_operators_refuse_wrong_shapes_and_types():
            lambda: o.shared_prefix_attention(h(1, 1, 2, 64), h(4, 2, 64).bfloat16(), h(4, 2, 64)),
            lambda: o.shared_prefix_attention(h(2, 1, 2, 64), None, None, h(1, 4, 2, 64), h(1, 4, 2, 64)),
            lambda: o.shared_prefix_attention(h(1, 1, 2, 64), h(4, 2, 64), h(4, 2, 64), scale=-1.0),
+           lambda: o.shared_prefix_attention(h(1, 1, 2, 64).requires_grad_(), h(4, 2, 64), h(4, 2, 64)),
+           lambda: o.linear_i8(x[0].requires_grad_(), i8(4, 128), one(4)),
            lambda: o.shared_prefix_attention(h(1, 1, 2, 64), None, None, h(1, 4, 2, 64), h(1, 4, 2, 64), torch.ones(1, dtype=torch.int64, device="cuda")),
            lambda: o.shared_prefix_attention(h(1, 1, 2, 64), None, None, h(1, 4, 2, 64), h(1, 4, 2, 64), torch.ones(1, dtype=torch.int32))]
     for i, call in enumerate(bad):
