@@ -7,6 +7,7 @@
 // add in, so every schedule below gives the same bits; it is rounded to fp32 once, before the scales.
 #include "linear_i8.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 #include "../../include/condmdi.h"
@@ -92,6 +93,31 @@ __device__ __forceinline__ void finish_at(const GemmI8Args& p, int row, int col,
     if (p.epi == 1) v = gelu_erf(v);
     if (p.epi == 3) v += Elem<T>::up(static_cast<const T*>(p.resid)[(int64_t)row * p.ldr + col]);
     static_cast<T*>(p.c)[(int64_t)row * p.ldc + col] = Elem<T>::down(v);
+}
+
+// W sums of a row at `at` in LDS, finished and stored from column `col` on; `whole`: all W lie in the matrix
+template <class T, int W>
+__device__ __forceinline__ void store_row(const GemmI8Args& p, int row, int col, bool whole, const int* at, float sa, const float (&ws)[W], const float (&bias)[W]) {
+    if (whole) {
+        float v[W];
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] = finish(at[e], sa, ws[e], bias[e]);
+        if (p.epi == 1) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] = gelu_erf(v[e]);
+        }
+        if (p.epi == 3) {
+            float r[W];
+            load_vec<T, W>(static_cast<const T*>(p.resid) + (int64_t)row * p.ldr + col, r);
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] += r[e];
+        }
+        store_vec<T, W>(static_cast<T*>(p.c) + (int64_t)row * p.ldc + col, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (col + e < p.n) finish_at<T>(p, row, col + e, at[e], sa, ws[e], bias[e]);
+    }
 }
 
 // Tiles: WM x WN waves, a wave owns TM x TN fragments of 32 x 32 (v_mfma_i32_32x32x32_i8).  K runs in steps of 128 columns
@@ -256,29 +282,116 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
         for (int it = 0; it < 32 / RPI; ++it) {
             const int lr = it * RPI + lane / LPR, row = m0 + (wm * TM + i) * 32 + lr;
             if (row >= p.m) continue;
-            const int* at = strip + lr * PITCH + (lane % LPR) * W;
-            if (whole) {
-                float v[W];
-#pragma unroll
-                for (int e = 0; e < W; ++e) v[e] = finish(at[e], sa[EARLY ? i : 0][it], ws[e], bias[e]);
-                if (p.epi == 1) {
-#pragma unroll
-                    for (int e = 0; e < W; ++e) v[e] = gelu_erf(v[e]);
-                }
-                if (p.epi == 3) {
-                    float r[W];
-                    load_vec<T, W>(static_cast<const T*>(p.resid) + (int64_t)row * p.ldr + col, r);
-#pragma unroll
-                    for (int e = 0; e < W; ++e) v[e] += r[e];
-                }
-                store_vec<T, W>(static_cast<T*>(p.c) + (int64_t)row * p.ldc + col, v);
-            } else {
-#pragma unroll
-                for (int e = 0; e < W; ++e)
-                    if (col + e < p.n) finish_at<T>(p, row, col + e, at[e], sa[EARLY ? i : 0][it], ws[e], bias[e]);
-            }
+            store_row<T>(p, row, col, whole, strip + lr * PITCH + (lane % LPR) * W, sa[EARLY ? i : 0][it], ws, bias);
         }
         asm volatile("" ::: "memory");
+    }
+}
+
+// Short K (STEPS * 128 <= 512 columns) and many rows: a tile's products are too short to hide its way in and out.  A block of 8 waves
+// keeps the weights of its 256 columns in registers and walks down the rows, 32 at a time, whose activations wait in a ring of three
+// LDS tiles; a wave's stores of one tile run under the products of the next, two blocks share a CU.  12608 x 1536 x 512 with fp32
+// results: 22.1 us, of which the 77 MB of C alone would take 13.
+constexpr int kShortTiles = 32;                                       // the most row tiles of a block
+constexpr int kShortWeights = 8 * 8192;
+template <class T, int STEPS>
+__global__ __launch_bounds__(512, 4) void gemm_i8_short_kernel(const GemmI8Args p, int tiles_m, int per, int groups_n) {
+    constexpr int TILE = STEPS * 32 * 128;
+    constexpr int W = Elem<T>::W, PITCH = 36, LPR = 32 / W, RPI = 64 / LPR, STORES = 32 / RPI;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    static_assert(2 * TILE + 8 * 16 * PITCH * 4 + kShortTiles * 32 * 4 <= kShortWeights, "");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, hi = lane >> 5;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);                  // neighbours share rows
+    const int n0 = id % groups_n * 256, t0 = id / groups_n * per, t1 = t0 + per < tiles_m ? t0 + per : tiles_m;
+    if (t0 >= t1) return;
+
+    const int r = (wave & 3) * 8 + (lane >> 3), at_slot = ((lane & 7) ^ ((r >> 1) & 7)) << 4;
+    // LDS: the weights on their way in (64 KiB), later slots 1 and 2 of the ring, the strips and the rows' scales; behind it slot 0
+    auto ring = [&](int slot) { return lds + (slot == 0 ? kShortWeights : (slot - 1) * TILE); };
+    auto bring = [&](int t, int slot) {                               // waves 0 - 3 bring the even steps, 4 - 7 the odd ones
+        const int last = p.m - 1 - t * 32;
+        const int off = (r < last ? r : last) * (int)p.lda + at_slot;
+        const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p.a + (int64_t)t * 32 * p.lda), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < (STEPS + 1) / 2; ++i) {
+            const int s = 2 * i + (wave >> 2);
+            if (s < STEPS)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (__attribute__((address_space(3))) void*)(ring(slot) + s * 4096 + (wave & 3) * 1024), 16,
+                                                         off, s * 128, 0, 0);
+        }
+    };
+    // the weights come through the LDS, two steps at a time in 8 KiB of each wave's own: as fragments straight from memory (32 bytes of
+    // a row at once) they took 8 us of 26
+    bring(t0, 0);
+    i32x4 fw[STEPS * 4];
+    char* mine = lds + wave * 8192;
+    const int wr0 = n0 + wave * 32, sw = (l31 >> 1) & 7;
+    const int8_t* wbase = p.w + (int64_t)(wr0 < p.n ? wr0 : p.n - 1) * p.ldw;
+    const auto rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(wbase), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int s0 = 0; s0 < STEPS; s0 += 2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                                 // 8 rows of a step
+            if (s0 + i / 4 >= STEPS) break;
+            const int row = i % 4 * 8 + (lane >> 3), last = p.n - 1 - wr0;
+            const int off = (row < last ? row : last > 0 ? last : 0) * (int)p.ldw + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(mine + i * 1024), 16, off, (s0 + i / 4) * 128, 0, 0);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int k = 4 * s0; k < 4 * s0 + 8 && k < 4 * STEPS; ++k)
+            fw[k] = *reinterpret_cast<const i32x4*>(mine + (k / 4 - s0) * 4096 + l31 * 128 + (((k % 4 * 2 + hi) ^ sw) << 4));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    __builtin_amdgcn_s_barrier();                                     // the LDS is the ring's now
+    if (t0 + 1 < t1) bring(t0 + 1, 1);
+    const int col = n0 + wave * 32 + (lane % LPR) * W;
+    float ws[W], bias[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const int c = col + i < p.n ? col + i : p.n - 1;
+        ws[i] = p.w_scale[c];
+        bias[i] = p.bias ? p.bias[c] : 0.f;
+    }
+    int* strip = reinterpret_cast<int*>(lds + 2 * TILE) + wave * 16 * PITCH;
+    float* scales = reinterpret_cast<float*>(lds + 2 * TILE + 8 * 16 * PITCH * 4);
+    for (int i = threadIdx.x; i < (t1 - t0) * 32; i += 512) scales[i] = p.a_scale[t0 * 32 + i < p.m ? t0 * 32 + i : p.m - 1];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // (read behind the loop's first barrier)
+
+    const bool whole = col + W <= p.n, all = n0 + 256 <= p.n;         // all: every lane of the block stores whole vectors
+    int slot = 0;
+    for (int t = t0; t < t1; ++t) {
+        // tile t has landed: behind its request there are at least that of t + 1 (STEPS / 2 of it by any wave) and, in a block that
+        // stores whole vectors, t - 1's stores
+        if (t == t0 || t + 1 >= t1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (all) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STEPS / 2 + STORES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STEPS / 2) : "memory");
+        __builtin_amdgcn_s_barrier();                                 // and every wave has left tile t - 1
+        const char* a = ring(slot) + l31 * 128;
+        slot = slot == 2 ? 0 : slot + 1;                              // t + 1's
+        if (t + 2 < t1) bring(t + 2, slot == 2 ? 0 : slot + 1);
+        i32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0;
+#pragma unroll
+        for (int k = 0; k < STEPS * 4; ++k) {
+            const i32x4 fa = *reinterpret_cast<const i32x4*>(a + k / 4 * 4096 + (((k % 4 * 2 + hi) ^ sw) << 4));
+            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa, fw[k], acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {                        // 16 rows: one wave writes and reads, no barrier
+#pragma unroll
+            for (int i = 0; i < 8; ++i) strip[mfma32_row(i, lane) * PITCH + l31] = acc[8 * half + i];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int it = 0; it < STORES / 2; ++it) {
+                const int lr = it * RPI + lane / LPR, row = t * 32 + 16 * half + lr;
+                if (row < p.m)
+                    store_row<T>(p, row, col, whole, strip + lr * PITCH + (lane % LPR) * W, scales[(t - t0) * 32 + 16 * half + lr], ws, bias);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
     }
 }
 
@@ -481,21 +594,50 @@ hipError_t launch_tile(const GemmI8Args& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <class T, int STEPS>
+hipError_t launch_short(const GemmI8Args& p, hipStream_t stream) {
+    constexpr int LDS = kShortWeights + STEPS * 32 * 128;
+    auto* kernel = gemm_i8_short_kernel<T, STEPS>;
+    if (LDS > 64 * 1024) {
+        static PerDevice<int> set;
+        int& done = set.get();
+        if (!done) {
+            hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+            if (e != hipSuccess) return e;
+            done = 1;
+        }
+    }
+    const int tiles_m = (p.m + 31) / 32, groups_n = (p.n + 255) / 256;
+    const int want = std::max(1, 2 * device_cu_count() / groups_n), per = std::min(kShortTiles, (tiles_m + want - 1) / want), groups_m = (tiles_m + per - 1) / per;
+    kernel<<<dim3((unsigned)(groups_m * groups_n)), 512, LDS, stream>>>(p, tiles_m, per, groups_n);
+    return hipGetLastError();
+}
+
 template <class T>
 hipError_t launch_typed(const GemmI8Args& p, hipStream_t stream) {
     // Measured on an MI355X (us, 8-bit operands, bf16 out unless said):
     //   rows kernel / 64 x 64 tile:          16 x 8192 x 4096: 9.1 / 12.7        32 x 8192 x 4096: 14.1 / 12.7
+    //   short K / the tile that is right:    12608 x 1536 x 512 fp32 out: 22.1 / 28.0    12608 x 512 x 512 fp32 + residual: 15.8 / 24.7
+    //                                        50000 x 1000 x 384: 33.2 / 51.3     8192 x 8192 x 512: 47.9 / 58.2    4096 x 4096 x 512: 18.8 / 18.1
+    //                                        and with 2^22 sums or fewer:        2048 x 2048 x 512: 8.8 / 8.1      64 x 65536 x 512: 15.3 / 14.5
     //   64 x 64, four stages / two stages:   65 x 8192 x 4096: 11.8 / 17.4       512 x 4096 x 4096: 15.5 / 17.8
     //   128 x 128, three stages / 64 x 64:   1024 x 4096 x 4096: 23.6 / 30.1     512 x 4096 x 4096 (half a chip of tiles): 20.6 / 15.5
-    //   128 x 128, two stages / three:       2048 x 4096 x 4096: 39.7 / 44.8     12608 x 1536 x 512 fp32 out: 29.2 / 36.8
-    //   256 x 256 / 128 x 128, two stages:   4096^3: 64 / 75    8192 x 8192 x 512: 62 / 81    2048 x 4096 x 4096 (half a chip): 50 / 40
-    //                                        12608 x 1536 x 512 fp32 out (300 tiles, a round and a sixth): 33.9 / 29.2
+    //   128 x 128, two stages / three:       2048 x 4096 x 4096: 39.7 / 44.8
+    //   256 x 256 / 128 x 128, two stages:   4096^3: 64 / 75    2048 x 4096 x 4096 (half a chip): 50 / 40
     const int cus = device_cu_count();
     auto tiles = [&](int side) { return (int64_t)((p.m + side - 1) / side) * ((p.n + side - 1) / side); };
     const int64_t t256 = tiles(256), t128 = tiles(128);
     if (p.m <= 16) {
         gemm_i8_rows_kernel<T><<<dim3((unsigned)((p.n + 15) / 16)), 256, 0, stream>>>(p);
         return hipGetLastError();
+    }
+    if (p.k <= 512 && (int64_t)p.m * p.n > (1 << 22)) {
+        switch (p.k / 128) {
+            case 1: return launch_short<T, 1>(p, stream);
+            case 2: return launch_short<T, 2>(p, stream);
+            case 3: return launch_short<T, 3>(p, stream);
+            default: return launch_short<T, 4>(p, stream);
+        }
     }
     // one block a CU: worth it where its rounds are at least three quarters full
     if (t256 >= cus && 4 * t256 >= 3 * ((t256 + cus - 1) / cus) * cus) return launch_tile<T, 4, 2, 2, 4, 2>(p, stream);

@@ -430,7 +430,8 @@ def test_linear_i8_rows_that_are_no_numbers(m):
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,steps", [(m, n, s) for s in (1, 2, 3, 4, 5, 6, 9) for m, n in ((70, 60), (2040, 2050), (4010, 2050), (4001, 4090))])
 def test_gemm_i8_every_tile_and_step_count(m, n, steps):
-    """Each tile (64, 128 in three and in two stages, 256) at every remainder of its ring; the sums against exact fp64 products."""
+    """Each schedule (tiles of 64, of 128 in three and in two stages, of 256; short K and many sums) at every remainder of its ring;
+    the sums against exact fp64 products."""
     g = torch.Generator(device="cuda").manual_seed(steps)
     k = 128 * steps
     a = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device="cuda")
@@ -439,6 +440,28 @@ def test_gemm_i8_every_tile_and_step_count(m, n, steps):
     got = ops().gemm_i8(a, one(m), w, one(n))
     want = a.double() @ w.double().t()                                 # every partial sum is a whole number below 2^53
     assert torch.equal(got.double(), want.float().double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,dtype,epi", [
+    (5003, 1001, 384, "f16", "gelu"), (4130, 1030, 512, "bf16", "resid"), (66000, 70, 128, "f32", "resid"), (530000, 20, 256, "bf16", "bias"),
+    (1030, 4099, 512, "f32", "gelu"), (40, 110000, 256, "f16", "bias"), (8300, 512, 512, "f32", "bias"),
+])
+def test_gemm_i8_short_k(m, n, k, dtype, epi):
+    """Short K and many sums: the bits that the other schedules give for a part of the rows."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    dt = DTYPES[dtype]
+    a = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device="cuda")
+    w = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8, device="cuda")
+    sa, sw = torch.rand(m, generator=g, device="cuda") / 64, torch.rand(n, generator=g, device="cuda") / k
+    bias = torch.randn(n, generator=g, device="cuda") if epi != "bias" else None
+    resid = torch.randn(m, n + 5, generator=g, device="cuda").to(dt)[:, 5:] if epi == "resid" else None
+    got = ops().gemm_i8(a, sa, w, sw, bias, epi=epi, resid=resid, dtype=dt)
+    step = max(1, min(1000, (1 << 22) // n)) if m > 1000 else 20
+    for i in list(range(0, m, step))[:6] + [m // step // 2 * step, (m - 1) // step * step]:
+        part = slice(i, min(i + step, m))
+        want = ops().gemm_i8(a[part], sa[part], w, sw, bias, epi=epi, resid=None if resid is None else resid[part], dtype=dt)
+        assert torch.equal(got[part], want), i
 
 
 # ---- shared-prefix attention ----------------------------------------------------------------------------------------------------
