@@ -169,6 +169,11 @@ def _norm_vjp(args, kw, gr, gh, wanted):
     return out
 
 
+def _not_captured():
+    if torch.cuda.is_current_stream_capturing():
+        _refuse("gated_norm with gradients cannot be captured: use gated_norm_fwd and gated_norm_vjp inside a graph")
+
+
 class _GatedNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, kw, *args):
@@ -180,6 +185,7 @@ class _GatedNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gr, gh):
+        _not_captured()                       # (the forward pass may have run before the capture)
         args = ctx.saved_tensors
         if gr is None and gh is None:
             return (None,) * (1 + len(args))
@@ -196,15 +202,14 @@ def gated_norm(x, y=None, *, gate=None, residual_scale=1.0, post="none", post_we
 
     x, y [batch, seq, dim] (float32, bfloat16 or float16; y None: no block in front); gate, scale, shift [dim] or [batch, dim];
     weight, bias, post_weight, post_bias [dim]; the parameters all float32 or all of x's type.  post 'none' | 'rms' | 'layer', pre
-    'rms' | 'layer'.  Differentiable (once) in every tensor; a call that would record a backward pass while its stream is
-    being captured is refused: capture gated_norm_fwd and gated_norm_vjp."""
+    'rms' | 'layer'.  Differentiable (once) in every tensor; a call that would record or run a backward pass while its
+    stream is being captured is refused: capture gated_norm_fwd and gated_norm_vjp."""
     if torch.is_grad_enabled():
         args = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
         for t in args:
             if t is not None and t.requires_grad:
                 _on_device(x, "x")
-                if torch.cuda.is_current_stream_capturing():
-                    _refuse("gated_norm with gradients cannot be captured: use gated_norm_fwd and gated_norm_vjp inside a graph")
+                _not_captured()
                 return _GatedNorm.apply(dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps), *args)
     return _norm_fwd(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps)
 

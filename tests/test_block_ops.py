@@ -791,6 +791,15 @@ def test_gated_norm_with_gradients_is_refused_under_capture():
             ops().gated_norm(x)
 
 
+def test_gated_norm_backward_is_refused_under_capture(monkeypatch):
+    o = ops()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    x = torch.zeros(1, 2, 8)
+    ctx = type("ctx", (), dict(saved_tensors=(x,) + (None,) * 8, kw={}, needs_input_grad=(False, True) + (False,) * 8))
+    with torch.no_grad(), pytest.raises(native().NativeError, match="captured"):
+        o._GatedNorm.backward(ctx, x, x)
+
+
 # ---- refusals (no GPU) --------------------------------------------------------------------------------------------------------------
 
 def test_block_operators_refuse_cpu_tensors_and_wrong_arguments():
