@@ -106,34 +106,39 @@ def _norm_desc(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, p
         ys, yp = y.stride(), y.data_ptr()
     else:
         ys, yp = (0, 0), 0
+    vector, of_samples = (d,), (b, d)
     for i, t in enumerate((gate, scale, shift, weight, bias, post_weight, post_bias)):
-        step = 0
-        if t is not None:
-            if pdt is None:
-                pdt = t.dtype
-            ts = t.shape
-            if t.dtype != pdt or (pdt != dtype and pdt != torch.float32):
-                _refuse(f"gate, scale, shift, weights and biases must all be float32 or all {dtype}, got {_PARAMS[i]} {t.dtype}")
-            if t.get_device() != device:
-                _elsewhere(_PARAMS[i], t, device)
-            if len(ts) == 1 and ts[0] == d:
-                if t.stride()[0] != 1 and d > 1:
-                    t = t.contiguous()
-            elif i < 3 and len(ts) == 2 and ts[0] == b and ts[1] == d:
-                st = t.stride()
-                if (st[1] != 1 and d > 1) or st[0] == 0:
-                    t = t.contiguous()
-                    st = t.stride()
-                # a [1, dim] parameter still belongs to its sample (its gradient is [1, dim]): any stride but 0 says so
-                step = st[0] if b > 1 else d
-            else:
-                _refuse(f"{_PARAMS[i]} must be [{d}]{f' or [{b}, {d}]' if i < 3 else ''}, got {list(ts)}")
-            ptrs.append(t.data_ptr())
-        else:
+        if t is None:
+            tensors.append(None)
             ptrs.append(0)
+            strides.append(0)
+            continue
+        if pdt is None:
+            pdt = t.dtype
+            if pdt is not dtype and pdt is not torch.float32:
+                _refuse(f"gate, scale, shift, weights and biases must all be float32 or all {dtype}, got {_PARAMS[i]} {pdt}")
+        if t.dtype is not pdt:
+            _refuse(f"gate, scale, shift, weights and biases must be of one type, got {_PARAMS[i]} {t.dtype} beside {pdt}")
+        if t.get_device() != device:
+            _elsewhere(_PARAMS[i], t, device)
+        ts = t.shape
+        if ts == vector:
+            if not t.is_contiguous():
+                t = t.contiguous()
+            step = 0
+        elif i < 3 and ts == of_samples:
+            st = t.stride()
+            if (st[1] != 1 and d > 1) or st[0] == 0:
+                t = t.contiguous()
+                st = t.stride()
+            # a [1, dim] parameter still belongs to its sample (its gradient is [1, dim]): any stride but 0 says so
+            step = st[0] if b > 1 else d
+        else:
+            _refuse(f"{_PARAMS[i]} must be [{d}]{f' or [{b}, {d}]' if i < 3 else ''}, got {list(ts)}")
         tensors.append(t)
+        ptrs.append(t.data_ptr())
         strides.append(step)
-    desc = _NORM_DESC.pack(b, s, d, code, code if pdt is None or pdt == dtype else 0, N.CMDI_NORMS[post], N.CMDI_NORMS[pre], residual_scale, eps,
+    desc = _NORM_DESC.pack(b, s, d, code, code if pdt is None or pdt is dtype else 0, N.CMDI_NORMS[post], N.CMDI_NORMS[pre], residual_scale, eps,
                            x.data_ptr(), yp, xs[0], xs[1], ys[0], ys[1], *ptrs[:3], *strides[:3], *ptrs[3:])
     return desc, tensors, device
 
@@ -339,10 +344,13 @@ def linear_i8(x, w, w_scale, bias=None, *, epi="bias", resid=None) -> torch.Tens
 def _heads(t: torch.Tensor, name: str, shape, dtype, device: int, limit=1 << 62):
     """(t of `shape` with rows of contiguous, 16-byte aligned dims that the kernels can read in place, or a contiguous copy; its
     address; its strides without the last).  A dimension of one element may carry any stride: 0 stands for it."""
-    if t.shape != shape or t.dtype != dtype:
+    if t.shape != shape or t.dtype is not dtype:
         _refuse(f"{name} must be {list(shape)} {dtype}, got {list(t.shape)} {t.dtype}")
     if t.get_device() != device:
         _elsewhere(name, t, device)
+    st, at = t.stride(), t.data_ptr()
+    if st[-1] == 1 and not at & 15 and st[-3] <= limit and not (st[0] | st[-2] | st[-3]) & 7 and at:
+        return t, at, st[:-1]
     if not t.numel():
         return t, 0, (0,) * (len(shape) - 1)
     for again in (False, True):
