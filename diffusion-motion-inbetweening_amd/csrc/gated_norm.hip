@@ -401,6 +401,7 @@ __global__ __launch_bounds__(JOIN_COLS * JOIN_SLICES) void gated_norm_join_kerne
         if (!(a.slots >> k & 1)) continue;
         float s = 0.f;
         if (col < a.dim)
+#pragma unroll 4
             for (int64_t c = slice; c < a.chunks; c += JOIN_SLICES) s += base[c * pitch + (int64_t)at * a.dim + col];
         __syncthreads();
         part[slice][threadIdx.x % JOIN_COLS] = s;
@@ -437,19 +438,34 @@ __global__ __launch_bounds__(JOIN_COLS * JOIN_SLICES) void gated_norm_join_all_k
     float tot[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) tot[k] = 0.f;
+    const bool apart = !a.span && (a.scale.bs || a.gate.bs);          // (span: g and 1 + s are taken along already)
+    float s1 = a.span || apart ? 1.f : 1.f + param_at(a.scale.p, col < a.dim ? col : 0, 0.f, pd);
+    float gg = a.span || apart ? 1.f : param_at(a.gate.p, col < a.dim ? col : 0, 1.f, pd);
+    constexpr int U = 4;                                              // groups whose sums are on their way together
     if (col < a.dim)
-        for (int64_t gi = slice; gi < a.groups; gi += JOIN_SLICES) {
-            const float* p = a.work + gi * pitch + col;
-            float v[4];
+        for (int64_t g0 = slice; g0 < a.groups; g0 += U * JOIN_SLICES) {
+            float v[U][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[k] = 0.f;
-                if (a.slots >> k & 1) { v[k] = *p; p += a.dim; }
+            for (int k = 0, at = 0; k < 4; ++k) {
+                const bool there = a.slots >> k & 1;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int64_t gi = g0 + u * JOIN_SLICES;
+                    v[u][k] = there && gi < a.groups ? a.work[gi * pitch + (int64_t)at * a.dim + col] : 0.f;
+                }
+                at += there;
             }
-            const float s1 = a.span ? 1.f : 1.f + param_at(a.scale.p, gi * a.scale.bs + col, 0.f, pd);
-            const float gg = a.span ? 1.f : param_at(a.gate.p, gi * a.gate.bs + col, 1.f, pd);   // (span: taken along already)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { tot[k] += v[k]; tot[4 + k] += (k < 2 ? s1 : gg) * v[k]; }
+            for (int u = 0; u < U; ++u) {
+                const int64_t gi = g0 + u * JOIN_SLICES;
+                if (gi >= a.groups) break;
+                if (apart) {
+                    s1 = 1.f + param_at(a.scale.p, gi * a.scale.bs + col, 0.f, pd);
+                    gg = param_at(a.gate.p, gi * a.gate.bs + col, 1.f, pd);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { tot[k] += v[u][k]; tot[4 + k] += (k < 2 ? s1 : gg) * v[u][k]; }
+            }
         }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -538,8 +554,9 @@ void gated_norm_plan(GatedNormArgs& a, bool vjp) {
         a.groups = a.batch;
         a.chunks = chunks;
         a.rows_per_group = a.seq;
-    } else if (vjp && chunks > 256) {
-        // no sample of its own anywhere: 32 groups of chunks whose joins run beside each other, then one of the groups
+    } else if (vjp && chunks > 512) {
+        // no sample of its own anywhere: 32 groups of chunks whose joins run beside each other, then one of the groups.  Against one join
+        // of all chunks (us, whole backward pass): 1000 chunks of width 515: 23 / 34;  512 chunks of width 4096: 71 / 63;  385 of 1024: 18.8 / 19.4
         a.chunks = (chunks + 31) / 32;
         a.groups = (chunks + a.chunks - 1) / a.chunks;
         a.rows_per_group = a.chunks * a.rows_per_chunk;
