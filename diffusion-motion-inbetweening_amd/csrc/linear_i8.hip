@@ -240,7 +240,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
         if (i < steps) bring(i, i);
     if (steps >= NST) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * PIECES) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+    meet_waves();
     read(lds, 0, 0);
     int at = 0;                                       // s % NST
     for (int s = 0; s < steps; ++s) {
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_t
             // step s + 1 has landed once at most the NST - 2 requests behind it are out
             if (s + NST <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * PIECES) : "memory");
             else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
+            meet_waves();
             read(lds + next * STAGE, 0, 0);
         }
         multiply(1, 0, NST == 2 ? PIECES / 2 : PIECES, s + NST < steps, s + NST, at);      // into the stage just left
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(512, 4) void gemm_i8_short_kernel(const GemmI8Args 
             fw[k] = *reinterpret_cast<const i32x4*>(mine + (k / 4 - s0) * 4096 + l31 * 128 + (((k % 4 * 2 + hi) ^ sw) << 4));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    __builtin_amdgcn_s_barrier();                                     // the LDS is the ring's now
+    meet_waves();                                                     // the LDS is the ring's now
     if (t0 + 1 < t1) bring(t0 + 1, 1);
     const int col = n0 + wave * 32 + (lane % LPR) * W;
     float ws[W], bias[W];
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(512, 4) void gemm_i8_short_kernel(const GemmI8Args 
         if (t == t0 || t + 1 >= t1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         else if (all) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STEPS / 2 + STORES) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STEPS / 2) : "memory");
-        __builtin_amdgcn_s_barrier();                                 // and every wave has left tile t - 1
+        meet_waves();                                                 // and every wave has left tile t - 1
         const char* a = ring(slot) + l31 * 128;
         slot = slot == 2 ? 0 : slot + 1;                              // t + 1's
         if (t + 2 < t1) bring(t + 2, slot == 2 ? 0 : slot + 1);

@@ -91,4 +91,12 @@ __device__ __forceinline__ float wave_highest(float v) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// The block's barrier without the waits of __syncthreads(): those of this wave's LDS accesses and requests that the barrier stands for
+// come before it, counted; no access moves over it in either direction.
+__device__ __forceinline__ void meet_waves() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 }  // namespace cmdi

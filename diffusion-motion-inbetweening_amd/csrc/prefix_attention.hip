@@ -464,7 +464,7 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
         int s = 0;
         auto meet = [&]() {   // K of s + 1 and V of s are in LDS, and every wave has left K and V of s - 1
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
+            meet_waves();
         };
         auto tile = [&](auto ks, auto vs) {
             constexpr int KS = decltype(ks)::value, VS = decltype(vs)::value;
