@@ -318,8 +318,8 @@ def gemm_i8(a, a_scale, w, w_scale, bias=None, *, epi="bias", resid=None, dtype=
 
 def linear_i8(x, w, w_scale, bias=None, *, epi="bias", resid=None) -> torch.Tensor:
     """A linear layer in 8-bit integers: rows of x [M, in] are quantised in the call, (w, w_scale) = quantize_rows(weight [out, in])
-    once -> [M, out] of x's type, without a backward pass.  epi 'bias', 'gelu' or 'resid' (+ resid [M, out]); the same bits as gemm_i8 behind
-    quantize_rows."""
+    once -> [M, out] of x's type, without a backward pass.  epi 'bias', 'gelu' or 'resid' (+ resid [M, out]); the same bits as
+    gemm_i8 behind quantize_rows."""
     x, dt, device = _float_rows(x)
     _no_backward("linear_i8", x, w_scale, bias, resid)
     w = _bytes_rows(w, "w", device)

@@ -304,7 +304,8 @@ int cmdi_gemm_i8(const void* d_a, const float* d_a_scale, const void* d_w, const
                  int64_t ldr, int32_t dtype, int32_t epi, cmdi_stream stream);
 
 /* The whole layer, the same bits as the two calls above: quantises x [m, cols] (ldx elements between rows) into d_work, then the
- * product with w [n, kp], kp = cols rounded up to 128, into c of x's `dtype`.  d_work: m * (kp + 4) bytes, 16-byte aligned. */
+ * product with w [n, kp], kp = cols rounded up to 128, into c of x's `dtype`, which must not overlap x (d_resid may be d_c).  d_work:
+ * m * (kp + 4) bytes, 16-byte aligned. */
 int cmdi_linear_i8(const void* d_x, int32_t dtype, int32_t m, int32_t cols, int64_t ldx, const void* d_w, const float* d_w_scale,
                    const float* d_bias, const void* d_resid, void* d_c, int32_t n, int32_t kp, int64_t ldw, int64_t ldc,
                    int64_t ldr, int32_t epi, void* d_work, int64_t work_bytes, cmdi_stream stream);
