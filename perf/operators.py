@@ -9,7 +9,6 @@ Three operators that meet in one transformer block of a denoiser or a text tower
 
 ``own`` says which side ``run`` takes: the framework's calls, or the plain forms below.
 """
-import functools
 import importlib
 import math
 
@@ -22,9 +21,7 @@ _DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 _BYTES = {"f32": 4, "bf16": 2, "f16": 2}
 
 
-@functools.lru_cache(None)
 def _ops():
-    """The framework's module: a program imports it once, not in every pass."""
     return importlib.import_module("diffusion-motion-inbetweening_amd.ops")
 
 
