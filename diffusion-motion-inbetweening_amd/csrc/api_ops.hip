@@ -174,6 +174,7 @@ int64_t cmdi_gated_norm_vjp_workspace(const cmdi_gated_norm_desc* d, const cmdi_
     GatedNormArgs a{};
     if (!g) return fail(CMDI_E_INVALID, "null gradients");
     if (int rc = norm_args(d, g, a)) return rc;
+    if (a.batch == 0 || a.seq == 0) return 0;
     gated_norm_plan(a, true);
     return gated_norm_work_floats(a) * (int64_t)sizeof(float);
 }

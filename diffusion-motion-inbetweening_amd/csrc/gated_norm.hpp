@@ -33,7 +33,7 @@ struct GatedNormArgs {
 
 constexpr int kGatedNormMaxDim = 16384;
 
-void gated_norm_plan(GatedNormArgs& a, bool vjp);
+void gated_norm_plan(GatedNormArgs& a, bool vjp);         // (at least one row)
 int64_t gated_norm_work_floats(const GatedNormArgs& a);   // after gated_norm_plan(a, true)
 hipError_t launch_gated_norm_fwd(const GatedNormArgs& a, hipStream_t stream);
 hipError_t launch_gated_norm_vjp(const GatedNormArgs& a, hipStream_t stream);

@@ -286,7 +286,7 @@ typedef struct {
     int64_t work_bytes;
 } cmdi_gated_norm_grads;
 int cmdi_gated_norm_vjp(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_grads* g, cmdi_stream stream);
-/* Bytes of d_work for these outputs (their pointers only say which are wanted), or a negative CMDI_E_*. */
+/* Bytes of d_work for these outputs (their pointers only say which are wanted), 0 without rows, or a negative CMDI_E_*. */
 int64_t cmdi_gated_norm_vjp_workspace(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_grads* g);
 
 /* Rows in 8 bits: scale[r] = max|x[r]| / 127 (fp32), q[r, k] = round(x[r, k] * (127 / max)), halves to even, both fp32
