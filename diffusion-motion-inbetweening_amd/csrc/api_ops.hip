@@ -18,7 +18,8 @@ bool dt_known(int dt) { return dt == CMDI_DT_F32 || dt == CMDI_DT_BF16 || dt == 
 bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool at_elem(const void* p, int dt) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(dt_bytes(dt) - 1)) == 0; }
 
-// the kernels' launches never exceed this many blocks (grid size in threads stays below 2^32)
+// Blocks of a launch of the 8-bit and attention kernels, 256 or 512 threads each (threads of a launch stay below 2^32); the norms'
+// kernels go out in as many launches as their blocks need (launches.hpp).
 constexpr int64_t kMaxBlocks = (int64_t)1 << 22;
 
 int norm_args(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_grads* g, GatedNormArgs& a) {
@@ -131,7 +132,8 @@ int gemm_i8_checked(const void* d_a, const float* d_a_scale, const void* d_w, co
     if (!at16(d_a) || !at16(d_w)) return fail(CMDI_E_INVALID, "a and w must be 16-byte aligned");
     if (!at_elem(d_c, dtype) || !at_elem(d_resid, dtype) || !at_elem(d_a_scale, CMDI_DT_F32) || !at_elem(d_w_scale, CMDI_DT_F32) || !at_elem(d_bias, CMDI_DT_F32))
         return fail(CMDI_E_INVALID, "a tensor is not aligned to its element");
-    if ((int64_t)((m + 63) / 64) * ((n + 63) / 64) > kMaxBlocks) return fail(CMDI_E_INVALID, "m * n too large");
+    // (up to 16 rows have four blocks where others have a tile)
+    if (((int64_t)m + 63) / 64 * (((int64_t)n + 63) / 64) >= kMaxBlocks) return fail(CMDI_E_INVALID, "m * n: 2^22 tiles of 64 x 64 or more");
     GemmI8Args p{static_cast<const int8_t*>(d_a), static_cast<const int8_t*>(d_w), d_a_scale, d_w_scale, d_bias, epi == 3 ? d_resid : nullptr, d_c,
                  m, n, k, lda, ldw, ldc, ldr, dtype, epi};
     if (!go) return CMDI_OK;
@@ -165,7 +167,6 @@ int cmdi_gated_norm_fwd(const cmdi_gated_norm_desc* d, void* d_r, void* d_h, cmd
     if (!at_elem(d_r, a.dtype) || !at_elem(d_h, a.dtype)) return fail(CMDI_E_INVALID, "an output is not aligned to its element");
     a.r = d_r; a.h = d_h;
     gated_norm_plan(a, false);
-    if (a.groups * a.chunks > kMaxBlocks) return fail(CMDI_E_INVALID, "too many samples");
     HIPCHK(launch_gated_norm_fwd(a, static_cast<hipStream_t>(stream)));
     return CMDI_OK;
 }
@@ -187,7 +188,6 @@ int cmdi_gated_norm_vjp(const cmdi_gated_norm_desc* d, const cmdi_gated_norm_gra
         return a.g_gate || a.g_scale || a.g_shift || a.g_w || a.g_b || a.g_wp || a.g_bp ? fail(CMDI_E_INVALID, "no rows: parameter gradients are the caller's zeros")
                                                                                          : CMDI_OK;
     gated_norm_plan(a, true);
-    if (a.groups * a.chunks > kMaxBlocks) return fail(CMDI_E_INVALID, "too many samples");
     const int64_t need = gated_norm_work_floats(a) * (int64_t)sizeof(float);
     if (need > 0 && (!g->d_work || g->work_bytes < need)) return fail(CMDI_E_INVALID, "workspace too small (cmdi_gated_norm_vjp_workspace)");
     if (!at_elem(g->d_work, CMDI_DT_F32)) return fail(CMDI_E_INVALID, "workspace is not aligned");

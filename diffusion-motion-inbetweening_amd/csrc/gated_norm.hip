@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "../../include/condmdi.h"
+#include "launches.hpp"
 #include "ops_common.hpp"
 
 namespace cmdi {
@@ -170,10 +171,13 @@ __device__ __forceinline__ void load_at(typename S::R& r, const Rows& t, int64_t
     load_row<S, T>(r, static_cast<const T*>(t.p) + at, lane, a.dim, at + S::W - 1 <= last);
 }
 
-// the rows of block `blockIdx.x`: a chunk of a group
+// this block's number over all launches of the pass
+__device__ __forceinline__ unsigned block_at(const GatedNormArgs& a) { return a.first + blockIdx.x; }
+
+// the rows of a block: a chunk of a group
 __device__ __forceinline__ void chunk_rows(const GatedNormArgs& a, int64_t& group, int64_t& chunk, int64_t& first, int64_t& end) {
-    group = blockIdx.x / (unsigned)a.chunks;
-    chunk = blockIdx.x % (unsigned)a.chunks;
+    group = block_at(a) / (unsigned)a.chunks;
+    chunk = block_at(a) % (unsigned)a.chunks;
     first = group * a.rows_per_group + chunk * a.rows_per_chunk;
     end = first + a.rows_per_chunk;
     const int64_t total = (int64_t)a.batch * a.seq, stop = (group + 1) * a.rows_per_group;
@@ -316,7 +320,7 @@ __global__ __launch_bounds__(S::BLOCK) void gated_norm_vjp_kernel(const GatedNor
     s.clear();
     if constexpr (SPAN) {
         Sums<W, NV> own;
-        const int64_t s0 = ((int64_t)blockIdx.x * TPB + team) * a.rows_per_chunk;
+        const int64_t s0 = ((int64_t)block_at(a) * TPB + team) * a.rows_per_chunk;
         const int64_t s1 = s0 + a.rows_per_chunk < a.batch ? s0 + a.rows_per_chunk : a.batch;
         for (int64_t b = s0; b < s1; ++b) {
             params(b);
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(S::BLOCK) void gated_norm_vjp_kernel(const GatedNor
         for (int64_t row = first + team; row < end; row += TPB) vjp_row<S, T>(a, row, wp, bp, w, inv_dim, lane, sum, s);
     }
     // the block's column sums: teams add in order, one sum after another, then one write
-    float* out = a.work + (int64_t)blockIdx.x * __builtin_popcount(a.slots) * a.dim;
+    float* out = a.work + (int64_t)block_at(a) * __builtin_popcount(a.slots) * a.dim;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         if (!(a.slots >> k & 1)) continue;
@@ -390,7 +394,7 @@ constexpr int JOIN_COLS = 64, JOIN_SLICES = 16;
 __global__ __launch_bounds__(JOIN_COLS * JOIN_SLICES) void gated_norm_join_kernel(const GatedNormArgs a, int per_sample, int keep) {
     __shared__ float part[JOIN_SLICES][JOIN_COLS];
     const unsigned cols = (unsigned)(a.dim + JOIN_COLS - 1) / JOIN_COLS;
-    const int64_t group = blockIdx.x / cols;
+    const int64_t group = a.first + blockIdx.x / cols;
     const int col = (int)(blockIdx.x % cols) * JOIN_COLS + threadIdx.x % JOIN_COLS, slice = threadIdx.x / JOIN_COLS;
     const int nslot = __builtin_popcount(a.slots);
     const int64_t pitch = (int64_t)nslot * a.dim;
@@ -579,26 +583,33 @@ int64_t gated_norm_work_floats(const GatedNormArgs& a) {
     return a.groups * a.chunks * (int64_t)__builtin_popcount(a.slots) * a.dim;
 }
 
-hipError_t launch_gated_norm_fwd(const GatedNormArgs& a, hipStream_t stream) {
+hipError_t launch_gated_norm_fwd(const GatedNormArgs& args, hipStream_t stream) {
+    GatedNormArgs a = args;
     return by_type(a, [&](auto t) {
         using T = decltype(t);
         return by_shape<T>(a.dim, [&](auto shape) {
             using S = decltype(shape);
-            gated_norm_fwd_kernel<T, S><<<dim3((unsigned)(a.groups * a.chunks)), dim3(S::BLOCK), 0, stream>>>(a);
-            return hipGetLastError();
+            return in_launches(a.groups * a.chunks, S::BLOCK, 1, [&](int64_t first, unsigned blocks) {
+                a.first = (uint32_t)first;
+                gated_norm_fwd_kernel<T, S><<<dim3(blocks), dim3(S::BLOCK), 0, stream>>>(a);
+                return hipGetLastError();
+            });
         });
     });
 }
 
-hipError_t launch_gated_norm_vjp(const GatedNormArgs& a, hipStream_t stream) {
+hipError_t launch_gated_norm_vjp(const GatedNormArgs& args, hipStream_t stream) {
+    GatedNormArgs a = args;
     hipError_t err = by_type(a, [&](auto t) {
         using T = decltype(t);
         return by_shape<T>(a.dim, [&](auto shape) {
             using S = decltype(shape);
-            const dim3 grid((unsigned)(a.groups * a.chunks)), block(S::BLOCK);
-            if (a.span) gated_norm_vjp_kernel<T, S, true><<<grid, block, 0, stream>>>(a);
-            else gated_norm_vjp_kernel<T, S, false><<<grid, block, 0, stream>>>(a);
-            return hipGetLastError();
+            return in_launches(a.groups * a.chunks, S::BLOCK, 1, [&](int64_t first, unsigned blocks) {
+                a.first = (uint32_t)first;
+                if (a.span) gated_norm_vjp_kernel<T, S, true><<<dim3(blocks), dim3(S::BLOCK), 0, stream>>>(a);
+                else gated_norm_vjp_kernel<T, S, false><<<dim3(blocks), dim3(S::BLOCK), 0, stream>>>(a);
+                return hipGetLastError();
+            });
         });
     });
     if (err != hipSuccess || !a.slots) return err;
@@ -606,8 +617,11 @@ hipError_t launch_gated_norm_vjp(const GatedNormArgs& a, hipStream_t stream) {
     const bool all = a.g_w || a.g_b || a.g_wp || a.g_bp || (a.g_scale && !a.scale.bs) || (a.g_shift && !a.shift.bs) || (a.g_gate && !a.gate.bs);
     const unsigned cols = (unsigned)((a.dim + JOIN_COLS - 1) / JOIN_COLS);
     if (own || a.chunks > 1) {
-        gated_norm_join_kernel<<<dim3(cols * (unsigned)a.groups), dim3(JOIN_COLS * JOIN_SLICES), 0, stream>>>(a, own, all);
-        err = hipGetLastError();
+        err = in_launches(cols * a.groups, JOIN_COLS * JOIN_SLICES, cols, [&](int64_t first, unsigned blocks) {
+            a.first = (uint32_t)first;
+            gated_norm_join_kernel<<<dim3(blocks), dim3(JOIN_COLS * JOIN_SLICES), 0, stream>>>(a, own, all);
+            return hipGetLastError();
+        });
         if (err != hipSuccess || !all) return err;
     }
     gated_norm_join_all_kernel<<<dim3(cols), dim3(JOIN_COLS * JOIN_SLICES), 0, stream>>>(a);

@@ -27,6 +27,7 @@ struct GatedNormArgs {
     float* work;                             // vjp: partial column sums
     // split of the rows (gated_norm_plan)
     int64_t groups, rows_per_group, chunks, rows_per_chunk;
+    uint32_t first = 0;                      // block or (joins) group that the launch's first block takes
     int32_t span;                            // vjp: teams take whole samples (many short ones); rows_per_chunk = samples a team
     int32_t slots;                           // column sums kept: bit 0 sum dh, 1 sum dh n, 2 sum dr ny, 3 sum dr (span: times 1 + s, g)
 };

@@ -292,20 +292,20 @@ int64_t cmdi_gated_norm_vjp_workspace(const cmdi_gated_norm_desc* d, const cmdi_
 /* Rows in 8 bits: scale[r] = max|x[r]| / 127 (fp32), q[r, k] = round(x[r, k] * (127 / max)), halves to even, both fp32
  * operations rounded; columns behind `cols` up to kp are 0.  A row whose largest magnitude is below 1e-35 is all zeros with
  * scale 0; one with an infinity or a NaN has scale NaN.  x [rows, cols] of `dtype` with `ld` elements between rows; q
- * [rows, kp] contiguous, 16-byte aligned, kp a multiple of 128, cols <= kp <= 130048. */
+ * [rows, kp] contiguous, 16-byte aligned, kp a multiple of 128, cols <= kp <= 130048; at most 2^22 rows. */
 int cmdi_quant_rows_i8(const void* d_x, int32_t dtype, int64_t rows, int32_t cols, int64_t ld, void* d_q, int32_t kp,
                        float* d_scale, cmdi_stream stream);
 /* C[m, n] = epi((sum_k a[m, k] w[n, k]) a_scale[m] w_scale[n] + bias[n]); the sum exact in 32-bit integers.  a, w: int8 rows,
  * lda / ldw bytes apart (multiples of 16, at most 2^22), 16-byte aligned; k a multiple of 128, at most 130048.  c (and d_resid
  * for epi 3) of `dtype`, ldc / ldr elements apart; bias fp32 or null.  epi as in cmdi_gemm_nt: 0 bias, 1 bias + GELU(erf),
- * 3 bias + residual (d_resid may be d_c).  m 0: nothing to do. */
+ * 3 bias + residual (d_resid may be d_c).  m 0: nothing to do; n at least 1; fewer than 2^22 tiles of 64 x 64 outputs. */
 int cmdi_gemm_i8(const void* d_a, const float* d_a_scale, const void* d_w, const float* d_w_scale, const float* d_bias,
                  const void* d_resid, void* d_c, int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldw, int64_t ldc,
                  int64_t ldr, int32_t dtype, int32_t epi, cmdi_stream stream);
 
 /* The whole layer, the same bits as the two calls above: quantises x [m, cols] (ldx elements between rows) into d_work, then the
  * product with w [n, kp], kp = cols rounded up to 128, into c of x's `dtype`, which must not overlap x (d_resid may be d_c).  d_work:
- * m * (kp + 4) bytes, 16-byte aligned. */
+ * m * (kp + 4) bytes, 16-byte aligned; m at most 2^22. */
 int cmdi_linear_i8(const void* d_x, int32_t dtype, int32_t m, int32_t cols, int64_t ldx, const void* d_w, const float* d_w_scale,
                    const float* d_bias, const void* d_resid, void* d_c, int32_t n, int32_t kp, int64_t ldw, int64_t ldc,
                    int64_t ldr, int32_t epi, void* d_work, int64_t work_bytes, cmdi_stream stream);
@@ -315,7 +315,9 @@ int cmdi_linear_i8(const void* d_x, int32_t dtype, int32_t m, int32_t cols, int6
  * A row that sees no key is 0 with lse -inf; keys behind a length are never read.  bf16 or f16, dim 64 or 128, heads a multiple
  * of kv_heads (head h reads key head h / (heads / kv_heads)); strides in elements, `dim` contiguous, 16-byte aligned, token
  * strides at most 2^23.  own_len: int32 [batch] on the device (taken as 0 .. own_max), or null: own_max.  scale > 0.
- * d_lse fp32 [batch, heads, queries] or null: log of the softmax's sum.  d_work: cmdi_prefix_attention_workspace bytes. */
+ * d_lse fp32 [batch, heads, queries] or null: log of the softmax's sum.  d_work: cmdi_prefix_attention_workspace bytes.
+ * prefix + own_max below 2^31 - 4096; batch * queries * heads below 2^31, and at most 2^24 where the keys are read in parts (the
+ * workspace is not 0); batch * kv_heads * ceil(queries * heads / kv_heads / 128) at most 2^22. */
 typedef struct {
     int32_t batch, queries, heads, kv_heads, dim, prefix, own_max, causal, dtype;
     float scale;

@@ -1,11 +1,15 @@
 """Block operators (ops.py) at the edges of what their documentation allows.  Formulas, cases and tolerances: test_block_ops.py."""
 import ctypes as C
+import shutil
 import subprocess
 import sys
 from pathlib import Path
 
+import pytest
+import torch
+
 from conftest import PKG
-from test_block_ops import native
+from test_block_ops import E, native, ops, within
 
 REPO = Path(__file__).resolve().parent.parent
 
@@ -28,3 +32,59 @@ def test_gated_norm_workspace_without_rows():
     n = native()
     d = n.GatedNormDesc(batch=0, seq=1, dim=0, post=0, pre=2, residual_scale=1.0, eps=1e-5)
     assert n.load().cmdi_gated_norm_vjp_workspace(C.byref(d), C.byref(n.GatedNormGrads())) == -1      # the other checks come first
+
+
+LAUNCHES = """
+#include <cstdio>
+#include "launches.hpp"
+int main() {
+    long long blocks, whole;
+    int threads;
+    while (std::scanf("%lld %d %lld", &blocks, &threads, &whole) == 3) {
+        cmdi::in_launches(blocks, threads, whole, [](int64_t first, unsigned n) { std::printf("%lld:%u ", (long long)first, n); return 0; });
+        std::printf("\\n");
+    }
+}
+"""
+
+
+def test_launches_cover_all_blocks_and_stay_below_2_to_32_threads(tmp_path):
+    cxx = shutil.which("g++") or shutil.which("clang++")
+    if not cxx:
+        pytest.skip("no C++ compiler")
+    (tmp_path / "l.cpp").write_text(LAUNCHES)
+    subprocess.run([cxx, "-std=c++17", "-I", str(REPO / PKG / "csrc"), str(tmp_path / "l.cpp"), "-o", str(tmp_path / "l")], check=True)
+    cases = [(b, t, w) for t in (128, 256, 512, 1024) for w in (1, 3, 256)
+             for b in (w, 5 * w, (1 << 21) // w * w, ((1 << 22) // w + 1) * w, ((1 << 31) // w) * w, ((1 << 31) - 1) * w)]
+    out = subprocess.run([str(tmp_path / "l")], input="\n".join(f"{b} {t} {w}" for b, t, w in cases), capture_output=True, text=True, check=True).stdout
+    for (b, t, w), line in zip(cases, out.splitlines()):
+        parts = [tuple(map(int, p.split(":"))) for p in line.split()]
+        assert sum(n for _, n in parts) == b and parts[0][0] == 0, (b, t, w)
+        for (f, n), (g, _) in zip(parts, parts[1:]):
+            assert n % w == 0 and f + n // w == g, (b, t, w)
+        assert max(n for _, n in parts) * t < 1 << 32, (b, t, w)
+    assert len(out.splitlines()) == len(cases)
+
+
+@pytest.mark.gpu
+def test_gated_norm_more_samples_than_a_launch_has_blocks():
+    """2^23 + 5 samples of one row: the rows' pass takes two launches, the joins of their column sums five."""
+    b, d = (1 << 23) + 5, 2
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, y, gr, gh, scale, shift, gate = rnd(b, 1, d), rnd(b, 1, d).abs(), rnd(b, 1, d).abs(), rnd(b, 1, d), rnd(b, d), rnd(b, d), rnd(d)
+    kw = dict(gate=gate, pre="rms")
+    r, h = ops().gated_norm_fwd(x, y, scale=scale, shift=shift, **kw)
+    got = ops().gated_norm_vjp(gr, gh, x, y, scale=scale, shift=shift, **kw)
+    for at in (0, (1 << 21) - 2, (1 << 22) - 2, (1 << 23) - 2):
+        p = slice(at, at + 7)
+        r2, h2 = ops().gated_norm_fwd(x[p], y[p], scale=scale[p], shift=shift[p], **kw)
+        assert torch.equal(r[p], r2) and torch.equal(h[p], h2), at
+        part = ops().gated_norm_vjp(gr[p], gh[p], x[p], y[p], scale=scale[p], shift=shift[p], **kw)
+        for n in ("x", "y", "scale", "shift"):
+            assert torch.equal(got[n][p], part[n]), (n, at)
+    # dr = gr where h has no gradient: dgate = sum gr y, all terms positive; 16 slices add 2^19 samples each one after another, then each other
+    got = ops().gated_norm_vjp(gr, None, x, y, scale=scale, shift=shift, **kw, wanted=("gate", "scale"))
+    want = (gr.double() * y.double()).sum((0, 1))
+    within(got["gate"], want, ((1 << 19) + 144) * E * want, "gate")
+    assert not got["scale"].any()
