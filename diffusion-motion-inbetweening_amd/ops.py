@@ -249,8 +249,10 @@ def _float_rows(x: torch.Tensor):
 
 def quantize_rows(x: torch.Tensor):
     """Rows of x [rows, cols] in 8 bits -> (q int8 [rows, cols rounded up to 128] with zeros behind the columns, scale float32
-    [rows]); x ~ q * scale.  For weights [out, in] once, for activations [tokens, in] in every call."""
+    [rows]); x ~ q * scale, without a backward pass.  For weights [out, in] once (a parameter's .detach()), for activations
+    [tokens, in] in every call."""
     x, code, device = _float_rows(x)
+    _no_backward("quantize_rows", x)
     rows, cols = x.shape
     kp = (cols + 127) // 128 * 128
     q = torch.empty((rows, kp), dtype=torch.int8, device=x.device)
@@ -297,8 +299,9 @@ def _epilogue(epi, resid, m: int, n: int, dtype, device: int):
 def gemm_i8(a, a_scale, w, w_scale, bias=None, *, epi="bias", resid=None, dtype=torch.float32) -> torch.Tensor:
     """C = epi((a wᵀ) * a_scale[:, None] * w_scale + bias) for int8 rows a [M, K], w [N, K] (K a multiple of 128, as
     quantize_rows pads it), the sum exact in 32-bit integers.  epi 'bias', 'gelu' or 'resid' (+ resid [M, N] of `dtype`); C of
-    `dtype`."""
+    `dtype`, without a backward pass."""
     device = _on_device(a, "a")
+    _no_backward("gemm_i8", a_scale, w_scale, bias, resid)
     out = N.CMDI_DT.get(dtype)
     if out is None:
         _refuse(f"dtype must be float32, bfloat16 or float16, got {dtype}")

@@ -88,3 +88,34 @@ def test_gated_norm_more_samples_than_a_launch_has_blocks():
     want = (gr.double() * y.double()).sum((0, 1))
     within(got["gate"], want, ((1 << 19) + 144) * E * want, "gate")
     assert not got["scale"].any()
+
+
+def test_refusal_of_a_lost_gradient():
+    o, t = ops(), torch.zeros(2, requires_grad=True)
+    with pytest.raises(native().NativeError, match="no backward pass"):
+        o._no_backward("f", None, torch.zeros(2), t)
+    with torch.no_grad():
+        o._no_backward("f", None, t)
+    o._no_backward("f", None, t.detach())
+
+
+@pytest.mark.gpu
+def test_8_bit_layer_refuses_every_call_that_would_lose_a_gradient():
+    o, err = ops(), native().NativeError
+    i8 = lambda *s: torch.ones(*s, dtype=torch.int8, device="cuda")  # noqa: E731
+    one = lambda *s: torch.ones(*s, device="cuda")  # noqa: E731
+    leaf = lambda *s: one(*s).requires_grad_()  # noqa: E731
+    a, w, x = i8(3, 128), i8(5, 128), one(3, 128)
+    calls = [lambda: o.quantize_rows(leaf(3, 100)),
+             lambda: o.gemm_i8(a, leaf(3), w, one(5)), lambda: o.gemm_i8(a, one(3), w, leaf(5)), lambda: o.gemm_i8(a, one(3), w, one(5), leaf(5)),
+             lambda: o.gemm_i8(a, one(3), w, one(5), epi="resid", resid=leaf(3, 5)),
+             lambda: o.linear_i8(leaf(3, 128), w, one(5)), lambda: o.linear_i8(x, w, leaf(5)), lambda: o.linear_i8(x, w, one(5), leaf(5)),
+             lambda: o.linear_i8(x, w, one(5), epi="resid", resid=leaf(3, 5))]
+    for i, call in enumerate(calls):
+        with pytest.raises(err, match="no backward pass"):
+            call()
+            pytest.fail(f"call {i} was accepted")
+        with torch.no_grad():
+            call()
+    for want, got in zip(o.quantize_rows(one(3, 100)), o.quantize_rows(leaf(3, 100).detach())):
+        assert torch.equal(want, got)
