@@ -17,6 +17,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -64,8 +65,17 @@ def _launch(device: int, entry, *args):
     _on(device, entry, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
+def _no_tangent(name: str, *tensors):
+    """A result without a tangent where an input carries one would be a derivative of zero, silently."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _refuse(f"{name} has no forward-mode derivative: call it on tensors without a tangent")
+
+
 def _no_backward(name: str, *tensors):
-    """A result without a gradient where one is asked for would train nothing, silently."""
+    """A result without a gradient where one is asked for would train nothing, silently; the same of tangents."""
+    _no_tangent(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -191,6 +201,7 @@ class _GatedNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gr, gh):
         _not_captured()                       # (the forward pass may have run before the capture)
+        _no_tangent("gated_norm's backward pass", gr, gh)
         args = ctx.saved_tensors
         if gr is None and gh is None:
             return (None,) * (1 + len(args))
@@ -207,21 +218,23 @@ def gated_norm(x, y=None, *, gate=None, residual_scale=1.0, post="none", post_we
 
     x, y [batch, seq, dim] (float32, bfloat16 or float16; y None: no block in front); gate, scale, shift [dim] or [batch, dim];
     weight, bias, post_weight, post_bias [dim]; the parameters all float32 or all of x's type.  post 'none' | 'rms' | 'layer', pre
-    'rms' | 'layer'.  Differentiable (once) in every tensor; a call that would record or run a backward pass while its
+    'rms' | 'layer'.  Differentiable (once, in reverse mode) in every tensor; a call that would record or run a backward pass while its
     stream is being captured is refused: capture gated_norm_fwd and gated_norm_vjp."""
+    args = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
+    _no_tangent("gated_norm", *args)
     if torch.is_grad_enabled():
-        args = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
         for t in args:
             if t is not None and t.requires_grad:
                 _on_device(x, "x")
                 _not_captured()
                 return _GatedNorm.apply(dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps), *args)
-    return _norm_fwd(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps)
+    return _norm_fwd(*args, post, pre, residual_scale, eps)
 
 
 def gated_norm_fwd(x, y=None, *, gate=None, residual_scale=1.0, post="none", post_weight=None, post_bias=None, pre="layer", weight=None, bias=None,
                    scale=None, shift=None, eps=1e-5):
     """gated_norm without a backward pass -> (r, h)."""
+    _no_tangent("gated_norm_fwd", x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
     return _norm_fwd(x, y, gate, scale, shift, weight, bias, post_weight, post_bias, post, pre, residual_scale, eps)
 
 
@@ -232,7 +245,9 @@ def gated_norm_vjp(grad_r, grad_h, x, y=None, *, gate=None, residual_scale=1.0, 
     unknown = set(wanted) - set(_NORM_INPUTS)
     if unknown:
         _refuse(f"no such inputs: {sorted(unknown)}")
-    return _norm_vjp((x, y, gate, scale, shift, weight, bias, post_weight, post_bias), dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps),
+    args = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
+    _no_tangent("gated_norm_vjp", grad_r, grad_h, *args)
+    return _norm_vjp(args, dict(post=post, pre=pre, residual_scale=residual_scale, eps=eps),
                      grad_r, grad_h, wanted)
 
 

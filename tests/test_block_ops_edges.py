@@ -7,6 +7,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from conftest import PKG
 from test_block_ops import E, native, ops, within
@@ -119,3 +120,51 @@ def test_8_bit_layer_refuses_every_call_that_would_lose_a_gradient():
             call()
     for want, got in zip(o.quantize_rows(one(3, 100)), o.quantize_rows(leaf(3, 100).detach())):
         assert torch.equal(want, got)
+
+
+def test_refusal_of_a_lost_tangent():
+    o, t = ops(), torch.zeros(2)
+    with forward_ad.dual_level():
+        o._no_tangent("f", None, t)
+        with pytest.raises(native().NativeError, match="forward-mode"):
+            o._no_tangent("f", None, t, forward_ad.make_dual(t, torch.ones(2)))
+    o._no_tangent("f", None, t)
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    """A tensor with a tangent, whether it requires a gradient or not, gives no result without one."""
+    o, err = ops(), native().NativeError
+    one = lambda *s: torch.ones(*s, device="cuda")  # noqa: E731
+    half = lambda *s: one(*s).half()  # noqa: E731
+    x, w8 = one(1, 2, 64), torch.ones(5, 128, dtype=torch.int8, device="cuda")
+    a8, q, k, own = torch.ones(2, 128, dtype=torch.int8, device="cuda"), half(1, 1, 2, 64), half(4, 2, 64), half(1, 3, 2, 64)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: o.gated_norm(dual(x)), lambda: o.gated_norm(dual(one(1, 2, 64).requires_grad_())), lambda: o.gated_norm(x, dual(x)),
+                 *(lambda n=n: o.gated_norm(x, x, post="layer", **{n: dual(one(64))}) for n in o._PARAMS),
+                 lambda: o.gated_norm(one(1, 2, 64).requires_grad_(), weight=dual(one(64))),
+                 lambda: o.gated_norm_fwd(x, dual(x)), lambda: o.gated_norm_fwd(x, scale=dual(one(64))),
+                 lambda: o.gated_norm_vjp(dual(x), None, x), lambda: o.gated_norm_vjp(None, dual(x), x), lambda: o.gated_norm_vjp(x, x, dual(x)),
+                 lambda: o.gated_norm_vjp(x, x, x, x, gate=dual(one(64))),
+                 lambda: o.quantize_rows(dual(x[0])), lambda: o.gemm_i8(a8, dual(one(2)), w8, one(5)), lambda: o.gemm_i8(a8, one(2), w8, one(5), dual(one(5))),
+                 lambda: o.gemm_i8(a8, one(2), w8, one(5), epi="resid", resid=dual(one(2, 5))),
+                 lambda: o.linear_i8(dual(x[0]), w8, one(5)), lambda: o.linear_i8(x[0], w8, dual(one(5))),
+                 lambda: o.shared_prefix_attention(dual(q), k, k), lambda: o.shared_prefix_attention(q, dual(k), k),
+                 lambda: o.shared_prefix_attention(q, k, dual(k)), lambda: o.shared_prefix_attention(q, k, k, dual(own), own),
+                 lambda: o.shared_prefix_attention(q, k, k, own, dual(own))]
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for i, call in enumerate(calls):
+                    with pytest.raises(err, match="forward-mode"):
+                        call()
+                        pytest.fail(f"call {i} was accepted")
+        # tensors without a tangent are taken as outside the level
+        r, h = o.gated_norm(x, x)
+    for a, b in zip((r, h), o.gated_norm(x, x)):
+        assert torch.equal(a, b)
+    # a tangent that only the incoming gradient carries
+    leaf = torch.randn(1, 2, 64, device="cuda", requires_grad=True)
+    r, _ = o.gated_norm(leaf)
+    with forward_ad.dual_level(), pytest.raises(err, match="forward-mode"):
+        torch.autograd.grad(r, leaf, forward_ad.make_dual(x, torch.ones_like(x)))
