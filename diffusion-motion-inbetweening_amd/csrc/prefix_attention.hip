@@ -319,8 +319,8 @@ struct Rows32 {
         }
     }
     // Where rows see different keys, a value that is infinite or not a number must reach the rows that see its key and no others (0 times
-    // it is not 0): it is added to their o as it is, which no weight above zero would change, and a zero takes its place in LDS.
-    // `lim`: keys of the tile that the lane's row sees.
+    // it is not 0): it is added to their o as it is, which no weight above zero would change, and a zero takes its place in LDS.  The
+    // tile's maximum is settled before: a row's first one multiplies its o by zero.  `lim`: keys of the tile that the lane's row sees.
     __device__ __forceinline__ void odd_values(const char* vt, int keys, int lim, int hi) {
 #pragma unroll 1
         for (int key = 0; key < keys; ++key) {
@@ -510,6 +510,14 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
             const int at = it.o0 + (s - it.np) * KT, lim = (seen < it.o1 ? seen : it.o1) - at;     // (only own keys are hidden from some rows)
             char* vt = lds + vs * TILE;
             if (__builtin_expect(any_odd<T, TILE / 1024>(vt, lane), 0)) {         // all waves say the same
+                if (busy) {                                       // the maxima over both units: none moves in the loop below
+                    w.mask(sc, lim, lane);
+                    w.settle(sc);
+                    w.keys(lds + ks * TILE + 32 * ROWB, kf);
+                    w.scores(kf, nx);
+                    w.mask(nx, lim - 32, lane);
+                    w.settle(nx);
+                }
                 w.odd_values(vt, KT, lim, hi);
                 __syncthreads();
                 clear_odd<T>(vt + wave * PIECES * 1024 + lane * 16, PIECES);

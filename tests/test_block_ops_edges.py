@@ -1,5 +1,6 @@
 """Block operators (ops.py) at the edges of what their documentation allows.  Formulas, cases and tolerances: test_block_ops.py."""
 import ctypes as C
+import math
 import shutil
 import subprocess
 import sys
@@ -10,7 +11,7 @@ import torch
 from torch.autograd import forward_ad
 
 from conftest import PKG
-from test_block_ops import E, native, ops, within
+from test_block_ops import E, attention_case, native, ops, within
 
 REPO = Path(__file__).resolve().parent.parent
 
@@ -168,3 +169,36 @@ def test_forward_mode_derivatives_are_refused():
     r, _ = o.gated_norm(leaf)
     with forward_ad.dual_level(), pytest.raises(err, match="forward-mode"):
         torch.autograd.grad(r, leaf, forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,grp,p,more", [(5, 2, 0, 0), (40, 1, 0, 0), (40, 4, 0, 3), (150, 1, 0, 0), (150, 2, 0, 70), (90, 1, 100, 0), (64, 1, 64, 0)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_attention_infinite_value_stays_one(n, grp, p, more, dtype):
+    """One infinite value among causal own keys is the result of every row that sees its key, with its sign, whatever tile it lies in; rows
+    that do not see it keep their bits.  (Scores of normal draws over 64 dims: no weight is near the smallest 16-bit one.)"""
+    q, pk, pv, ok, ov, _ = attention_case(2, n, 2 * grp, 2, 64, p, n + more, dtype, seed=n + p)
+    want = ops().shared_prefix_attention(q, pk, pv, ok, ov)
+    for at in sorted({0, 1, 31, 33, 45, 70, more, n // 2, n + more - 1} & set(range(n + more))):
+        for bad in (math.inf, -math.inf, math.nan):
+            v2 = ov.clone()
+            v2[1, at, 1, 3] = bad
+            got = ops().shared_prefix_attention(q, pk, pv, ok, v2)
+            first = max(0, at - more)                                    # the first query that sees key `at`
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1, :first], want[1, :first]) and torch.equal(got[1, :, :grp], want[1, :, :grp]), (at, bad)
+            there = got[1, first:, grp:, 3].float()
+            assert (torch.isnan(there) if bad != bad else there == bad).all(), (at, bad)
+            assert torch.isfinite(got[1, first:, grp:, [d for d in range(64) if d != 3]]).all(), (at, bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [8, 100])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_attention_infinite_value_where_the_maximum_leaps(n, dtype):
+    """Prefix keys whose weights vanish beside the own ones: what was summed before is multiplied by zero, an infinity of the new keys is not."""
+    q, pk, pv, ok, ov, _ = attention_case(1, n, 1, 1, 64, 64, n, dtype, seed=n)
+    q.zero_(), pk.zero_(), ok.zero_()
+    q[..., 0], pk[..., 0] = 1, -200
+    ov[0, n // 2, 0, 5] = -math.inf
+    out = ops().shared_prefix_attention(q, pk, pv, ok, ov, scale=1.0)[0, :, 0]
+    assert torch.isfinite(out[: n // 2]).all() and (out[n // 2:, 5] == -math.inf).all() and torch.isfinite(out[:, [d for d in range(64) if d != 5]]).all()
