@@ -209,13 +209,19 @@ __device__ __forceinline__ void clear_odd(char* from, int n) {
 
 // A wave's 32 rows against 32 keys at a time.  A row's maximum is moved only when a score passes it by 2^8: until then its p stay
 // below 256, which changes no relative rounding and saves the exchange between the lanes and the rescaling of o.
+//
+// With s the raw score and c = scale log2 e, p = 2^(s c - m c) is one multiply-add and one exponential: m c, rounded to fp32, is the same
+// addend for all of a row's keys, but its rounding is a factor of p, and beyond |m c| = 2^27 one that leaves the operands' range.  So a
+// row is FAR once |m c| passes 2^16: its scores have m taken off before they are scaled (exact where p is not 0).  A far row's limit is
+// -inf, which sends every unit through the seldom taken path that does so.
+constexpr float kFar = 65536.f;
 template <class T, int DIM>
 struct Rows32 {
     static constexpr int ROWB = DIM * 2, DS = DIM / 16, DB = DIM / 32, FRAGS = 2 * DB, AHEAD = 4;
     s8 q[DS], p[2], vf[AHEAD];
     f32x16 o[DB];
-    float m, l, limit, base;              // limit: a raw score above it moves m;  base: -m, or 0 while nothing is seen
-    float scale2;
+    float m, l, limit, base;              // m: largest raw score;  limit: a raw score above it moves m;  base: -m c, 0 for far rows and unseen ones
+    float scale2;                         // c
     int krow[DS], vat[DB], vat8[DB];      // LDS offsets of the lane's fragments within a 32-key unit
 
     // `keys_at`: where the ring of K lies in LDS (in the offsets, so that every slot is within reach of an instruction's constant)
@@ -268,19 +274,37 @@ struct Rows32 {
         for (int i = 0; i < 16; ++i)
             if (mfma32_row(i, lane) >= lim) sc[i] = -INFINITY;
     }
-    __device__ __forceinline__ void settle(const f32x16& sc) {
+    // p of a row whose largest score is m: 2^((s - off) c + base)
+    struct Frame { float off, base; };
+    __device__ __forceinline__ Frame frame(float m) const {
+#pragma clang fp contract(off)                        // (the product as it was rounded, wherever it is used)
+        if (m == -INFINITY) return {0.f, 0.f};
+        return fabsf(m * scale2) >= kFar ? Frame{m, 0.f} : Frame{0.f, -m * scale2};
+    }
+    // the factor of what was summed while `from` was the largest score, now that `to` is
+    __device__ __forceinline__ float rescale(float from, float to) const {
+#pragma clang fp contract(off)
+        const Frame f = frame(from), t = frame(to);
+        return from == -INFINITY ? 0.f : from == to ? 1.f : exp2f(__builtin_fmaf(f.off - t.off, scale2, t.base - f.base));
+    }
+    // (not twice on the same scores: those of far rows are changed)
+    __device__ __forceinline__ void settle(f32x16& sc) {
         float top = fmaxf(sc[0], sc[1]);
 #pragma unroll
         for (int i = 2; i < 16; ++i) top = fmaxf(top, sc[i]);
         if (__builtin_expect(__any(top > limit), 0)) {
-            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * scale2);
-            const float k = mn == -INFINITY ? 0.f : exp2f(m - mn);
+            const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+            const float k = rescale(m, mn);
             l *= k;
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= k;
+            const Frame f = frame(mn);
+            const bool near = mn != -INFINITY && f.off == 0.f;
             m = mn;
-            limit = mn == -INFINITY ? -INFINITY : (mn + 8.f) / scale2;
-            base = mn == -INFINITY ? 0.f : -mn;
+            limit = near ? (8.f - f.base) / scale2 : -INFINITY;
+            base = f.base;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] -= f.off;
         }
     }
     // P^T as the B operand of the unit's two 16-key products, its sum into l
@@ -340,7 +364,8 @@ struct Rows32 {
         if (!r.ok) return;
         const bool some = l > 0.f || l != l;                      // a NaN sum is a result, an empty row is not
         const float inv = some ? 1.f / l : 0.f;
-        const float lse2 = some ? m + log2f(l) : -INFINITY;
+        const Frame f = frame(m);
+        const float lse2 = some ? __builtin_fmaf(f.off, scale2, log2f(l) - f.base) : -INFINITY;
         const int64_t row = ((int64_t)r.b * a.queries + r.i) * a.heads + r.h;
         if (slots == 1) {
             T* out = static_cast<T*>(a.out) + row * DIM + 4 * hi;
@@ -517,6 +542,8 @@ __device__ __forceinline__ void attend_rows(const PrefixAttnArgs& a, const Prefi
                     w.scores(kf, nx);
                     w.mask(nx, lim - 32, lane);
                     w.settle(nx);
+                    w.keys(lds + ks * TILE, kf);
+                    w.scores(kf, sc);
                 }
                 w.odd_values(vt, KT, lim, hi);
                 __syncthreads();
@@ -681,8 +708,8 @@ __device__ __forceinline__ void attend_wave(const PrefixAttnArgs& a, const Prefi
         }
         __syncthreads();
         if (wave < half) {
-            const float mo = jm[wave * 64 + l31], lo = jm[wave * 64 + 32 + l31], mt = fmaxf(w.m, mo), base = mt == -INFINITY ? 0.f : mt;
-            const float ka = exp2f(w.m - base), kb = exp2f(mo - base);
+            const float mo = jm[wave * 64 + l31], lo = jm[wave * 64 + 32 + l31], mt = fmaxf(w.m, mo);
+            const float ka = w.rescale(w.m, mt), kb = w.rescale(mo, mt);
             const float* from = jo + (wave * 32 + l31) * (DIM + 4) + 4 * hi;
 #pragma unroll
             for (int d = 0; d < DB; ++d)

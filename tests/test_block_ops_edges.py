@@ -11,7 +11,7 @@ import torch
 from torch.autograd import forward_ad
 
 from conftest import PKG
-from test_block_ops import E, attention_case, native, ops, within
+from test_block_ops import E, attention_case, half_step, native, ops, rounding, within
 
 REPO = Path(__file__).resolve().parent.parent
 
@@ -202,3 +202,32 @@ def test_attention_infinite_value_where_the_maximum_leaps(n, dtype):
     ov[0, n // 2, 0, 5] = -math.inf
     out = ops().shared_prefix_attention(q, pk, pv, ok, ov, scale=1.0)[0, :, 0]
     assert torch.isfinite(out[: n // 2]).all() and (out[n // 2:, 5] == -math.inf).all() and torch.isfinite(out[:, [d for d in range(64) if d != 5]]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(1, 1, 1, 1, 0, 130), (3, 1, 4, 2, 700, 40), (1, 70, 2, 1, 100, 70), (2, 90, 1, 1, 0, 90)], ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("dtype,top", [("f16", 60000.0), ("f16", 5000.0), ("f16", 900.0), ("bf16", 1e5), ("bf16", 1e15)])
+def test_attention_scores_of_any_finite_size(case, dtype, top):
+    """Scores far beyond what fp32 tells apart by one: a row's largest key alone remains, for finite q and k of any size.  q and k are
+    whole multiples of powers of two, the same in all dims, the products exact; the runner-up lies 1 / 64 of the largest score below it."""
+    b, n, h, hk, p, o = case
+    q, pk, pv, ok, ov, _ = attention_case(b, n, h, hk, 64, p, o, dtype, seed=7)
+    q.fill_(2.0 ** math.floor(math.log2(top)))
+    k = [t for t in (pk, ok) if t is not None]
+    g = torch.Generator().manual_seed(int(top))
+    for t in k:
+        t.copy_((torch.randint(-63, 64, (*t.shape[:-1], 1), generator=g) * 2.0 ** (math.floor(math.log2(top)) - 6)).to(t.dtype))
+    out, lse = ops().shared_prefix_attention(q, pk, pv, ok, ov, return_lse=True)
+    f = lambda t: t.double().cpu()  # noqa: E731
+    for i in range(b):
+        for t in range(n):
+            seen = o - n + t + 1
+            for j in range(h):
+                kk = torch.cat(([f(pk[:, j // (h // hk), 0])] if p else []) + [f(ok[i, :seen, j // (h // hk), 0])])
+                vv = torch.cat(([f(pv[:, j // (h // hk)])] if p else []) + [f(ov[i, :seen, j // (h // hk)])])
+                s = kk * float(q[i, t, j, 0]) * 8                        # 64 dims over their root
+                w = torch.softmax(s, 0)                              # ties share: at most 2 rounding steps of p and of the output
+                want = w @ vv
+                tol = 2 * half_step(q.dtype) * (w @ vv.abs()) + rounding(q.dtype, want)
+                assert ((f(out[i, t, j]) - want).abs() <= tol).all(), (i, t, j)
+                assert abs(float(lse[i, j, t]) - float(torch.logsumexp(s, 0))) <= 4 * E * float(s.abs().max()), (i, t, j)
