@@ -14,8 +14,10 @@
 // Matrix instructions: v_mfma_f32_32x32x16 (bf16 / f16 operands, fp32 sums; an eighth more throughput here than 16x16x32).
 // S^T = K Q^T puts a row of Q into a lane column, so maximum and sum stay in the lane but for one exchange, and S^T's accumulators
 // ARE the operand of O^T += V^T P^T: lane half h holds keys 8 i + 4 h + r of a tile, and the transposed LDS reads
-// (ds_read_b64_tr_b16) fetch V in that same order.  P is rounded to the operands' 16 bits (half a step relative, as the matrix unit
-// asks), its sum l is taken before that.
+// (ds_read_b64_tr_b16) fetch V in that same order.  P is rounded to the operands' 16 bits, as the matrix unit asks: half a step
+// relative, and in f16 a weight below 2^-14 of that by a fixed step, so that a long tail of small weights would be lost from o.  Their
+// p are therefore 2^LIFT times as large (below 2^15 with what the maximum may lag behind): the step is 2^-32 of the row's largest
+// weight.  l is summed in fp32 before the rounding.
 #include "prefix_attention.hpp"
 
 #include <algorithm>
@@ -37,6 +39,7 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 template <class T> struct Mma;
 template <> struct Mma<Bf16> {
     static constexpr unsigned short TOP = 0x7f80;     // exponent of an infinity or a NaN
+    static constexpr float LIFT = 0.f;                // p are 2^LIFT times their formula
     static __device__ __forceinline__ float up(short v) { return __uint_as_float((unsigned)(unsigned short)v << 16); }
     static __device__ __forceinline__ f32x16 mul(s8 a, s8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
@@ -45,6 +48,7 @@ template <> struct Mma<Bf16> {
 };
 template <> struct Mma<_Float16> {
     static constexpr unsigned short TOP = 0x7c00;
+    static constexpr float LIFT = 7.f;
     static __device__ __forceinline__ float up(short v) { return (float)__builtin_bit_cast(_Float16, v); }
     static __device__ __forceinline__ f32x16 mul(s8 a, s8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
@@ -220,7 +224,7 @@ struct Rows32 {
     static constexpr int ROWB = DIM * 2, DS = DIM / 16, DB = DIM / 32, FRAGS = 2 * DB, AHEAD = 4;
     s8 q[DS], p[2], vf[AHEAD];
     f32x16 o[DB];
-    float m, l, limit, base;              // m: largest raw score;  limit: a raw score above it moves m;  base: -m c, 0 for far rows and unseen ones
+    float m, l, limit, base;              // m: largest raw score;  limit: a raw score above it moves m;  base: LIFT - m c, LIFT for far rows and unseen ones
     float scale2;                         // c
     int krow[DS], vat[DB], vat8[DB];      // LDS offsets of the lane's fragments within a 32-key unit
 
@@ -230,7 +234,7 @@ struct Rows32 {
         m = -INFINITY;
         l = 0.f;
         limit = -INFINITY;
-        base = 0.f;
+        base = Mma<T>::LIFT;
         scale2 = scale * kLog2e;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -274,12 +278,13 @@ struct Rows32 {
         for (int i = 0; i < 16; ++i)
             if (mfma32_row(i, lane) >= lim) sc[i] = -INFINITY;
     }
-    // p of a row whose largest score is m: 2^((s - off) c + base)
+    // p of a row whose largest score is m: 2^((s - off) c + base), 2^LIFT of the largest one's
     struct Frame { float off, base; };
     __device__ __forceinline__ Frame frame(float m) const {
 #pragma clang fp contract(off)                        // (the product as it was rounded, wherever it is used)
-        if (m == -INFINITY) return {0.f, 0.f};
-        return fabsf(m * scale2) >= kFar ? Frame{m, 0.f} : Frame{0.f, -m * scale2};
+        const float lift = Mma<T>::LIFT;
+        if (m == -INFINITY) return {0.f, lift};
+        return fabsf(m * scale2) >= kFar ? Frame{m, lift} : Frame{0.f, lift - m * scale2};
     }
     // the factor of what was summed while `from` was the largest score, now that `to` is
     __device__ __forceinline__ float rescale(float from, float to) const {
@@ -301,7 +306,7 @@ struct Rows32 {
             const Frame f = frame(mn);
             const bool near = mn != -INFINITY && f.off == 0.f;
             m = mn;
-            limit = near ? (8.f - f.base) / scale2 : -INFINITY;
+            limit = near ? (Mma<T>::LIFT + 8.f - f.base) / scale2 : -INFINITY;
             base = f.base;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[i] -= f.off;

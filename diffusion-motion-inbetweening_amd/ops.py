@@ -391,8 +391,9 @@ def shared_prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_l
     q [batch, queries, heads, dim]; prefix_k, prefix_v [prefix, kv_heads, dim] (or None); own_k, own_v [batch, own_max, kv_heads,
     dim] (or None); own_len int32 [batch] on the device (None: own_max); bfloat16 or float16, dim 64 or 128, heads a multiple of
     kv_heads.  scale None: 1 / sqrt(dim).  -> out [batch, queries, heads, dim], with return_lse also the log-sums float32 [batch,
-    heads, queries].  A query that sees no key gives 0 and -inf.  For serving: there is no
-    backward pass."""
+    heads, queries].  A query that sees no key (or scores of -inf alone) gives 0 and -inf.  Scores, maxima and sums
+    are fp32; the softmax's weights meet the values in q's type (half a step of it relative each, in float16 also 2^-32 of the
+    query's largest).  For serving: there is no backward pass."""
     device = _on_device(q, "q")
     _no_backward("shared_prefix_attention", q, prefix_k, prefix_v, own_k, own_v)
     dtype, shape = q.dtype, q.shape

@@ -315,6 +315,9 @@ int cmdi_linear_i8(const void* d_x, int32_t dtype, int32_t m, int32_t cols, int6
  * A row that sees no key is 0 with lse -inf; keys behind a length are never read.  bf16 or f16, dim 64 or 128, heads a multiple
  * of kv_heads (head h reads key head h / (heads / kv_heads)); strides in elements, `dim` contiguous, 16-byte aligned, token
  * strides at most 2^23.  own_len: int32 [batch] on the device (taken as 0 .. own_max), or null: own_max.  scale > 0.
+ * Scores, their maximum and sums are fp32; each weight (2^x of the scores, before the division by their sum) is rounded to `dtype`: by
+ * half a step of it relative (bf16 2^-8, f16 2^-11), in f16 also by 2^-32 of the row's largest one.
+ * A row all of whose scores are -inf counts as one that sees no key.
  * d_lse fp32 [batch, heads, queries] or null: log of the softmax's sum.  d_work: cmdi_prefix_attention_workspace bytes.
  * prefix + own_max below 2^31 - 4096; batch * queries * heads below 2^31, and at most 2^24 where the keys are read in parts (the
  * workspace is not 0); batch * kv_heads * ceil(queries * heads / kv_heads / 128) at most 2^22. */

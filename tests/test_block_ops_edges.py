@@ -231,3 +231,35 @@ def test_attention_scores_of_any_finite_size(case, dtype, top):
                 tol = 2 * half_step(q.dtype) * (w @ vv.abs()) + rounding(q.dtype, want)
                 assert ((f(out[i, t, j]) - want).abs() <= tol).all(), (i, t, j)
                 assert abs(float(lse[i, j, t]) - float(torch.logsumexp(s, 0))) <= 4 * E * float(s.abs().max()), (i, t, j)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(1, 1, 0, 640), (3, 2, 1280, 64), (1, 70, 640, 0), (2, 100, 0, 256)], ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("less", [25.1, 28.3])
+def test_attention_tail_of_small_weights(case, dtype, less):
+    """One key in 32 has a score above the others' by `less` in base-2 logarithms and values of zero, so that the result is the others'
+    weights alone.  A weight is off by half a step of its type (bf16) or by 2^-32 of the largest (f16, whose smaller steps end there)."""
+    b, n, p, o = case
+    q, pk, pv, ok, ov, _ = attention_case(b, n, 2, 1, 64, p, o, dtype, seed=3)
+    q.zero_()
+    q[..., 0] = 1
+    high = torch.tensor(less).to(q.dtype)
+    for k, v in ((pk, pv), (ok, ov)):
+        if k is None:
+            continue
+        axis = k.dim() - 3
+        head = (torch.arange(k.shape[axis]) % 32 == 0).cuda().view(-1, 1, 1)
+        k.zero_()
+        k[..., 0] = torch.where(head, high.cuda(), torch.zeros((), dtype=q.dtype, device="cuda"))[..., 0]
+        v.copy_(torch.where(head, torch.zeros((), dtype=q.dtype, device="cuda"), v.abs().clamp(0.5, 4) * (1024 if dtype == "f16" else 1)))
+    out, lse = ops().shared_prefix_attention(q, pk, pv, ok, ov, causal=False, scale=math.log(2), return_lse=True)
+    keys = torch.cat([t.double().cpu() for t in ([] if pk is None else [pk]) + ([] if ok is None else [ok[0]])])[:, 0, 0]
+    for i in range(b):
+        vals = torch.cat([t.double().cpu() for t in ([] if pv is None else [pv]) + ([] if ov is None else [ov[i]])])[:, 0]
+        w = torch.softmax(keys * math.log(2), 0)
+        want = w @ vals
+        step = 2.0 ** -32 if dtype == "f16" else half_step(q.dtype) * 2.0 ** -float(high)
+        tol = step * w.max() * vals.sum(0) + 64 * E * want + rounding(q.dtype, want)
+        assert ((out[i].double().cpu() - want).abs() <= tol).all(), ((out[i].double().cpu() - want).abs() / tol).max()
+        assert (lse[i].double().cpu() - torch.logsumexp(keys * math.log(2), 0)).abs().max() <= 64 * E * less
