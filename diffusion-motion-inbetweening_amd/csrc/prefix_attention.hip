@@ -286,11 +286,11 @@ struct Rows32 {
         if (m == -INFINITY) return {0.f, lift};
         return fabsf(m * scale2) >= kFar ? Frame{m, lift} : Frame{0.f, lift - m * scale2};
     }
-    // the factor of what was summed while `from` was the largest score, now that `to` is
-    __device__ __forceinline__ float rescale(float from, float to) const {
+    // the factor of what was summed while `from` was the largest score, now that `to`'s frame is t
+    __device__ __forceinline__ float rescale(float from, const Frame& t) const {
 #pragma clang fp contract(off)
-        const Frame f = frame(from), t = frame(to);
-        return from == -INFINITY ? 0.f : from == to ? 1.f : exp2f(__builtin_fmaf(f.off - t.off, scale2, t.base - f.base));
+        const Frame f = frame(from);
+        return from == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(f.off - t.off, scale2, t.base - f.base));
     }
     // (not twice on the same scores: those of far rows are changed)
     __device__ __forceinline__ void settle(f32x16& sc) {
@@ -299,17 +299,19 @@ struct Rows32 {
         for (int i = 2; i < 16; ++i) top = fmaxf(top, sc[i]);
         if (__builtin_expect(__any(top > limit), 0)) {
             const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
-            const float k = rescale(m, mn);
+            const Frame f = frame(mn);
+            const float k = rescale(m, f);
             l *= k;
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= k;
-            const Frame f = frame(mn);
-            const bool near = mn != -INFINITY && f.off == 0.f;
             m = mn;
-            limit = near ? (Mma<T>::LIFT + 8.f - f.base) / scale2 : -INFINITY;
             base = f.base;
+            const bool far = f.off != 0.f;
+            limit = far || mn == -INFINITY ? -INFINITY : (Mma<T>::LIFT + 8.f - f.base) * __builtin_amdgcn_rcpf(scale2);
+            if (__builtin_expect(__any(far), 0)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[i] -= f.off;
+                for (int i = 0; i < 16; ++i) sc[i] -= f.off;
+            }
         }
     }
     // P^T as the B operand of the unit's two 16-key products, its sum into l
@@ -714,7 +716,8 @@ __device__ __forceinline__ void attend_wave(const PrefixAttnArgs& a, const Prefi
         __syncthreads();
         if (wave < half) {
             const float mo = jm[wave * 64 + l31], lo = jm[wave * 64 + 32 + l31], mt = fmaxf(w.m, mo);
-            const float ka = w.rescale(w.m, mt), kb = w.rescale(mo, mt);
+            const auto f = w.frame(mt);
+            const float ka = w.rescale(w.m, f), kb = w.rescale(mo, f);
             const float* from = jo + (wave * 32 + l31) * (DIM + 4) + 4 * hi;
 #pragma unroll
             for (int d = 0; d < DB; ++d)
