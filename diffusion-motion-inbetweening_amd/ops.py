@@ -282,8 +282,8 @@ def _bytes_rows(t: torch.Tensor, name: str, device: int) -> torch.Tensor:
     if t.get_device() != device:
         _elsewhere(name, t, device)
     st = t.stride()
-    if st[1] != 1 or st[0] % 16 or st[0] < t.shape[1] or t.data_ptr() % 16:
-        t = t.contiguous()
+    if st[1] != 1 or st[0] % 16 or st[0] < t.shape[1] or st[0] > 1 << 22 or t.data_ptr() % 16:
+        t = t.clone(memory_format=_CONTIGUOUS)          # (.contiguous() leaves a contiguous tensor where it is)
     return t
 
 
@@ -380,7 +380,7 @@ def _heads(t: torch.Tensor, name: str, shape, dtype, device: int, limit=1 << 62)
             fine = fine and s % 8 == 0
         if again or (fine and st[-3] <= limit):
             return t, at, st[:-1]
-        t = t.contiguous()
+        t = t.clone(memory_format=_CONTIGUOUS)          # (.contiguous() leaves a contiguous tensor where it is)
 
 
 def shared_prefix_attention(q, prefix_k, prefix_v, own_k=None, own_v=None, own_len=None, *, causal=True, scale=None, return_lse=False):

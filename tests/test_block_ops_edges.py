@@ -263,3 +263,38 @@ def test_attention_tail_of_small_weights(case, dtype, less):
         tol = step * w.max() * vals.sum(0) + 64 * E * want + rounding(q.dtype, want)
         assert ((out[i].double().cpu() - want).abs() <= tol).all(), ((out[i].double().cpu() - want).abs() / tol).max()
         assert (lse[i].double().cpu() - torch.logsumexp(keys * math.log(2), 0)).abs().max() <= 64 * E * less
+
+
+@pytest.mark.gpu
+def test_contiguous_tensors_at_any_address():
+    """Tensors that are contiguous but off the kernels' 16 bytes, or whose rows stand too far apart for them, are copied, not refused."""
+    o = ops()
+    g = torch.Generator().manual_seed(11)
+
+    def off(t, by=1):
+        """The same values, contiguous, `by` elements behind an allocation's start."""
+        room = torch.empty(t.numel() + by, dtype=t.dtype, device="cuda")
+        room[by:].copy_(t.reshape(-1))
+        moved = room[by:].view(t.shape)
+        assert moved.is_contiguous() and moved.data_ptr() % 16
+        return moved
+    for d, n, b in ((64, 3, 2), (128, 40, 1)):
+        q, pk, pv, ok, ov, lens = attention_case(b, n, 4, 2, d, 70, 50, "bf16", seed=d)
+        names = dict(q=q, pk=pk, pv=pv, ok=ok, ov=ov)
+        want = o.shared_prefix_attention(q, pk, pv, ok, ov, lens)
+        for which in (["q"], ["pk"], ["pv"], ["ok"], ["ov"], list(names)):
+            args = {k: off(v, 1 + 2 * i) if k in which else v for i, (k, v) in enumerate(names.items())}
+            assert torch.equal(o.shared_prefix_attention(args["q"], args["pk"], args["pv"], args["ok"], args["ov"], lens), want), which
+    a = torch.randint(-127, 128, (40, 256), generator=g, dtype=torch.int8).cuda()
+    w = torch.randint(-127, 128, (30, 256), generator=g, dtype=torch.int8).cuda()
+    sa, sw, x = torch.rand(40, generator=g).cuda(), torch.rand(30, generator=g).cuda(), torch.randn(40, 256, generator=g).cuda()
+    want, layer = o.gemm_i8(a, sa, w, sw), o.linear_i8(x, w, sw)
+    assert torch.equal(o.gemm_i8(off(a), off(sa), w, off(sw)), want) and torch.equal(o.gemm_i8(a, sa, off(w, 4), sw), want)
+    assert torch.equal(o.gemm_i8(off(a[:1], 3), sa[:1], off(w[:1]), sw[:1]), want[:1, :1])
+    assert torch.equal(o.linear_i8(off(x), off(w, 5), sw), layer) and torch.equal(o.linear_i8(off(x, 3)[:7], off(w, 5), off(sw)), o.linear_i8(x[:7], w, sw))
+    # rows more than 2^22 bytes apart
+    far = torch.empty(39 * ((1 << 22) + 16) + 256, dtype=torch.int8, device="cuda").as_strided((40, 256), ((1 << 22) + 16, 1))
+    far.copy_(a)
+    assert torch.equal(o.gemm_i8(far, sa, w, sw), want)
+    far[:30].copy_(w)
+    assert torch.equal(o.gemm_i8(a, sa, far[:30], sw), want) and torch.equal(o.linear_i8(x, far[:30], sw), layer)
