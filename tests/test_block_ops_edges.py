@@ -11,7 +11,7 @@ import torch
 from torch.autograd import forward_ad
 
 from conftest import PKG
-from test_block_ops import E, attention_case, half_step, native, ops, rounding, within
+from test_block_ops import E, attention_case, half_step, native, norm64, norm_case, ops, rounding, within
 
 REPO = Path(__file__).resolve().parent.parent
 
@@ -298,3 +298,28 @@ def test_contiguous_tensors_at_any_address():
     assert torch.equal(o.gemm_i8(far, sa, w, sw), want)
     far[:30].copy_(w)
     assert torch.equal(o.gemm_i8(a, sa, far[:30], sw), want) and torch.equal(o.linear_i8(x, far[:30], sw), layer)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("parts", ["gate scale shift", "scale", "shift", "scale shift", "gate shift"])
+@pytest.mark.parametrize("case", [(256, 1, 7, "f32", "f32", "rms", "layer", True), (700, 3, 40, "bf16", "bf16", "layer", "rms", True), (300, 32, 512, "f16", "f32", "none", "layer", False),
+                                  (1500, 2, 515, "bf16", "f32", "layer", "layer", True), (290, 5, 2048, "f16", "f16", "rms", "rms", True),
+                                  (2300, 1, 1025, "f32", "f32", "layer", "layer", True), (257, 2, 8200, "bf16", "bf16", "rms", "layer", True)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_gated_norm_many_short_samples_with_parameters_of_their_own(case, parts):
+    """Gradients of scale, shift and gate where a team of lanes takes whole samples, and of what all samples share beside them."""
+    b, s, d, dtype, params, post, pre, affine = case
+    t, kw, (gr, gh) = norm_case(b, s, d, dtype, params, post, pre, "sample" if "gate" in parts else "none", False, affine, seed=b)
+    g = torch.Generator().manual_seed(s)
+    for n in ("scale", "shift"):
+        if n in parts:
+            kw[n] = torch.randn(b, d, generator=g).mul(.3).to(torch.float32 if params == "f32" else t["x"].dtype).cuda()
+    val, tol = norm64(t["x"], t["y"], **kw, grad_r=gr, grad_h=gh)
+    got = ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw)
+    for n, v in got.items():
+        if v is not None:
+            within(v, val["g_" + n], tol["g_" + n] + rounding(v.dtype, val["g_" + n]), n)
+    assert sorted(n for n in got if got[n] is not None) == sorted(n[2:] for n in val if n.startswith("g_"))
+    # every gradient for itself: the same bits
+    for n in [n for n in got if got[n] is not None]:
+        assert torch.equal(ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw, wanted=(n,))[n], got[n]), n
