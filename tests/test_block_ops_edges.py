@@ -1,6 +1,7 @@
 """Block operators (ops.py) at the edges of what their documentation allows.  Formulas, cases and tolerances: test_block_ops.py."""
 import ctypes as C
 import math
+import re
 import shutil
 import subprocess
 import sys
@@ -323,3 +324,46 @@ def test_gated_norm_many_short_samples_with_parameters_of_their_own(case, parts)
     # every gradient for itself: the same bits
     for n in [n for n in got if got[n] is not None]:
         assert torch.equal(ops().gated_norm_vjp(gr, gh, t["x"], t["y"], **kw, wanted=(n,))[n], got[n]), n
+
+
+def test_attention_requests_do_not_read_a_descriptor_just_written(tmp_path):
+    """The requests to LDS are written in assembly, where the compiler does not see what they read: a descriptor or an address in scalar
+    registers that a vector instruction (a restored spill, for one) wrote needs five wait states, and M0 has no other user."""
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not Path(hipcc).exists():
+        pytest.skip("hipcc not available")
+    out = tmp_path / "attention.s"
+    run = subprocess.run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fno-gpu-rdc", "-w", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                          "--cuda-device-only", "-S", "-I", str(REPO / PKG / "csrc"), str(REPO / PKG / "csrc" / "prefix_attention.hip"), "-o", str(out)],
+                         capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr[-1500:]
+
+    def scalars(text):
+        regs = set()
+        for a, b, c in re.findall(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b", text):
+            regs |= {int(c)} if c else set(range(int(a), int(b) + 1))
+        return regs
+    behind, in_asm, requests = [], False, 0                 # (scalar registers that a vector instruction wrote, its wait states), newest last
+    for raw in out.read_text().split("\n"):
+        line = raw.strip()
+        if line.startswith((";;#ASMSTART", ";;#ASMEND")):
+            in_asm = line.startswith(";;#ASMSTART")
+            continue
+        code = line.split(";")[0].strip()
+        if not code or code.startswith("."):
+            continue
+        if code.endswith(":"):                              # (what ran before a label is taken to be what stands before it)
+            continue
+        assert in_asm or not re.search(r"\bm0\b", code), code
+        if code.startswith("buffer_"):
+            requests += in_asm
+            states = 0
+            for regs, n in reversed(behind):
+                if states >= 5:
+                    break
+                assert not regs & scalars(code), code
+                states += n
+        nop = re.match(r"s_nop (\w+)", code)
+        behind.append((scalars(code.split(None, 1)[1].split(",")[0]) if code.startswith("v_") and " " in code else set(), int(nop[1], 0) + 1 if nop else 1))
+        behind = behind[-8:]
+    assert requests >= 8 * 12
