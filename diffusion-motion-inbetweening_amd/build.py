@@ -50,8 +50,8 @@ UNITS = {
     "postprocess.hip": ["-ffp-contract=off"],
 }
 # no packed-fp32 VALU instructions (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32), which hipcc otherwise forms by itself from scalar
-# float code: some of their forms have given wrong results on this hardware now and then.  (The host pass warns that it does
-# not know the feature.)
+# float code: a precaution for the whole library, whose sums were never checked against their rarer forms (a sampling step of the
+# flagship takes 1.949 ms instead of 1.944).  The host pass warns that it does not know the feature.
 COMMON = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
           "-fno-gpu-rdc", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

@@ -17,9 +17,9 @@
 //
 // Bound by memory: forward reads x, y and writes r, h; backward reads x, y, dr', dh and writes dx, dy (r is computed again from
 // x and y, unrounded, which costs no more reads than r itself would).  A row stays in the registers of its team of lanes, so the
-// variance is taken of the centred values at no extra reads.  16 x 2048 rows of 2048 bf16: forward 95 us (5.7 TB/s, part of it from the
-// last-level cache), backward 196 us (4.1 TB/s; 60 registers a lane for a row's values and its four sums), its joins 14 us; 64 x 197
-// rows of 512 fp32: 18 us.
+// variance is taken of the centred values at no extra reads.  16 x 2048 rows of 2048 bf16: forward 95 - 100 us (5.4 - 5.7 TB/s, part of it
+// from the last-level cache), backward 193 - 208 us (3.9 - 4.2 TB/s; 60 registers a lane for a row's values and its four sums), its joins
+// 14 - 15 us; 64 x 197 rows of 512 fp32: 18 us.
 #include "gated_norm.hpp"
 
 #include <type_traits>

@@ -129,8 +129,8 @@ __device__ __forceinline__ void store_row(const GemmI8Args& p, int row, int col,
 // A step is four substeps of 32 columns; the fragments of the next substep are read while this one multiplies.  The step's one
 // barrier sits before its LAST substep: by then every wave has that substep's fragments in registers, so stage s may be
 // overwritten (requests of step s + 2 go out) and, with the wait in front of it, step s + 1 has landed and its first fragments are
-// read under the last products: the matrix pipe waits for other waves once a step, never for LDS.  8192 x 8192 x 4096: 285 - 327 us by
-// the card's clock (1.7 - 1.9 POP/s); what it leaves is the epilogue of each of the four rounds, under which no other block of the CU runs.
+// read under the last products: the matrix pipe waits for other waves once a step, never for LDS.  8192 x 8192 x 4096: 285 - 340 us by
+// the card's clock (1.6 - 1.9 POP/s); what it leaves is the epilogue of each of the four rounds, under which no other block of the CU runs.
 template <class T, int TM, int TN, int WM, int WN, int NST>
 __global__ __launch_bounds__(64 * WM * WN, TM * TN == 16 ? 1 : 2) void gemm_i8_tile_kernel(const GemmI8Args p, int tiles_m, int tiles_n) {
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;

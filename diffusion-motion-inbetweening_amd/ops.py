@@ -219,7 +219,8 @@ def gated_norm(x, y=None, *, gate=None, residual_scale=1.0, post="none", post_we
     x, y [batch, seq, dim] (float32, bfloat16 or float16; y None: no block in front); gate, scale, shift [dim] or [batch, dim];
     weight, bias, post_weight, post_bias [dim]; the parameters all float32 or all of x's type.  post 'none' | 'rms' | 'layer', pre
     'rms' | 'layer'.  Differentiable (once, in reverse mode) in every tensor; a call that would record or run a backward pass while its
-    stream is being captured is refused: capture gated_norm_fwd and gated_norm_vjp."""
+    stream is being captured is refused: the engine accumulates a leaf's gradient on the stream where an eager graph has used it, and
+    that work in the midst of a capture ends the process.  Capture gated_norm_fwd and gated_norm_vjp."""
     args = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
     _no_tangent("gated_norm", *args)
     if torch.is_grad_enabled():
